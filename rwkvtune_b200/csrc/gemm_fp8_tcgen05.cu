@@ -1,0 +1,633 @@
+// 8-bit GEMM on pairs of SMs: C[M,N] = op(A) op(B) for operands in the block format of fp8_format.cuh, one 256x256 output
+// tile per cluster of two CTAs, issued as tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale with fp32 accumulation.
+//
+// Scales.  The format's scales are powers of two, so the tensor core applies them: its instruction takes one E8M0 byte per
+// row and 32 contraction elements, and the byte of a 128-block is simply named by the four instructions that cover the
+// block.  The accumulator is never rescaled by ordinary threads (which, at 128 columns of contraction a step, would cost
+// as long as the step's products themselves).  A scale warp in each CTA gathers the bytes of four blocks (512 elements of
+// the contraction) into the 32-lane layout that tcgen05.cp copies into tensor memory.
+//
+// Operands may be K-major or MN-major; tiles of 128 x 128 have the same scale in either direction, so one packed copy of an
+// activation, a gradient or a weight serves every product it takes part in:  y = x W^T (NT), dx = dy W (NN),
+// dW = dy^T x (TN).  Every operand tile is 128 rows of 128 bytes in shared memory, whatever its direction.
+// Blocks of one row (a_rows = 1) exist for a K-major A.
+//
+// Epilogues: store bf16; add a bf16 residual; and two that put the result back into the block format without writing it in
+// 16 bits - relu(x)^2 (the forward activation that is kept for backward) and x * 2 sqrt(h) with h the kept activation (its
+// derivative).  A CTA owns 128 rows and two blocks of 128 columns, so a tile's scale is a maximum inside one CTA; a thread
+// owns a row, so the scale of a row block is a maximum inside one thread.
+//
+// Tensor memory holds two 256-column accumulators that overlap by 64 columns plus four 16-column sets of scales.  The
+// epilogue of a tile reads the shared 64 columns first and releases them; the products of the next tile start there, so
+// the overlap costs one 64-column read per tile instead of a whole drained accumulator.
+//
+// Every mbarrier wait is bounded as in gemm_tcgen05_2cta.cu: on expiry a code goes to `status`, all roles leave, the CTAs
+// meet, tensor memory is released and the kernel returns.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "fp8_format.cuh"
+#include "tensormap_cache.cuh"
+
+namespace {
+
+constexpr int TM = 128;                        // rows of C per CTA; the pair covers 256
+constexpr int TN = 256;                        // columns of C per pair
+constexpr int TK = 128;                        // contraction elements (bytes) per ring stage: one scale block
+constexpr int STAGES = 5;
+constexpr int OP_BYTES = 128 * 128;            // one operand tile of one CTA
+constexpr int STAGE_BYTES = 2 * OP_BYTES;
+constexpr int OUT_BYTES = TM * 128;            // 128 rows x 64 bf16, or x 128 packed bytes
+constexpr int SF_STAGES = 4;
+constexpr int SF_GROUP = 4;                    // scale blocks per set
+constexpr int SF_BYTES = 512 * 3;              // 128 rows of A, 256 of B, four bytes each
+constexpr int WARP_TMA = 0, WARP_MMA = 1, WARP_SCALE = 2, WARP_EPI = 3;
+constexpr int NUM_THREADS = 32 * (WARP_EPI + 4);
+constexpr int TMEM_COLS = 512, ACC1_COL = 192, SF_COL = 448, SF_COLS = 16, SF_B_OFFSET = 8;
+constexpr unsigned long long WAIT_NS = 4000000000ull;
+
+enum Epilogue { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_RELU_SQ = 2, EPI_RELU_SQ_GRAD = 3 };
+
+struct Barriers {
+  uint64_t full[STAGES];         // leader: both CTAs' operand loads have landed
+  uint64_t empty[STAGES];        // every CTA: the products that read the stage are done
+  uint64_t sf_full[SF_STAGES];   // leader: both CTAs' scale warps have written the set
+  uint64_t sf_empty[SF_STAGES];  // every CTA: the products that use the set are done
+  uint64_t acc_full[2];          // every CTA: accumulator complete
+  uint64_t acc_free;             // leader: the shared columns of the tile's accumulator have been read (eight warps)
+  uint32_t tmem_base;
+  int abort_flag;
+  uint32_t block_max[2][4];      // epilogue: maxima of the four warps, two blocks in flight
+};
+
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * OUT_BYTES + SF_STAGES * SF_BYTES + 512 + 1024;
+
+struct Args {
+  int M, N, K;
+  const uint8_t* a_exp;
+  const uint8_t* b_exp;
+  int a_rows;                    // 1 or 128
+  long long a_ld;                // a_rows = 1: exponents of one column block
+  int a_sm, a_sk, b_sn, b_sk;    // strides of the tile exponents along M / N and along the contraction
+  bf16* c;
+  const bf16* residual;
+  long long ldc, ldr;
+  int direct;                    // rows of C or of the residual do not start on 16 bytes
+  const uint8_t* h_val;          // kept activation, packed like the result
+  const uint8_t* h_exp;
+  uint8_t* q_exp;
+  long long q_ldv, q_lde;        // leading dimensions of the packed result (and of h)
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
+  uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+  return out;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.b32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ unsigned long long globaltimer_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, Barriers* bars, int* status, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long deadline = globaltimer_ns() + WAIT_NS;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 0x3ff) == 0) {
+      if (*reinterpret_cast<volatile int*>(&bars->abort_flag)) return false;
+      if (globaltimer_ns() > deadline) break;
+    }
+  }
+  *reinterpret_cast<volatile int*>(&bars->abort_flag) = 1;
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_cta(smem_u32(&bars->abort_flag), cluster_ctarank() ^ 1u)), "r"(1)
+               : "memory");
+  if (status) atomicCAS(status, 0, code);
+  return false;
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar_cluster_addr), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(map), "r"(src), "r"(x), "r"(y)
+               : "memory");
+}
+// operand tile: 128 rows of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes apart (either direction)
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// scale set: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, uint32_t acc) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
+      "}\n"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+template <bool A_MN, bool B_MN, int EPI, int Q_ROWS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ Args g) {
+  extern __shared__ unsigned char smem_dyn[];
+  const uint32_t raw = smem_u32(smem_dyn);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t out_stage = base + STAGES * STAGE_BYTES;
+  const uint32_t sf_stage = out_stage + 2 * OUT_BYTES;
+  Barriers* bars = reinterpret_cast<Barriers*>(smem_dyn + (sf_stage - raw) + SF_STAGES * SF_BYTES);
+  static_assert(sizeof(Barriers) <= 512, "room for the barriers");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();            // 0 = leader
+  const int pair = (int)blockIdx.x >> 1, n_pairs = (int)gridDim.x >> 1;
+  const int M = g.M, N = g.N;
+  const int tiles_n = (N + TN - 1) / TN, num_tiles = ((M + 2 * TM - 1) / (2 * TM)) * tiles_n;
+  const int num_kb = (g.K + TK - 1) / TK;
+  int* const status = g.status;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
+    for (int s = 0; s < SF_STAGES; ++s) { mbar_init(&bars->sf_full[s], 2); mbar_init(&bars->sf_empty[s], 1); }
+    mbar_init(&bars->acc_full[0], 1);
+    mbar_init(&bars->acc_full[1], 1);
+    mbar_init(&bars->acc_free, 8);
+    bars->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == WARP_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)),
+                 "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+
+  if (warp == WARP_TMA) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += n_pairs) {
+        const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM;
+        const int n0 = (tile % tiles_n) * TN + (int)rank * 128;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&bars->empty[stage], phase ^ 1, bars, status, 211)) { ok = false; break; }
+          if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * STAGE_BYTES);
+          const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[stage]), 0);
+          const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OP_BYTES;
+          const int k0 = kb * TK;
+          tma_load_2d_pair(sa, &map_a, full_leader, A_MN ? m0 : k0, A_MN ? k0 : m0);
+          tma_load_2d_pair(sb, &map_b, full_leader, B_MN ? n0 : k0, B_MN ? k0 : n0);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == WARP_MMA) {
+    if (lane == 0 && rank == 0) {
+      // kind::mxf8f6f4: A and B e4m3 (0), E8M0 scales (bit 23), directions, N = 256, M = 256 across the pair
+      constexpr uint32_t idesc = ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(TN >> 3) << 17) | (1u << 23) |
+                                 ((uint32_t)((2 * TM) >> 7) << 27);
+      // 32 contraction elements further: 32 bytes along a K-major row, 32 rows of an MN-major tile
+      constexpr uint32_t a_adv = (A_MN ? 32 * 128 : 32) >> 4, b_adv = (B_MN ? 32 * 128 : 32) >> 4;
+      int stage = 0, sf = 0, local = 0;
+      uint32_t phase = 0, sf_phase = 0;
+      bool ok = true;
+      for (int tile = pair; tile < num_tiles && ok; tile += n_pairs, ++local) {
+        if (local > 0 && !mbar_wait(&bars->acc_free, (local - 1) & 1, bars, status, 212)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (local & 1) * ACC1_COL;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          const uint32_t sfa = tmem_base + SF_COL + sf * SF_COLS, sfb = sfa + SF_B_OFFSET;
+          const uint32_t id = kb % SF_GROUP;
+          if (id == 0) {
+            if (!mbar_wait(&bars->sf_full[sf], sf_phase, bars, status, 213)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t src = sf_stage + sf * SF_BYTES;
+            scales_to_tmem(sfa, scale_desc(src));
+            scales_to_tmem(sfb, scale_desc(src + 512));
+            scales_to_tmem(sfb + 4, scale_desc(src + 1024));
+          }
+          if (!mbar_wait(&bars->full[stage], phase, bars, status, 214)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = base + stage * STAGE_BYTES;
+          const uint64_t adesc = operand_desc(sa), bdesc = operand_desc(sa + OP_BYTES);
+          const uint32_t desc = idesc | (id << 4) | (id << 29);
+#pragma unroll
+          for (int k = 0; k < TK / 32; ++k)
+            umma_pair(d_tmem, adesc + (uint64_t)(k * a_adv), bdesc + (uint64_t)(k * b_adv), desc, sfa, sfb, (kb | k) ? 1u : 0u);
+          umma_commit_pair(&bars->empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (id == SF_GROUP - 1 || kb == num_kb - 1) {
+            umma_commit_pair(&bars->sf_empty[sf]);
+            if (++sf == SF_STAGES) { sf = 0; sf_phase ^= 1; }
+          }
+        }
+        if (ok) umma_commit_pair(&bars->acc_full[local & 1]);
+      }
+    }
+  } else if (warp == WARP_SCALE) {
+    // Sets of scales: word r of an operand holds the bytes of rows r (128 of A, 256 of B) for four blocks of the
+    // contraction; word r goes to lane r % 32, column r / 32.
+    int sf = 0;
+    uint32_t sf_phase = 0;
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += n_pairs) {
+      const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM, n0 = (tile % tiles_n) * TN;
+      for (int kb0 = 0; kb0 < num_kb; kb0 += SF_GROUP) {
+        // lanes 0-3: A, 4-7 and 8-11: the two column blocks of B
+        uint32_t byte = 0;
+        const int which = lane >> 2, kb = kb0 + (lane & 3);
+        if (kb < num_kb) {
+          if (which == 0 && g.a_rows == 128 && m0 < M) byte = g.a_exp[(long long)(m0 >> 7) * g.a_sm + (long long)kb * g.a_sk];
+          if ((which == 1 || which == 2) && n0 + (which - 1) * 128 < N)
+            byte = g.b_exp[(long long)((n0 >> 7) + which - 1) * g.b_sn + (long long)kb * g.b_sk];
+        }
+        uint32_t rows4[4] = {0, 0, 0, 0};
+        if (!A_MN && g.a_rows == 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (kb0 + i < num_kb && m0 + 4 * lane < g.a_ld)
+              rows4[i] = __ldg(reinterpret_cast<const uint32_t*>(g.a_exp + (long long)(kb0 + i) * g.a_ld + m0 + 4 * lane));
+        }
+        if (!mbar_wait(&bars->sf_empty[sf], sf_phase ^ 1, bars, status, 215)) { ok = false; break; }
+        byte <<= 8 * (lane & 3);
+        byte |= __shfl_xor_sync(0xffffffffu, byte, 1);
+        byte |= __shfl_xor_sync(0xffffffffu, byte, 2);
+        const uint32_t wa = __shfl_sync(0xffffffffu, byte, 0), wb0 = __shfl_sync(0xffffffffu, byte, 4),
+                       wb1 = __shfl_sync(0xffffffffu, byte, 8);
+        const uint32_t dst = sf_stage + sf * SF_BYTES;
+        if (!A_MN && g.a_rows == 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {      // word of row 4 * lane + i: byte i of the four blocks
+            const uint32_t lo = __byte_perm(rows4[0], rows4[1], i | ((4 + i) << 4));
+            const uint32_t hi = __byte_perm(rows4[2], rows4[3], i | ((4 + i) << 4));
+            const int r = 4 * lane + i;
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (r & 31) * 16 + (r >> 5) * 4), "r"(__byte_perm(lo, hi, 0x5410))
+                         : "memory");
+          }
+        } else {
+          st_shared16(dst + lane * 16, make_uint4(wa, wa, wa, wa));
+        }
+        st_shared16(dst + 512 + lane * 16, make_uint4(wb0, wb0, wb0, wb0));
+        st_shared16(dst + 1024 + lane * 16, make_uint4(wb1, wb1, wb1, wb1));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->sf_full[sf]), 0));
+        if (++sf == SF_STAGES) { sf = 0; sf_phase ^= 1; }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;                 // tensor-memory lanes [32q, 32q + 32)
+    const int row = quarter * 32 + lane;          // row of this CTA's 128 owned by this thread
+    const bool elected = threadIdx.x == 32 * WARP_EPI;
+    int local = 0, buf = 0;
+    for (int tile = pair; tile < num_tiles; tile += n_pairs, ++local) {
+      const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM, n0 = (tile % tiles_n) * TN;
+      const int gm = m0 + row;
+      const int acc = local & 1;
+      mbar_wait(&bars->acc_full[acc], (local >> 1) & 1, bars, status, 216);
+      epi_sync();
+      if (*reinterpret_cast<volatile int*>(&bars->abort_flag)) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * ACC1_COL;
+      const uint32_t free_leader = map_to_cta(smem_u32(&bars->acc_free), 0);
+      if constexpr (EPI == EPI_STORE || EPI == EPI_RESIDUAL) {
+#pragma unroll 1
+        for (int i = 0; i < TN / 64; ++i) {
+          const int chunk = acc == 0 ? TN / 64 - 1 - i : i;      // the columns shared with the other accumulator first
+          const int gn0 = n0 + chunk * 64;
+          uint32_t v[64];
+          tmem_ld32(t_row + chunk * 64, v);
+          tmem_ld32(t_row + chunk * 64 + 32, v + 32);
+          uint4 cin[EPI == EPI_RESIDUAL ? 8 : 1];
+          if (EPI == EPI_RESIDUAL) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              cin[j] = make_uint4(0u, 0u, 0u, 0u);
+              if (gm < M && gn0 + j * 8 < N) {
+                const bf16* p = g.residual + (long long)gm * g.ldr + gn0 + j * 8;
+                if (!g.direct) {
+                  cin[j] = __ldcs(reinterpret_cast<const uint4*>(p));
+                } else {
+                  float t[8];
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) t[e] = gn0 + j * 8 + e < N ? __bfloat162float(p[e]) : 0.f;
+                  cin[j] = pack8(t);
+                }
+              }
+            }
+          }
+          tmem_wait_ld();
+          if (i == 0) {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_cluster(free_leader);
+          }
+          if (elected) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          epi_sync();
+          const uint32_t stage_addr = out_stage + buf * OUT_BYTES;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float f[8], prev[8];
+            if (EPI == EPI_RESIDUAL) unpack8(cin[j], prev);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j * 8 + e]) + (EPI == EPI_RESIDUAL ? prev[e] : 0.f);
+            st_shared16(stage_addr + row * 128 + ((j ^ (row & 7)) << 4), pack8(f));
+          }
+          if (!g.direct) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            epi_sync();
+            if (elected && m0 < M) {
+              tma_store_2d(&map_out, stage_addr, gn0, m0);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {                                                // unaligned rows: copied out value by value
+            epi_sync();
+            for (int r = quarter; r < TM && m0 + r < M; r += 4)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int col = lane + h * 32;
+                uint16_t val;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(val)
+                             : "r"(stage_addr + r * 128 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2));
+                if (gn0 + col < N) reinterpret_cast<uint16_t*>(g.c)[(long long)(m0 + r) * g.ldc + gn0 + col] = val;
+              }
+          }
+          buf ^= 1;
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int half = acc == 0 ? 1 - i : i;
+          const int gn0 = n0 + half * 128, nb = gn0 >> 7;
+          uint32_t v[128];
+          uint4 hv[EPI == EPI_RELU_SQ_GRAD ? 8 : 1];
+          uint32_t he = 0;
+          if (EPI == EPI_RELU_SQ_GRAD) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              hv[j] = gm < M && gn0 + j * 16 < g.q_ldv
+                          ? __ldcs(reinterpret_cast<const uint4*>(g.h_val + (long long)gm * g.q_ldv + gn0 + j * 16))
+                          : make_uint4(0u, 0u, 0u, 0u);
+            if (gm < M && gn0 < N)
+              he = Q_ROWS == 1 ? g.h_exp[(long long)nb * g.q_lde + gm] : g.h_exp[(long long)(m0 >> 7) * g.q_lde + nb];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tmem_ld32(t_row + half * 128 + j * 32, v + j * 32);
+          tmem_wait_ld();
+          if (i == 0) {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_cluster(free_leader);
+          }
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float h[16];
+            if (EPI == EPI_RELU_SQ_GRAD) {
+              fp8_unpack4(hv[j].x, h); fp8_unpack4(hv[j].y, h + 4); fp8_unpack4(hv[j].z, h + 8); fp8_unpack4(hv[j].w, h + 12);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float x = __uint_as_float(v[j * 16 + e]);
+              if (EPI == EPI_RELU_SQ) {
+                x = x < 0.f ? 0.f : x;             // a NaN stays one
+                x *= x;
+              } else {
+                x *= 2.f * sqrtf(fp8_scaled(h[e], he));
+              }
+              if (gm >= M || gn0 + j * 16 + e >= N) x = 0.f;
+              v[j * 16 + e] = __float_as_uint(x);
+              top = max(top, __float_as_uint(x) & 0x7fffffffu);
+            }
+          }
+          if (Q_ROWS == 128) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0) bars->block_max[buf][quarter] = top;
+          }
+          if (elected) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          epi_sync();
+          if (Q_ROWS == 128)
+            top = max(max(bars->block_max[buf][0], bars->block_max[buf][1]), max(bars->block_max[buf][2], bars->block_max[buf][3]));
+          const uint32_t e = fp8_block_exponent(top);
+          const float s = fp8_inverse_scale(e == 255u ? 127u : e);
+          const uint32_t stage_addr = out_stage + buf * OUT_BYTES;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const uint32_t* p = v + j * 16 + t * 4;
+              w[t] = e == 255u ? 0x7f7f7f7fu
+                               : fp8_pack4(__uint_as_float(p[0]) * s, __uint_as_float(p[1]) * s, __uint_as_float(p[2]) * s,
+                                           __uint_as_float(p[3]) * s);
+            }
+            st_shared16(stage_addr + row * 128 + ((j ^ (row & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          epi_sync();
+          if (m0 < M && gn0 < N) {
+            if (elected) {
+              tma_store_2d(&map_out, stage_addr, gn0, m0);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              if (Q_ROWS == 128) g.q_exp[(long long)(m0 >> 7) * g.q_lde + nb] = (uint8_t)e;
+            }
+            if (Q_ROWS == 1 && gm < M) g.q_exp[(long long)nb * g.q_lde + gm] = (uint8_t)e;
+          }
+          buf ^= 1;
+        }
+      }
+    }
+    if (elected) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();            // neither CTA leaves (or frees tensor memory) while the other may still signal or read it
+  if (warp == WARP_MMA) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS));
+  }
+}
+
+// Tensor map over [rows, cols] of 1- or 2-byte elements, box of 128 rows x 128 bytes, 128-byte swizzle.
+int encode(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* ptr, long long rows, long long cols, long long ld) {
+  if (((uintptr_t)ptr & 15) || (ld * elem) % 16) return RWKV_ERR_BAD_ALIGNMENT;
+  rwkv_tmap::EncodeTiledFn enc = rwkv_tmap::get_encode();
+  if (!enc) return RWKV_ERR_NOT_INITIALISED;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * elem)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / elem), 128}, estr[2] = {1, 1};
+  CUresult r = CUDA_SUCCESS;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    r = enc(map, type, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_ERROR_INVALID_CONTEXT) break;
+    cudaFree(nullptr);       // a thread without CUDA work so far (an autograd worker): binds the device's context
+  }
+  return r == CUDA_SUCCESS ? RWKV_OK : RWKV_ERR_CUDA_BASE + 900 + (int)r;
+}
+
+template <bool A_MN, bool B_MN, int EPI, int Q_ROWS>
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Args& g, cudaStream_t st) {
+  auto kern = gemm_fp8_kernel<A_MN, B_MN, EPI, Q_ROWS>;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return RWKV_ERR_CUDA_BASE + (int)e;
+  static std::atomic<unsigned long long> configured{0};          // devices whose copy of the kernel may use the memory
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (e != cudaSuccess) return RWKV_ERR_CUDA_BASE + (int)e;
+    configured.fetch_or(bit);
+  }
+  const long long tiles = (long long)((g.M + 2 * TM - 1) / (2 * TM)) * ((g.N + TN - 1) / TN);
+  if (tiles > 0x3fffffff) return RWKV_ERR_TOO_LARGE;
+  const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
+  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, st>>>(ma, mb, mo, g);
+  return rwkv_launch_status();
+}
+
+inline int up(int n, int m) { return (n + m - 1) / m * m; }
+
+}  // namespace
+
+// C[M,N] = op(A) op(B) of packed operands (fp8_format.cuh).
+//   a_mn = 0: A is [M,K], a_rows 1 or 128;  a_mn = 1: A is stored [K,M], a_rows 128
+//   b_mn = 0: B is [N,K];  b_mn = 1: B is stored [K,N]; both in tiles
+//   epilogue 0: c = bf16 result (row stride ldc);  1: c = result + residual (bf16, row stride ldr)
+//            2: (q_val, q_exp) = packed relu(result)^2, NT only;  3: = packed result * 2 sqrt(h), NN only;
+//            the packed result and h are [M,N] with blocks of q_rows rows
+//   status: device int, set non-zero if a device-side wait expired
+RWKV_EXPORT int rwkv_gemm_fp8_tcgen05(const void* a_val, const void* a_exp, int a_rows, const void* b_val, const void* b_exp,
+                                      int M, int N, int K, int a_mn, int b_mn, int epilogue, void* c, long long ldc,
+                                      const void* residual, long long ldr, const void* h_val, const void* h_exp, void* q_val,
+                                      void* q_exp, int q_rows, void* status, void* stream) {
+  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7ffffe00 || N > 0x7ffffe00 || K > 0x7ffffe00) return RWKV_ERR_BAD_SHAPE;
+  if (!(a_rows == 128 || (a_rows == 1 && !a_mn)) || epilogue < 0 || epilogue > 3) return RWKV_ERR_BAD_SHAPE;
+  if (epilogue <= 1 ? (!c || ldc < N || (epilogue == 1 && (!residual || ldr < N)))
+                    : (!q_val || !q_exp || !(q_rows == 1 || q_rows == 128) || (epilogue == 3 && (!h_val || !h_exp)) ||
+                       ((uintptr_t)h_val & 15)))
+    return RWKV_ERR_BAD_SHAPE;
+  CUtensorMap ma, mb, mo;
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  int r = a_mn ? encode(&ma, u8, 1, a_val, K, M, up(M, 16)) : encode(&ma, u8, 1, a_val, M, K, up(K, 16));
+  if (r) return r;
+  r = b_mn ? encode(&mb, u8, 1, b_val, K, N, up(N, 16)) : encode(&mb, u8, 1, b_val, N, K, up(K, 16));
+  if (r) return r;
+  Args g = {};
+  g.M = M; g.N = N; g.K = K;
+  g.a_exp = (const uint8_t*)a_exp; g.b_exp = (const uint8_t*)b_exp;
+  g.a_rows = a_rows;
+  g.a_ld = up(M, 16);
+  const int mb_n = up(M, 128) / 128, nb_n = up(N, 128) / 128, kb_n = up(K, 128) / 128;
+  g.a_sm = a_mn ? 1 : kb_n; g.a_sk = a_mn ? mb_n : 1;
+  g.b_sn = b_mn ? 1 : kb_n; g.b_sk = b_mn ? nb_n : 1;
+  g.c = (bf16*)c; g.residual = (const bf16*)residual; g.ldc = ldc; g.ldr = ldr;
+  g.h_val = (const uint8_t*)h_val; g.h_exp = (const uint8_t*)h_exp; g.q_exp = (uint8_t*)q_exp;
+  g.q_ldv = up(N, 16);
+  g.q_lde = q_rows == 1 ? up(M, 16) : nb_n;
+  g.status = (int*)status;
+  if (epilogue <= 1) {
+    g.direct = ((uintptr_t)c & 15) || (ldc & 7) || (epilogue == 1 && (((uintptr_t)residual & 15) || (ldr & 7) || (N & 7)));
+    if (g.direct) {
+      mo = ma;               // never read
+    } else {
+      r = encode(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c, M, N, ldc);
+    }
+  } else {
+    r = encode(&mo, u8, 1, q_val, M, N, g.q_ldv);
+  }
+  if (r) return r;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (epilogue == 2) {
+    if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
+    return q_rows == 1 ? launch<false, false, EPI_RELU_SQ, 1>(ma, mb, mo, g, st) : launch<false, false, EPI_RELU_SQ, 128>(ma, mb, mo, g, st);
+  }
+  if (epilogue == 3) {
+    if (a_mn || !b_mn) return RWKV_ERR_BAD_SHAPE;
+    return q_rows == 1 ? launch<false, true, EPI_RELU_SQ_GRAD, 1>(ma, mb, mo, g, st)
+                       : launch<false, true, EPI_RELU_SQ_GRAD, 128>(ma, mb, mo, g, st);
+  }
+  if (epilogue == 1) {
+    if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
+    return launch<false, false, EPI_RESIDUAL, 0>(ma, mb, mo, g, st);
+  }
+  if (a_mn && b_mn) return launch<true, true, EPI_STORE, 0>(ma, mb, mo, g, st);
+  if (a_mn) return RWKV_ERR_BAD_SHAPE;
+  return b_mn ? launch<false, true, EPI_STORE, 0>(ma, mb, mo, g, st) : launch<false, false, EPI_STORE, 0>(ma, mb, mo, g, st);
+}

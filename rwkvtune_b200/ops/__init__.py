@@ -157,6 +157,10 @@ def linear_relu_sq(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     return reference.relu_squared(torch.nn.functional.linear(x, weight))
 
 
+# ------------------------------------------------------------------------------- 8-bit blocks
+from .fp8 import Fp8Blocks, fp8_channel_mix_ffn, fp8_linear, pack_fp8, unpack_fp8  # noqa: E402
+
+
 # ------------------------------------------------------------------------------- fused element-wise
 def layer_norm(x, weight, bias, eps: float = LAYERNORM_EPS):
     if _native(x, "layer_norm"):

@@ -180,3 +180,42 @@ def adamw_step(p32, g, m, v, lr: float, beta1: float, beta2: float, eps: float, 
     denom = (v / bc2).sqrt_().add_(eps)
     p32.mul_(1 - lr * weight_decay).addcdiv_(m, denom, value=-lr / bc1)
     return p32
+
+
+# --------------------------------------------------------------------------- 8-bit blocks
+FP8_BLOCK = 128
+
+
+def fp8_exponents(largest: torch.Tensor) -> torch.Tensor:
+    """Exponent byte of blocks whose largest magnitudes are ``largest`` (fp32): the smallest ``E >= 0`` with
+    ``largest <= 448 * 2^(E - 127)``, 255 where it is not finite."""
+    bits = largest.float().abs().contiguous().view(torch.int32)
+    e = (bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000).int()
+    return torch.where(bits >= 0x7F800000, 255, e.clamp(min=0)).to(torch.uint8)
+
+
+def _fp8_scale(exponents: torch.Tensor) -> torch.Tensor:
+    return torch.ldexp(torch.ones_like(exponents, dtype=torch.float64), exponents.int() - 127)
+
+
+def fp8_pack(x: torch.Tensor, rows: int):
+    """``(values float8_e4m3fn [R, C], exponents uint8 [ceil(R / rows), ceil(C / 128)])`` of a matrix, in blocks of ``rows``
+    (1 or 128) by 128: ``x ~ values * 2^(exponents - 127)``, rounded to nearest even.  A block that holds an infinity or a
+    NaN becomes NaN."""
+    R, C = x.shape
+    padded = F.pad(x.float(), (0, -C % FP8_BLOCK, 0, -R % rows))
+    blocks = padded.unflatten(1, (-1, FP8_BLOCK)).unflatten(0, (-1, rows))             # [R / rows, rows, C / 128, 128]
+    bits = (blocks.contiguous().view(torch.int32) & 0x7FFFFFFF).amax(dim=(1, 3))       # a NaN is larger than infinity here
+    e = fp8_exponents(bits.view(torch.float32))
+    v = blocks.double() / _fp8_scale(e)[:, None, :, None]
+    v = torch.where((e == 255)[:, None, :, None], torch.nan, v).float()
+    return v.flatten(2).flatten(0, 1)[:R, :C].to(torch.float8_e4m3fn), e
+
+
+def fp8_unpack(values: torch.Tensor, exponents: torch.Tensor, rows: int) -> torch.Tensor:
+    """The fp32 values that a packed matrix stands for (finite inputs stay finite: a value that the rounding lifted above
+    the largest number is that number)."""
+    R, C = values.shape
+    e = exponents.repeat_interleave(rows, 0)[:R].repeat_interleave(FP8_BLOCK, 1)[:, :C]
+    top = torch.finfo(torch.float32).max
+    return (values.double() * _fp8_scale(e)).clamp(-top, top).float()

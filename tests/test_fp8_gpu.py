@@ -1,0 +1,303 @@
+"""8-bit block kernels: packing bit for bit against the CPU statement, products against 64-bit products of the packed
+operands, gradients through the public entry points."""
+import math
+
+import pytest
+import torch
+
+from rwkvtune_b200 import ops
+from rwkvtune_b200.ops import fp8, gemm_native
+from rwkvtune_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def no_expired_wait():
+    yield
+    torch.cuda.synchronize()
+    assert gemm_native.check_status() == 0
+
+
+def sample(R, C, dtype=BF, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, C, generator=g) * torch.exp(2 * torch.randn(R, 1, generator=g))
+    x[:, ::37] *= 50
+    return x.clamp(-6e4, 6e4).to(dtype)
+
+
+def weights(N, K, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return ((torch.rand(N, K, generator=g) - 0.5) * 2 / math.sqrt(K)).to(BF)
+
+
+def same_bits(p, x, rows):
+    values, exponents = ref.fp8_pack(x.cpu(), rows)
+    assert torch.equal(p.exponents.cpu(), exponents)
+    got, want = p.values.cpu().view(torch.uint8), values.view(torch.uint8)
+    nan = exponents.repeat_interleave(rows, 0)[:x.shape[0]].repeat_interleave(128, 1)[:, :x.shape[1]] == 255
+    assert torch.equal(got[~nan], want[~nan]) and (got[nan] & 0x7F == 0x7F).all()
+
+
+# ------------------------------------------------------------------------------- packing
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, torch.float16, torch.float32])
+@pytest.mark.parametrize("R,C", [(1, 1), (1, 2048), (5, 130), (128, 128), (130, 257), (300, 1000), (129, 90)])
+def test_pack_and_unpack(R, C, dtype, rows):
+    x = sample(R, C, dtype).cuda()
+    p = ops.pack_fp8(x, rows=rows)
+    same_bits(p, x, rows)
+    for out in (BF, torch.float16, torch.float32):
+        want = ops.unpack_fp8(p.to("cpu"), out)
+        assert torch.equal(ops.unpack_fp8(p, out).cpu(), want)
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_pack_of_strided_and_unaligned_inputs(rows, dtype):
+    base = sample(140, 410, dtype).cuda()
+    for x in (base[:, 1:301], base[3:, 8:264], base[::2, 2:200], base.t(), base[:1, 5:9], base[:, ::2],
+              base[0].expand(140, 410), base.view(-1)[1:1 + 139 * 410].view(139, 410)):
+        same_bits(ops.pack_fp8(x, rows=rows), x.contiguous(), rows)
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+def test_pack_of_non_finite_zero_and_extreme_blocks(rows):
+    x = sample(260, 400, torch.float32)
+    x[5, 140], x[200, 3], x[130, 399] = math.nan, math.inf, -math.inf
+    x[128:256, 128:256] = 0
+    x[256:, :128] = 3.4e38
+    x[256:, 128:256] = 2.0 ** -120
+    x = x.cuda()
+    p = ops.pack_fp8(x, rows=rows)
+    same_bits(p, x, rows)
+    y = ops.unpack_fp8(p)
+    torch.testing.assert_close(y.cpu(), ops.unpack_fp8(p.to("cpu")), rtol=0, atol=0, equal_nan=True)
+    assert torch.isfinite(y[256:, :256]).all()
+
+
+# ------------------------------------------------------------------------------- products
+def values64(p):
+    return ops.unpack_fp8(p, torch.float32).double()
+
+
+def near(got, want, magnitude, n):
+    """One rounding to bf16 (half a step: 2^-8 of the value) on top of fp32 sums: an instruction adds 32 products and the
+    running sum with an error of at most 2^-22 of the largest magnitude that occurs, n / 32 instructions one after another."""
+    assert got.shape == want.shape and got.dtype == BF
+    tol = 2.0 ** -8 * want.abs() + (n / 32 + 1) * 2.0 ** -22 * magnitude + 1e-38
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, first at {bad.nonzero()[0].tolist()}: " \
+                          f"{got[bad][0].item()} for {want[bad][0].item()}"
+
+
+SIZES = [(128, 128, 128), (256, 256, 256), (1, 128, 128), (300, 520, 384), (5, 24, 40), (257, 130, 1000), (1000, 523, 129),
+         (64, 2048, 640), (700, 1024, 2048)]
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("rows", [1, 128])
+def test_nt(M, N, K, rows):
+    a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda())
+    A, B = values64(a), values64(b)
+    near(fp8._mm_nt(a, b, BF), A @ B.t(), A.abs() @ B.abs().t(), K)
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("rows", [1, 128])
+def test_nt_residual(M, N, K, rows):
+    a, b, c = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda()), sample(M, N, seed=7).cuda()
+    A, B = values64(a), values64(b)
+    near(fp8._mm_nt(a, b, BF, c), c.double() + A @ B.t(), A.abs() @ B.abs().t() + c.double().abs(), K)
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("rows", [1, 128])
+def test_nn(M, N, K, rows):
+    a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(K, N).cuda())
+    A, B = values64(a), values64(b)
+    near(fp8._mm_nn(a, b, BF), A @ B, A.abs() @ B.abs(), K)
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_tn(M, N, K):
+    a, b = ops.pack_fp8(sample(K, M).cuda()), ops.pack_fp8(sample(K, N, seed=5).cuda())
+    A, B = values64(a), values64(b)
+    near(fp8._mm_tn(a, b, BF), A.t() @ B, A.abs().t() @ B.abs(), K)
+
+
+def packed_near(q, want, magnitude, n, rows):
+    """A packed result: each value within half an e4m3 step (2^-4 of it, or 2^-10 of its block's unit) of the 64-bit one,
+    plus the fp32 sums' own error; scales as the definition gives them from the 64-bit values."""
+    tol_sum = (n / 32 + 1) * 2.0 ** -22 * magnitude
+    top = torch.nn.functional.pad(want.abs(), (0, -want.shape[1] % 128, 0, -want.shape[0] % rows))
+    top = top.unflatten(1, (-1, 128)).unflatten(0, (-1, rows)).amax(dim=(1, 3))
+    assert torch.equal(q.exponents, ref.fp8_exponents(top.float()))
+    unit = torch.exp2(q.exponents.double() - 127).repeat_interleave(rows, 0)[:q.R].repeat_interleave(128, 1)[:, :q.C]
+    tol = 2.0 ** -4 * want.abs() + 2.0 ** -10 * unit + 2 * tol_sum + 1e-38
+    assert ((values64(q) - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("rows", [1, 128])
+def test_relu_sq_packed(M, N, K, rows):
+    a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda())
+    A, B = values64(a), values64(b)
+    pre, mag = A @ B.t(), A.abs() @ B.abs().t()
+    packed_near(fp8._hidden(a, b, rows), torch.relu(pre) ** 2, 2 * pre.abs() * mag + 1e-30, K, rows)
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("rows", [1, 128])
+def test_relu_sq_grad_packed(M, N, K, rows):
+    d, w = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(K, N).cuda())
+    h = ops.pack_fp8((torch.relu(sample(M, N, seed=3).float()) ** 2).to(BF).cuda(), rows=rows)
+    D, W, slope = values64(d), values64(w), 2 * values64(h).sqrt()
+    packed_near(fp8._hidden_grad(d, w, h), (D @ W) * slope, (D.abs() @ W.abs()) * slope + 1e-30, K + 64, rows)
+
+
+def test_long_contraction_and_many_tiles():
+    """More tiles than SM pairs, more scale sets than the ring holds, 8-bit scales that differ from block to block."""
+    M, N, K = 2600, 2100, 5000
+    for rows in (1, 128):
+        a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda())
+        A, B = values64(a), values64(b)
+        near(fp8._mm_nt(a, b, BF), A @ B.t(), A.abs() @ B.abs().t(), K)
+        q = fp8._hidden(a, b, rows)
+        pre = A @ B.t()
+        packed_near(q, torch.relu(pre) ** 2, 2 * pre.abs() * (A.abs() @ B.abs().t()) + 1e-30, K, rows)
+    b = ops.pack_fp8(weights(M, N, 4).cuda())
+    a = ops.pack_fp8(sample(M, K).cuda())
+    A, B = values64(a), values64(b)
+    near(fp8._mm_tn(a, b, BF), A.t() @ B, A.abs().t() @ B.abs(), M)
+
+
+def test_non_finite_blocks_reach_exactly_their_products():
+    x, w = sample(300, 256), weights(64, 256)
+    x[140, 3] = math.inf
+    y = ops.fp8_linear(x.cuda(), ops.pack_fp8(w.cuda()))
+    assert y[140].isnan().all() and torch.isfinite(torch.cat([y[:140], y[141:]])).all()
+    y = ops.fp8_linear(x.cuda(), w.cuda())
+    assert y[128:256].isnan().all() and torch.isfinite(torch.cat([y[:128], y[256:]])).all()
+    out = ops.fp8_channel_mix_ffn(x.cuda(), w.cuda(), weights(256, 64).cuda(), x.cuda().nan_to_num(0, 0, 0))
+    assert out[128:256].isnan().all() and torch.isfinite(out[256:]).all()
+    out = ops.fp8_channel_mix_ffn(x.cuda(), ops.pack_fp8(w.cuda()), ops.pack_fp8(weights(256, 64).cuda()),
+                                  x.cuda().nan_to_num(0, 0, 0))
+    assert out[140].isnan().all() and torch.isfinite(torch.cat([out[:140], out[141:]])).all()
+
+
+# ------------------------------------------------------------------------------- through the public entry points
+@pytest.mark.parametrize("shape,N", [((1, 64), 128), ((2, 3, 200), 90), ((40, 17, 384), 523)])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_linear_autograd(shape, N, frozen):
+    K, M = shape[-1], math.prod(shape[:-1])
+    rows = 1 if frozen else 128
+    x = sample(M, K).view(shape).cuda().requires_grad_()
+    w, dy = weights(N, K).cuda(), sample(M, N, seed=9).cuda()
+    X, W, D = values64(ops.pack_fp8(x.detach().view(M, K), rows)), values64(ops.pack_fp8(w)), values64(ops.pack_fp8(dy, rows))
+    y = ops.fp8_linear(x, ops.pack_fp8(w) if frozen else w.requires_grad_())
+    assert y.shape == shape[:-1] + (N,) and y.is_contiguous()
+    y.backward(dy.view(y.shape))
+    near(y.view(M, N), X @ W.t(), X.abs() @ W.abs().t(), K)
+    near(x.grad.view(M, K), D @ W, D.abs() @ W.abs(), N)
+    if not frozen:
+        near(w.grad, D.t() @ X, D.abs().t() @ X.abs(), M)
+
+
+@pytest.mark.parametrize("M,C,H", [(1, 64, 256), (130, 192, 768), (1111, 256, 1000)])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_channel_mix_autograd(M, C, H, frozen):
+    rows = 1 if frozen else 128
+    x, res = sample(M, C).cuda().requires_grad_(), sample(M, C, seed=2).cuda().requires_grad_()
+    wk, wv, dy = weights(H, C).cuda(), weights(C, H, 3).cuda(), sample(M, C, seed=9).cuda()
+    x8, k8, v8, d8 = ops.pack_fp8(x, rows), ops.pack_fp8(wk), ops.pack_fp8(wv), ops.pack_fp8(dy, rows)
+    h8 = fp8._hidden(x8, k8, rows)                # these two are compared with their 64-bit values above
+    p8 = fp8._hidden_grad(d8, v8, h8)
+    X, K, V, D, Hd, P = (values64(t) for t in (x8, k8, v8, d8, h8, p8))
+    args = (k8, v8) if frozen else (wk.requires_grad_(), wv.requires_grad_())
+    y = ops.fp8_channel_mix_ffn(x, *args, res)
+    y.backward(dy)
+    near(y, res.double() + Hd @ V.t(), Hd.abs() @ V.abs().t() + res.double().abs(), H)
+    near(x.grad, P @ K, P.abs() @ K.abs(), H)
+    assert torch.equal(res.grad, dy)
+    if not frozen:
+        near(wk.grad, P.t() @ X, P.abs().t() @ X.abs(), M)
+        near(wv.grad, D.t() @ Hd, D.abs().t() @ Hd.abs(), M)
+
+
+def test_frozen_rows_do_not_depend_on_the_batch():
+    w8 = ops.pack_fp8(weights(384, 640).cuda())
+    k8, v8 = ops.pack_fp8(weights(512, 640, 5).cuda()), ops.pack_fp8(weights(640, 512, 6).cuda())
+    x, res = sample(300, 640).cuda(), sample(300, 640, seed=8).cuda()
+    for f in (lambda a, r: ops.fp8_linear(a, w8), lambda a, r: ops.fp8_channel_mix_ffn(a, k8, v8, r)):
+        whole = f(x, res)
+        for i in (0, 1, 127, 128, 255, 299):
+            assert torch.equal(f(x[i:i + 1], res[i:i + 1]), whole[i:i + 1])
+
+
+def test_same_bits_twice_and_on_other_streams():
+    x, w = sample(900, 512).cuda().requires_grad_(), weights(700, 512).cuda().requires_grad_()
+    dy = sample(900, 700, seed=4).cuda()
+
+    def run():
+        y = ops.fp8_linear(x, w)
+        return (y.detach(), *torch.autograd.grad(y, [x, w], dy))
+
+    first = run()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    results = []
+    for s in streams * 3:
+        with torch.cuda.stream(s):
+            results.append(run())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(a, b) for a, b in zip(first, r))
+
+
+def test_captured_and_replayed():
+    k8, v8 = ops.pack_fp8(weights(512, 256).cuda()), ops.pack_fp8(weights(256, 512, 2).cuda())
+    x, res = torch.zeros(70, 256, dtype=BF, device="cuda"), torch.zeros(70, 256, dtype=BF, device="cuda")
+    with torch.no_grad():
+        ops.fp8_channel_mix_ffn(x, k8, v8, res)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.fp8_channel_mix_ffn(x, k8, v8, res)
+        for seed in (1, 2):
+            x.copy_(sample(70, 256, seed=seed)), res.copy_(sample(70, 256, seed=seed + 10))
+            graph.replay()
+            assert torch.equal(out, ops.fp8_channel_mix_ffn(x, k8, v8, res))
+
+
+def test_broadcast_gradients():
+    x, w = sample(140, 128).cuda().requires_grad_(), weights(96, 128).cuda().requires_grad_()
+    ops.fp8_linear(x, w).sum().backward()
+    D, X, W = torch.ones(140, 96, dtype=torch.float64, device="cuda"), values64(ops.pack_fp8(x)), values64(ops.pack_fp8(w))
+    near(x.grad, D @ W, D @ W.abs(), 96)
+    near(w.grad, D.t() @ X, D.t() @ X.abs(), 140)
+
+
+def test_empty_batches():
+    w = weights(48, 96).cuda().requires_grad_()
+    x = torch.empty(2, 0, 96, dtype=BF, device="cuda", requires_grad=True)
+    y = ops.fp8_linear(x, w)
+    y.sum().backward()
+    assert y.shape == (2, 0, 48) and y.dtype == BF and x.grad.shape == x.shape and not w.grad.any()
+    wk, wv = ops.pack_fp8(weights(64, 96).cuda()), ops.pack_fp8(weights(96, 64).cuda())
+    assert ops.fp8_channel_mix_ffn(x.detach(), wk, wv, x.detach()).shape == x.shape
+
+
+def test_refusals_on_cuda():
+    x, w = torch.ones(4, 64, device="cuda"), torch.ones(8, 64, device="cuda")
+    with pytest.raises(TypeError):
+        ops.fp8_linear(x, w)
+    with pytest.raises(TypeError):
+        ops.fp8_linear(x.to(BF), w)
+    with pytest.raises(ValueError):
+        ops.fp8_linear(x.to(BF), w.to(BF).cpu())
+    with pytest.raises(ValueError):
+        ops.fp8_linear(x.to(BF), ops.pack_fp8(w.cpu()))
+    with pytest.raises(TypeError):
+        ops.pack_fp8(x.double())
