@@ -1,0 +1,26 @@
+// One library call for the launches of an 8-bit operator.  A forward or backward pass is three to six kernels of a few
+// microseconds on small batches, and a foreign call with twenty arguments costs about as much as a launch; the host side
+// therefore describes the launches in one array of plain records.
+#include "fp8_steps.cuh"
+
+RWKV_EXPORT int rwkv_fp8_pack(const void* x, int dtype, long long ldx, void* values, void* exps, int R, int C, int rows,
+                              void* stream);
+RWKV_EXPORT int rwkv_fp8_unpack(const void* values, const void* exps, void* y, int dtype, long long ldy, int R, int C, int rows,
+                                void* stream);
+
+// Runs `count` steps in order on `stream`; returns the status of the first that was refused or failed to launch.
+RWKV_EXPORT int rwkv_fp8_run(const Fp8Step* steps, int count, void* stream) {
+  if (count < 0 || (count > 0 && !steps)) return RWKV_ERR_BAD_SHAPE;
+  for (int i = 0; i < count; ++i) {
+    const Fp8Step& s = steps[i];
+    int r = RWKV_ERR_BAD_SHAPE;
+    switch (s.kind) {
+      case FP8_STEP_PACK: r = rwkv_fp8_pack(s.x, s.dtype, s.ldx, s.q_val, s.q_exp, s.M, s.N, s.q_rows, stream); break;
+      case FP8_STEP_UNPACK: r = rwkv_fp8_unpack(s.a_val, s.a_exp, s.c, s.dtype, s.ldc, s.M, s.N, s.a_rows, stream); break;
+      case FP8_STEP_GEMM: r = rwkv_fp8_gemm(s, (cudaStream_t)stream); break;
+      default: break;
+    }
+    if (r) return r;
+  }
+  return RWKV_OK;
+}

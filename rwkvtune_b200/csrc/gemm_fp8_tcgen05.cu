@@ -28,6 +28,7 @@
 #include <atomic>
 
 #include "fp8_format.cuh"
+#include "fp8_steps.cuh"
 #include "tensormap_cache.cuh"
 
 namespace {
@@ -569,51 +570,48 @@ inline int up(int n, int m) { return (n + m - 1) / m * m; }
 // C[M,N] = op(A) op(B) of packed operands (fp8_format.cuh).
 //   a_mn = 0: A is [M,K], a_rows 1 or 128;  a_mn = 1: A is stored [K,M], a_rows 128
 //   b_mn = 0: B is [N,K];  b_mn = 1: B is stored [K,N]; both in tiles
-//   epilogue 0: c = bf16 result (row stride ldc);  1: c = result + residual (bf16, row stride ldr)
+//   epilogue 0: c = bf16 result (row stride ldc);  1: c = result + residual (bf16, row stride ldr), NT only;
 //            2: (q_val, q_exp) = packed relu(result)^2, NT only;  3: = packed result * 2 sqrt(h), NN only;
 //            the packed result and h are [M,N] with blocks of q_rows rows
 //   status: device int, set non-zero if a device-side wait expired
-RWKV_EXPORT int rwkv_gemm_fp8_tcgen05(const void* a_val, const void* a_exp, int a_rows, const void* b_val, const void* b_exp,
-                                      int M, int N, int K, int a_mn, int b_mn, int epilogue, void* c, long long ldc,
-                                      const void* residual, long long ldr, const void* h_val, const void* h_exp, void* q_val,
-                                      void* q_exp, int q_rows, void* status, void* stream) {
+int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t st) {
+  const int M = s.M, N = s.N, K = s.K, a_mn = s.a_mn, b_mn = s.b_mn, epilogue = s.epilogue, q_rows = s.q_rows;
   if (M <= 0 || N <= 0 || K <= 0 || M > 0x7ffffe00 || N > 0x7ffffe00 || K > 0x7ffffe00) return RWKV_ERR_BAD_SHAPE;
-  if (!(a_rows == 128 || (a_rows == 1 && !a_mn)) || epilogue < 0 || epilogue > 3) return RWKV_ERR_BAD_SHAPE;
-  if (epilogue <= 1 ? (!c || ldc < N || (epilogue == 1 && (!residual || ldr < N)))
-                    : (!q_val || !q_exp || !(q_rows == 1 || q_rows == 128) || (epilogue == 3 && (!h_val || !h_exp)) ||
-                       ((uintptr_t)h_val & 15)))
+  if (!(s.a_rows == 128 || (s.a_rows == 1 && !a_mn)) || epilogue < 0 || epilogue > 3) return RWKV_ERR_BAD_SHAPE;
+  if (epilogue <= 1 ? (!s.c || s.ldc < N || (epilogue == 1 && (!s.residual || s.ldr < N)))
+                    : (!s.q_val || !s.q_exp || !(q_rows == 1 || q_rows == 128) ||
+                       (epilogue == 3 && (!s.h_val || !s.h_exp || ((uintptr_t)s.h_val & 15)))))
     return RWKV_ERR_BAD_SHAPE;
   CUtensorMap ma, mb, mo;
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  int r = a_mn ? encode(&ma, u8, 1, a_val, K, M, up(M, 16)) : encode(&ma, u8, 1, a_val, M, K, up(K, 16));
+  int r = a_mn ? encode(&ma, u8, 1, s.a_val, K, M, up(M, 16)) : encode(&ma, u8, 1, s.a_val, M, K, up(K, 16));
   if (r) return r;
-  r = b_mn ? encode(&mb, u8, 1, b_val, K, N, up(N, 16)) : encode(&mb, u8, 1, b_val, N, K, up(K, 16));
+  r = b_mn ? encode(&mb, u8, 1, s.b_val, K, N, up(N, 16)) : encode(&mb, u8, 1, s.b_val, N, K, up(K, 16));
   if (r) return r;
   Args g = {};
   g.M = M; g.N = N; g.K = K;
-  g.a_exp = (const uint8_t*)a_exp; g.b_exp = (const uint8_t*)b_exp;
-  g.a_rows = a_rows;
+  g.a_exp = (const uint8_t*)s.a_exp; g.b_exp = (const uint8_t*)s.b_exp;
+  g.a_rows = s.a_rows;
   g.a_ld = up(M, 16);
   const int mb_n = up(M, 128) / 128, nb_n = up(N, 128) / 128, kb_n = up(K, 128) / 128;
   g.a_sm = a_mn ? 1 : kb_n; g.a_sk = a_mn ? mb_n : 1;
   g.b_sn = b_mn ? 1 : kb_n; g.b_sk = b_mn ? nb_n : 1;
-  g.c = (bf16*)c; g.residual = (const bf16*)residual; g.ldc = ldc; g.ldr = ldr;
-  g.h_val = (const uint8_t*)h_val; g.h_exp = (const uint8_t*)h_exp; g.q_exp = (uint8_t*)q_exp;
+  g.c = (bf16*)s.c; g.residual = (const bf16*)s.residual; g.ldc = s.ldc; g.ldr = s.ldr;
+  g.h_val = (const uint8_t*)s.h_val; g.h_exp = (const uint8_t*)s.h_exp; g.q_exp = (uint8_t*)s.q_exp;
   g.q_ldv = up(N, 16);
   g.q_lde = q_rows == 1 ? up(M, 16) : nb_n;
-  g.status = (int*)status;
+  g.status = (int*)s.status;
   if (epilogue <= 1) {
-    g.direct = ((uintptr_t)c & 15) || (ldc & 7) || (epilogue == 1 && (((uintptr_t)residual & 15) || (ldr & 7) || (N & 7)));
+    g.direct = ((uintptr_t)s.c & 15) || (s.ldc & 7) || (epilogue == 1 && (((uintptr_t)s.residual & 15) || (s.ldr & 7) || (N & 7)));
     if (g.direct) {
       mo = ma;               // never read
     } else {
-      r = encode(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, c, M, N, ldc);
+      r = encode(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, s.c, M, N, s.ldc);
     }
   } else {
-    r = encode(&mo, u8, 1, q_val, M, N, g.q_ldv);
+    r = encode(&mo, u8, 1, s.q_val, M, N, g.q_ldv);
   }
   if (r) return r;
-  cudaStream_t st = (cudaStream_t)stream;
   if (epilogue == 2) {
     if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
     return q_rows == 1 ? launch<false, false, EPI_RELU_SQ, 1>(ma, mb, mo, g, st) : launch<false, false, EPI_RELU_SQ, 128>(ma, mb, mo, g, st);

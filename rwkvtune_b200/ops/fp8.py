@@ -33,23 +33,24 @@ BLOCK = reference.FP8_BLOCK
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
+def _sizes(R: int, C: int, rows: int):
+    """Bytes of the values and of the exponents of a packed matrix."""
+    return R * (-(-C // 16) * 16), -(-C // BLOCK) * (-(-R // 16) * 16 if rows == 1 else -(-R // BLOCK))
+
+
 class Fp8Blocks:
     """A packed matrix: ``R`` rows by ``C`` columns of e4m3 values with one exponent byte per block of ``rows`` x 128.
 
-    ``shape`` and ``dtype`` are those of the tensor it was packed from and of what :func:`unpack_fp8` returns.  ``data`` is
-    one byte buffer: values row by row, each row padded to 16 bytes, then the exponents (``[ceil(R/128)][ceil(C/128)]`` for
-    tiles, ``[ceil(C/128)][R padded to 16]`` for row blocks)."""
+    ``shape`` and ``dtype`` are those of the tensor it was packed from and of what :func:`unpack_fp8` returns.  It lies at
+    ``offset`` in the byte buffer ``data``: values row by row, each row padded to 16 bytes, then the exponents
+    (``[ceil(R/128)][ceil(C/128)]`` for tiles, ``[ceil(C/128)][R padded to 16]`` for row blocks)."""
 
-    __slots__ = ("data", "R", "C", "rows", "shape", "dtype", "exponent_offset")
+    __slots__ = ("data", "offset", "R", "C", "rows", "shape", "dtype", "exponent_offset")
 
-    def __init__(self, data: Optional[torch.Tensor], R: int, C: int, rows: int, shape, dtype, device=None):
-        self.R, self.C, self.rows, self.shape, self.dtype = R, C, rows, torch.Size(shape), dtype
+    def __init__(self, data: torch.Tensor, offset: int, R: int, C: int, rows: int, shape=None, dtype=torch.bfloat16):
+        self.data, self.offset, self.R, self.C, self.rows, self.dtype = data, offset, R, C, rows, dtype
+        self.shape = (R, C) if shape is None else shape
         self.exponent_offset = R * (-(-C // 16) * 16)
-        self.data = data if data is not None else torch.empty(self.exponent_offset + self._exponent_bytes(), dtype=torch.uint8,
-                                                              device=device)
-
-    def _exponent_bytes(self) -> int:
-        return -(-self.C // BLOCK) * (-(-self.R // 16) * 16 if self.rows == 1 else -(-self.R // BLOCK))
 
     @property
     def device(self) -> torch.device:
@@ -57,54 +58,135 @@ class Fp8Blocks:
 
     @property
     def nbytes(self) -> int:
-        return self.data.numel()
+        return sum(_sizes(self.R, self.C, self.rows))
+
+    @property
+    def address(self) -> int:
+        return self.data.data_ptr() + self.offset
 
     @property
     def values(self) -> torch.Tensor:
         """``float8_e4m3fn [R, C]``, a view of the buffer."""
-        return self.data[:self.exponent_offset].view(torch.float8_e4m3fn).view(self.R, -(-self.C // 16) * 16)[:, :self.C]
+        v = self.data[self.offset:self.offset + self.exponent_offset].view(torch.float8_e4m3fn)
+        return v.view(self.R, -(-self.C // 16) * 16)[:, :self.C]
 
     @property
     def exponents(self) -> torch.Tensor:
         """``uint8 [ceil(R / rows), ceil(C / 128)]``, a view of the buffer: the scale of a block is ``2^(exponent - 127)``."""
-        e, nb = self.data[self.exponent_offset:], -(-self.C // BLOCK)
+        e, nb = self.data[self.offset + self.exponent_offset:self.offset + self.nbytes], -(-self.C // BLOCK)
         if self.rows == 1:
             return e.view(nb, -(-self.R // 16) * 16)[:, :self.R].t()
         return e.view(-(-self.R // BLOCK), nb)
 
     def to(self, device) -> "Fp8Blocks":
         data = self.data.to(device)
-        return self if data is self.data else Fp8Blocks(data, self.R, self.C, self.rows, self.shape, self.dtype)
+        return self if data is self.data else Fp8Blocks(data, self.offset, self.R, self.C, self.rows, self.shape, self.dtype)
 
     def __repr__(self) -> str:
         return f"Fp8Blocks(shape={tuple(self.shape)}, rows={self.rows}, dtype={self.dtype}, device={self.device})"
 
 
-def _native():
-    from . import fp8_native
+def _room(device, *specs):
+    """Uninitialised packed matrices ``(R, C, rows)`` in one buffer; ``None`` stays ``None``."""
+    total, at = 0, []
+    for spec in specs:
+        at.append(total)
+        if spec is not None:
+            total += -(-sum(_sizes(*spec)) // 128) * 128
+    data = torch.empty(total, dtype=torch.uint8, device=device)
+    return [None if spec is None else Fp8Blocks(data, o, *spec) for o, spec in zip(at, specs)]
 
-    return fp8_native
+
+class _HostRun:
+    """The steps of an operator, computed one by one in plain PyTorch."""
+
+    def __init__(self, device):
+        pass
+
+    def pack(self, x, q):
+        if q.R:
+            values, exponents = reference.fp8_pack(x, q.rows)
+            q.values.copy_(values)
+            q.exponents.copy_(exponents)
+
+    def unpack(self, p, out):
+        top = torch.finfo(out.dtype).max
+        out.copy_(_f32(p).clamp(-top, top).view(out.shape))
+
+    def nt(self, a, b, out, residual=None):
+        y = _f32(a) @ _f32(b).t()
+        out.copy_(y if residual is None else y + residual.float())
+
+    def nn(self, a, b, out):
+        out.copy_(_f32(a) @ _f32(b))
+
+    def tn(self, a, b, out):
+        out.copy_(_f32(a).t() @ _f32(b))
+
+    def nt_relu_sq(self, a, b, q):
+        self.pack(torch.relu(_f32(a) @ _f32(b).t()) ** 2, q)
+
+    def nn_relu_sq_grad(self, a, b, h, q):
+        self.pack((_f32(a) @ _f32(b)) * 2 * torch.sqrt(_f32(h)), q)
+
+    def go(self):
+        pass
 
 
-def _meta(p: Fp8Blocks):
-    return p.R, p.C, p.rows, p.shape, p.dtype
+class _DeviceRun:
+    """The steps of an operator, collected and launched together."""
+
+    def __init__(self, device):
+        from . import fp8_native
+
+        self.native, self.device, self.steps = fp8_native, device, []
+        self.keep = []                            # copies made on the way: their memory is not reused before the launch
+
+    def pack(self, x, q):
+        if q.R:
+            if (q.C > 1 and x.stride(1) != 1) or (q.R > 1 and x.stride(0) < q.C):
+                x = x.contiguous()
+            self.steps.append(self.native.pack(x, q))
+            self.keep.append(x)
+
+    def unpack(self, p, out):
+        if p.R:
+            self.steps.append(self.native.unpack(p, out))
+
+    def nt(self, a, b, out, residual=None):
+        if a.R:
+            self.steps.append(self.native.mm_nt(a, b, out, residual))
+            self.keep.append(residual)
+
+    def nn(self, a, b, out):
+        if a.R:
+            self.steps.append(self.native.mm_nn(a, b, out))
+
+    def tn(self, a, b, out):
+        if a.R:
+            self.steps.append(self.native.mm_tn(a, b, out))
+        else:
+            out.zero_()
+
+    def nt_relu_sq(self, a, b, q):
+        if a.R:
+            self.steps.append(self.native.mm_nt_relu_sq(a, b, q))
+
+    def nn_relu_sq_grad(self, a, b, h, q):
+        if a.R:
+            self.steps.append(self.native.mm_nn_relu_sq_grad(a, b, h, q))
+
+    def go(self):
+        if self.steps:
+            self.native.run(self.device, self.steps)
 
 
-def _pack2(x: torch.Tensor, rows: int, shape=None) -> Fp8Blocks:
-    """Pack a matrix whose arguments have been checked."""
-    R, C = x.shape
-    p = Fp8Blocks(None, R, C, rows, x.shape if shape is None else shape, x.dtype, x.device)
-    if R == 0:
-        return p
-    if x.is_cuda:
-        if x.stride(1) != 1 and C > 1 or x.stride(0) < C and R > 1:
-            x = x.contiguous()
-        _native().pack(x, p.data, p.exponent_offset, rows)
-    else:
-        values, exponents = reference.fp8_pack(x, rows)
-        p.values.copy_(values)
-        p.exponents.copy_(exponents)
-    return p
+def _run_on(t: torch.Tensor):
+    return (_DeviceRun if t.is_cuda else _HostRun)(t.device)
+
+
+def _f32(p: Fp8Blocks) -> torch.Tensor:
+    return reference.fp8_unpack(p.values, p.exponents, p.rows)
 
 
 def pack_fp8(x: torch.Tensor, rows: int = BLOCK) -> Fp8Blocks:
@@ -116,7 +198,13 @@ def pack_fp8(x: torch.Tensor, rows: int = BLOCK) -> Fp8Blocks:
         raise ValueError(f"pack_fp8: rows is 1 or {BLOCK}, got {rows!r}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"pack_fp8: the last dimension must not be empty, got shape {tuple(x.shape)}")
-    return _pack2(x.detach().reshape(-1, x.shape[-1]), rows, x.shape)
+    x2 = _rows_of(x.detach())
+    (p,) = _room(x.device, (*x2.shape, rows))
+    p.shape, p.dtype = x.shape, x.dtype
+    run = _run_on(x)
+    run.pack(x2, p)
+    run.go()
+    return p
 
 
 def unpack_fp8(p: Fp8Blocks, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -127,60 +215,19 @@ def unpack_fp8(p: Fp8Blocks, dtype: Optional[torch.dtype] = None) -> torch.Tenso
     if dtype not in _FLOATS:
         raise TypeError(f"unpack_fp8: unsupported type {dtype}")
     out = torch.empty(p.shape, dtype=dtype, device=p.device)
-    if p.R == 0:
-        return out
-    if out.is_cuda:
-        _native().unpack(p, out)
-    else:
-        top = torch.finfo(dtype).max
-        out.copy_(reference.fp8_unpack(p.values, p.exponents, p.rows).clamp(-top, top).view(p.shape))
+    run = _run_on(out)
+    run.unpack(p, out)
+    run.go()
     return out
 
 
 # ------------------------------------------------------------------------------- products of packed matrices
-def _f32(p: Fp8Blocks) -> torch.Tensor:
-    return reference.fp8_unpack(p.values, p.exponents, p.rows)
-
-
-def _mm_nt(a: Fp8Blocks, b: Fp8Blocks, dtype, residual=None) -> torch.Tensor:
-    if a.data.is_cuda and a.R:
-        return _native().mm_nt(a, b, residual)
-    y = _f32(a) @ _f32(b).t()
-    return (y if residual is None else y + residual.float()).to(dtype)
-
-
-def _mm_nn(a: Fp8Blocks, b: Fp8Blocks, dtype) -> torch.Tensor:
-    if a.data.is_cuda and a.R:
-        return _native().mm_nn(a, b)
-    return (_f32(a) @ _f32(b)).to(dtype)
-
-
-def _mm_tn(a: Fp8Blocks, b: Fp8Blocks, dtype) -> torch.Tensor:
-    if a.data.is_cuda and a.R:
-        return _native().mm_tn(a, b)
-    return (_f32(a).t() @ _f32(b)).to(dtype)
-
-
-def _hidden(a: Fp8Blocks, wk: Fp8Blocks, rows: int) -> Fp8Blocks:
-    """``P(relu(a wk^T)^2)``"""
-    if a.data.is_cuda and a.R:
-        h = Fp8Blocks(None, a.R, wk.R, rows, (a.R, wk.R), torch.bfloat16, a.device)
-        _native().mm_nt_relu_sq(a, wk, h)
-        return h
-    return _pack2(torch.relu(_f32(a) @ _f32(wk).t()) ** 2, rows)
-
-
-def _hidden_grad(d: Fp8Blocks, wv: Fp8Blocks, h: Fp8Blocks) -> Fp8Blocks:
-    """``P((d wv) * 2 sqrt(h))``"""
-    if d.data.is_cuda and d.R:
-        p = Fp8Blocks(None, h.R, h.C, h.rows, h.shape, torch.bfloat16, d.device)
-        _native().mm_nn_relu_sq_grad(d, wv, h, p)
-        return p
-    return _pack2((_f32(d) @ _f32(wv)) * 2 * torch.sqrt(_f32(h)), h.rows)
-
-
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
-    return t.reshape(-1, t.shape[-1])
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+def _meta(p: Optional[Fp8Blocks]):
+    return None if p is None else (p.offset, p.R, p.C, p.rows)
 
 
 class _Linear(torch.autograd.Function):
@@ -188,19 +235,42 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w):
-        x8, w8 = _pack2(_rows_of(x), BLOCK), _pack2(w, BLOCK)
-        # each packed operand is kept only for the product that reads it
-        ctx.save_for_backward(x8.data if ctx.needs_input_grad[1] else None, w8.data if ctx.needs_input_grad[0] else None)
+        x2 = _rows_of(x)
+        (M, K), N = x2.shape, w.shape[0]
+        need_x, need_w = ctx.needs_input_grad
+        # a packed operand is kept for the product that reads it in backward
+        x8, w8 = _room(x.device, (M, K, BLOCK) if need_w else None, (N, K, BLOCK) if need_x else None)
+        kept = (x8 or w8).data if need_x or need_w else None
+        ctx.save_for_backward(kept)
         ctx.meta, ctx.shape, ctx.types = (_meta(x8), _meta(w8)), x.shape, (x.dtype, w.dtype)
-        return _mm_nt(x8, w8, x.dtype).reshape(*x.shape[:-1], w.shape[0])
+        if not (need_x and need_w):
+            a, b = _room(x.device, None if need_w else (M, K, BLOCK), None if need_x else (N, K, BLOCK))
+            x8, w8 = x8 or a, w8 or b
+        y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+        run = _run_on(x)
+        run.pack(x2, x8)
+        run.pack(w, w8)
+        run.nt(x8, w8, y)
+        run.go()
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x8, w8 = (None if d is None else Fp8Blocks(d, *m) for d, m in zip(ctx.saved_tensors, ctx.meta))
-        d8 = _pack2(_rows_of(dy), BLOCK)
-        dx = _mm_nn(d8, w8, ctx.types[0]).reshape(ctx.shape) if ctx.needs_input_grad[0] else None
-        dw = _mm_tn(d8, x8, ctx.types[1]) if ctx.needs_input_grad[1] else None
+        (data,) = ctx.saved_tensors
+        x8, w8 = (None if m is None else Fp8Blocks(data, *m) for m in ctx.meta)
+        d2 = _rows_of(dy)
+        (d8,) = _room(dy.device, (*d2.shape, BLOCK))
+        run = _run_on(dy)
+        run.pack(d2, d8)
+        dx = dw = None
+        if w8 is not None:
+            dx = torch.empty(ctx.shape, dtype=ctx.types[0], device=dy.device)
+            run.nn(d8, w8, _rows_of(dx))
+        if x8 is not None:
+            dw = torch.empty(d8.C, x8.C, dtype=ctx.types[1], device=dy.device)
+            run.tn(d8, x8, dw)
+        run.go()
         return dx, dw
 
 
@@ -217,11 +287,25 @@ class _LinearFrozen(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         w8 = Fp8Blocks(ctx.saved_tensors[0], *ctx.meta)
-        return _mm_nn(_pack2(_rows_of(dy), 1), w8, dy.dtype).reshape(ctx.shape), None, None
+        d2 = _rows_of(dy)
+        (d8,) = _room(dy.device, (*d2.shape, 1))
+        dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device)
+        run = _run_on(dy)
+        run.pack(d2, d8)
+        run.nn(d8, w8, _rows_of(dx))
+        run.go()
+        return dx, None, None
 
 
 def _linear_frozen(x, w8):
-    return _mm_nt(_pack2(_rows_of(x), 1), w8, x.dtype).reshape(*x.shape[:-1], w8.R)
+    x2 = _rows_of(x)
+    (x8,) = _room(x.device, (*x2.shape, 1))
+    y = torch.empty(*x.shape[:-1], w8.R, dtype=x.dtype, device=x.device)
+    run = _run_on(x)
+    run.pack(x2, x8)
+    run.nt(x8, w8, _rows_of(y))
+    run.go()
+    return y
 
 
 def _check_activation(name: str, x, like=None) -> None:
@@ -265,40 +349,62 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]) -> torch
 class _ChannelMix(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wk, wv, residual):
-        x8, k8, v8 = _pack2(_rows_of(x), BLOCK), _pack2(wk, BLOCK), _pack2(wv, BLOCK)
-        h8 = _hidden(x8, k8, BLOCK)
-        need_x, need_k, need_v = ctx.needs_input_grad[:3]
-        inner = need_x or need_k
-        ctx.save_for_backward(x8.data if need_k else None, k8.data if need_x else None, v8.data if inner else None,
-                              h8.data if inner or need_v else None)
-        ctx.meta, ctx.shape, ctx.types = (_meta(x8), _meta(k8), _meta(v8), _meta(h8)), x.shape, (x.dtype, wk.dtype, wv.dtype)
-        return _mm_nt(h8, v8, x.dtype, _rows_of(residual)).reshape(residual.shape)
+        x2, dev = _rows_of(x), x.device
+        (M, C), (N, H) = x2.shape, wv.shape
+        need_x, need_k, need_v, _ = ctx.needs_input_grad
+        specs = ((M, C, BLOCK), (H, C, BLOCK), (N, H, BLOCK), (M, H, BLOCK))
+        keep = (need_k, need_x, need_x or need_k, need_x or need_k or need_v)
+        ops8 = _room(dev, *(s if k else None for s, k in zip(specs, keep)))
+        ctx.save_for_backward(ops8[3].data if keep[3] else None)
+        ctx.meta, ctx.shape, ctx.types = [_meta(p) for p in ops8], x.shape, (x.dtype, wk.dtype, wv.dtype)
+        if not all(keep):
+            ops8 = [a or b for a, b in zip(ops8, _room(dev, *(None if k else s for s, k in zip(specs, keep))))]
+        x8, k8, v8, h8 = ops8
+        y = torch.empty(residual.shape, dtype=x.dtype, device=dev)
+        run = _run_on(x)
+        run.pack(x2, x8)
+        run.pack(wk, k8)
+        run.pack(wv, v8)
+        run.nt_relu_sq(x8, k8, h8)
+        run.nt(h8, v8, _rows_of(y), _rows_of(residual))
+        run.go()
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x8, k8, v8, h8 = (None if d is None else Fp8Blocks(d, *m) for d, m in zip(ctx.saved_tensors, ctx.meta))
+        (data,) = ctx.saved_tensors
         need_x, need_k, need_v, need_r = ctx.needs_input_grad
         dx = dwk = dwv = None
-        if need_x or need_k or need_v:
-            d8 = _pack2(_rows_of(dy), BLOCK)
-        if need_x or need_k:
-            p8 = _hidden_grad(d8, v8, h8)
-            dx = _mm_nn(p8, k8, ctx.types[0]).reshape(ctx.shape) if need_x else None
-            dwk = _mm_tn(p8, x8, ctx.types[1]) if need_k else None
-        if need_v:
-            dwv = _mm_tn(d8, h8, ctx.types[2])
+        if data is not None:
+            x8, k8, v8, h8 = (None if m is None else Fp8Blocks(data, *m) for m in ctx.meta)
+            d2, dev = _rows_of(dy), dy.device
+            d8, p8 = _room(dev, (*d2.shape, BLOCK), (h8.R, h8.C, BLOCK) if need_x or need_k else None)
+            run = _run_on(dy)
+            run.pack(d2, d8)
+            if need_x or need_k:
+                run.nn_relu_sq_grad(d8, v8, h8, p8)
+            if need_x:
+                dx = torch.empty(ctx.shape, dtype=ctx.types[0], device=dev)
+                run.nn(p8, k8, _rows_of(dx))
+            if need_k:
+                dwk = torch.empty(p8.C, x8.C, dtype=ctx.types[1], device=dev)
+                run.tn(p8, x8, dwk)
+            if need_v:
+                dwv = torch.empty(d8.C, h8.C, dtype=ctx.types[2], device=dev)
+                run.tn(d8, h8, dwv)
+            run.go()
         return dx, dwk, dwv, (dy if need_r else None)
 
 
 class _ChannelMixFrozen(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, kdata, vdata, residual, k8, v8):
-        h8 = _hidden(_pack2(_rows_of(x), 1), k8, 1)
+        y, h8 = _channel_mix_frozen(x, k8, v8, residual)
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(kdata, vdata, h8.data)
-            ctx.meta, ctx.shape = (_meta(k8), _meta(v8), _meta(h8)), x.shape
-        return _mm_nt(h8, v8, x.dtype, _rows_of(residual)).reshape(residual.shape)
+            ctx.meta, ctx.shape = [_meta(p) for p in (k8, v8, h8)], x.shape
+        return y
 
     @staticmethod
     @once_differentiable
@@ -306,9 +412,28 @@ class _ChannelMixFrozen(torch.autograd.Function):
         dx = None
         if ctx.needs_input_grad[0]:
             k8, v8, h8 = (Fp8Blocks(d, *m) for d, m in zip(ctx.saved_tensors, ctx.meta))
-            p8 = _hidden_grad(_pack2(_rows_of(dy), 1), v8, h8)
-            dx = _mm_nn(p8, k8, dy.dtype).reshape(ctx.shape)
+            d2 = _rows_of(dy)
+            d8, p8 = _room(dy.device, (*d2.shape, 1), (h8.R, h8.C, 1))
+            dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device)
+            run = _run_on(dy)
+            run.pack(d2, d8)
+            run.nn_relu_sq_grad(d8, v8, h8, p8)
+            run.nn(p8, k8, _rows_of(dx))
+            run.go()
         return dx, None, None, (dy if ctx.needs_input_grad[3] else None), None, None
+
+
+def _channel_mix_frozen(x, k8, v8, residual):
+    x2 = _rows_of(x)
+    (x8,) = _room(x.device, (*x2.shape, 1))
+    (h8,) = _room(x.device, (x2.shape[0], k8.R, 1))
+    y = torch.empty(residual.shape, dtype=x.dtype, device=x.device)
+    run = _run_on(x)
+    run.pack(x2, x8)
+    run.nt_relu_sq(x8, k8, h8)
+    run.nt(h8, v8, _rows_of(y), _rows_of(residual))
+    run.go()
+    return y, h8
 
 
 def fp8_channel_mix_ffn(xk: torch.Tensor, w_key: Union[torch.Tensor, Fp8Blocks], w_value: Union[torch.Tensor, Fp8Blocks],
@@ -326,11 +451,10 @@ def fp8_channel_mix_ffn(xk: torch.Tensor, w_key: Union[torch.Tensor, Fp8Blocks],
     if residual.shape != xk.shape[:-1] + (w_value.shape[0],):
         raise ValueError(f"{name}: a residual of shape {tuple(xk.shape[:-1]) + (w_value.shape[0],)} was expected, got "
                          f"{tuple(residual.shape)}")
-    if residual.stride(-1) != 1 and residual.shape[-1] > 1:
+    if not residual.is_contiguous() and (residual.dim() != 2 or residual.stride(1) != 1 or residual.stride(0) < residual.shape[1]):
         residual = residual.contiguous()
     if not packed:
         return _ChannelMix.apply(xk, w_key, w_value, residual)
     if torch.is_grad_enabled() and (xk.requires_grad or residual.requires_grad):
         return _ChannelMixFrozen.apply(xk, w_key.data, w_value.data, residual, w_key, w_value)
-    h8 = _hidden(_pack2(_rows_of(xk), 1), w_key, 1)
-    return _mm_nt(h8, w_value, xk.dtype, _rows_of(residual)).reshape(residual.shape)
+    return _channel_mix_frozen(xk, w_key, w_value, residual)[0]

@@ -1,100 +1,91 @@
 """Binding of the 8-bit block kernels (``csrc/fp8_blocks.cu``, ``csrc/gemm_fp8_tcgen05.cu``).
 
-Operands are :class:`rwkvtune_b200.ops.fp8.Fp8Blocks` on one CUDA device; every call runs on the current stream of that
-device and allocates its results there.  No sizes are refused: rows of packed matrices are padded to 16 bytes, and results
+An operator describes its launches as records (``csrc/fp8_steps.cuh``) and hands them over in one library call
+(:func:`run`): on a small batch a foreign call with twenty arguments costs as much as a launch.  Everything runs on the
+current stream of the operands' device.  No sizes are refused: rows of packed matrices are padded to 16 bytes, and results
 whose rows do not start on 16 bytes take a slower store inside the same kernel.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import struct
 
 import torch
 
 from . import _ext, gemm_native
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-_ARGTYPES = {
-    "rwkv_fp8_pack": [_P, _I, _L, _P, _P, _I, _I, _I, _P],
-    "rwkv_fp8_unpack": [_P, _P, _P, _I, _L, _I, _I, _I, _P],
-    "rwkv_gemm_fp8_tcgen05": [_P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _L, _P, _L, _P, _P, _P, _P, _I, _P, _P],
-}
-_NULL = contextlib.nullcontext()
+_PACK, _UNPACK, _GEMM = 0, 1, 2
+_STORE, _RESIDUAL, _RELU_SQ, _RELU_SQ_GRAD = 0, 1, 2, 3
+_record = struct.Struct("=12i3q12Q").pack      # Fp8Step, field by field
 _declared = False
 
 
-def _call(name: str, *args) -> None:
+def _status(device: torch.device) -> int:
+    return gemm_native._status(device).data_ptr()
+
+
+def pack(x: torch.Tensor, q) -> bytes:
+    """``x [R, C]`` with unit inner stride -> ``q``."""
+    at = q.address
+    return _record(_PACK, q.R, q.C, 0, 0, q.rows, _DTYPES[x.dtype], 0, 0, 0, 0, 0, x.stride(0) if q.R > 1 else q.C, 0, 0,
+                   x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, at, at + q.exponent_offset, 0)
+
+
+def unpack(p, out: torch.Tensor) -> bytes:
+    at = p.address
+    return _record(_UNPACK, p.R, p.C, 0, p.rows, 0, _DTYPES[out.dtype], 0, 0, 0, 0, 0, 0, p.C, 0, 0, at, at + p.exponent_offset,
+                   0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0)
+
+
+def _product(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, out=None, residual=None, h=None, q=None) -> bytes:
+    pa, pb = a.address, b.address
+    ph = pq = he = qe = qr = pr = ldr = 0
+    if h is not None:
+        ph = h.address
+        he = ph + h.exponent_offset
+    if q is not None:
+        pq, qr = q.address, q.rows
+        qe = pq + q.exponent_offset
+    if residual is not None:
+        pr, ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
+    return _record(_GEMM, M, N, K, a.rows, qr, 0, a_mn, b_mn, epilogue, 0, 0, 0, N, ldr, 0, pa, pa + a.exponent_offset,
+                   pb, pb + b.exponent_offset, 0 if out is None else out.data_ptr(), pr, ph, he, pq, qe, _status(a.data.device))
+
+
+def mm_nt(a, b, out, residual=None) -> bytes:
+    """``out [M, N] = a [M, K] @ b [N, K]^T (+ residual)``"""
+    return _product(a, b, a.R, b.R, a.C, 0, 0, _STORE if residual is None else _RESIDUAL, out, residual)
+
+
+def mm_nn(a, b, out) -> bytes:
+    """``out [M, N] = a [M, K] @ b [K, N]``"""
+    return _product(a, b, a.R, b.C, a.C, 0, 1, _STORE, out)
+
+
+def mm_tn(a, b, out) -> bytes:
+    """``out [M, N] = a [K, M]^T @ b [K, N]``, both in tiles"""
+    return _product(a, b, a.C, b.C, a.R, 1, 1, _STORE, out)
+
+
+def mm_nt_relu_sq(a, b, q) -> bytes:
+    """``q = packed relu(a @ b^T)^2``"""
+    return _product(a, b, a.R, b.R, a.C, 0, 0, _RELU_SQ, q=q)
+
+
+def mm_nn_relu_sq_grad(a, b, h, q) -> bytes:
+    """``q = packed (a @ b) * 2 sqrt(h)``"""
+    return _product(a, b, a.R, b.C, a.C, 0, 1, _RELU_SQ_GRAD, h=h, q=q)
+
+
+def run(device: torch.device, steps) -> None:
+    """Launch ``steps`` in order on the device's current stream."""
     global _declared
-    if not _declared:      # declared once: plain integers and addresses can then be passed as they are
-        for fn, types in _ARGTYPES.items():
-            getattr(_ext.lib(), fn).argtypes = types
+    if not _declared:
+        _ext.lib().rwkv_fp8_run.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
         _declared = True
-    _ext.call(name, *args)
-
-
-def on_device(device: torch.device):
-    """Context in which ``device`` is current (nothing to do when it is already)."""
-    return _NULL if device.index is None or device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
-
-
-def pack(x: torch.Tensor, data: torch.Tensor, exponent_offset: int, rows: int) -> None:
-    """``x [R, C]`` with unit inner stride -> ``data`` (values, then exponents at ``exponent_offset``)."""
-    base = data.data_ptr()
-    R, C = x.shape
-    with on_device(x.device):
-        _call("rwkv_fp8_pack", x.data_ptr(), _DTYPES[x.dtype], x.stride(0) if R > 1 else C, base, base + exponent_offset, R, C,
-              rows, _ext.stream())
-
-
-def unpack(p, out: torch.Tensor) -> None:
-    base = p.data.data_ptr()
-    with on_device(out.device):
-        _call("rwkv_fp8_unpack", base, base + p.exponent_offset, out.data_ptr(), _DTYPES[out.dtype], p.C, p.R, p.C, p.rows,
-              _ext.stream())
-
-
-def _gemm(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, out=None, residual=None, h=None, q=None) -> None:
-    pa, pb = a.data.data_ptr(), b.data.data_ptr()
-    ph, pq = (0 if t is None else t.data.data_ptr() for t in (h, q))
-    with on_device(a.data.device):
-        _call("rwkv_gemm_fp8_tcgen05", pa, pa + a.exponent_offset, a.rows, pb, pb + b.exponent_offset, M, N, K, a_mn, b_mn,
-              epilogue, 0 if out is None else out.data_ptr(), N, 0 if residual is None else residual.data_ptr(),
-              0 if residual is None else (residual.stride(0) if M > 1 else N), ph, 0 if h is None else ph + h.exponent_offset,
-              pq, 0 if q is None else pq + q.exponent_offset, 0 if q is None else q.rows,
-              gemm_native._status(a.data.device).data_ptr(), _ext.stream())
-
-
-def _new(like, M: int, N: int) -> torch.Tensor:
-    return torch.empty(M, N, dtype=torch.bfloat16, device=like.data.device)
-
-
-def mm_nt(a, b, residual=None) -> torch.Tensor:
-    """``a [M, K] @ b [N, K]^T (+ residual [M, N])`` in bf16."""
-    out = _new(a, a.R, b.R)
-    _gemm(a, b, a.R, b.R, a.C, 0, 0, 0 if residual is None else 1, out, residual)
-    return out
-
-
-def mm_nn(a, b) -> torch.Tensor:
-    """``a [M, K] @ b [K, N]`` in bf16."""
-    out = _new(a, a.R, b.C)
-    _gemm(a, b, a.R, b.C, a.C, 0, 1, 0, out)
-    return out
-
-
-def mm_tn(a, b) -> torch.Tensor:
-    """``a [K, M]^T @ b [K, N]`` in bf16, both in tiles."""
-    out = _new(a, a.C, b.C)
-    _gemm(a, b, a.C, b.C, a.R, 1, 1, 0, out)
-    return out
-
-
-def mm_nt_relu_sq(a, b, q) -> None:
-    """``q = packed relu(a @ b^T)^2``."""
-    _gemm(a, b, a.R, b.R, a.C, 0, 0, 2, q=q)
-
-
-def mm_nn_relu_sq_grad(a, b, h, q) -> None:
-    """``q = packed (a @ b) * 2 sqrt(h)``."""
-    _gemm(a, b, a.R, b.C, a.C, 0, 1, 3, h=h, q=q)
+    if device.index is not None and device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return run(device, steps)
+    _ext.LAUNCH_COUNT += len(steps) - 1
+    _ext.call("rwkv_fp8_run", b"".join(steps), len(steps), _ext.stream())

@@ -20,6 +20,22 @@ def no_expired_wait():
     assert gemm_native.check_status() == 0
 
 
+def product(name, a, b, M, N, *more):
+    out = torch.full((M, N), math.nan, dtype=BF, device="cuda")
+    run = fp8._run_on(a.data)
+    getattr(run, name)(a, b, out, *more)
+    run.go()
+    return out
+
+
+def packed_product(name, a, b, M, N, rows, *more):
+    (q,) = fp8._room(a.device, (M, N, rows))
+    run = fp8._run_on(a.data)
+    getattr(run, name)(a, b, *more, q)
+    run.go()
+    return q
+
+
 def sample(R, C, dtype=BF, seed=0):
     g = torch.Generator().manual_seed(seed)
     x = torch.randn(R, C, generator=g) * torch.exp(2 * torch.randn(R, 1, generator=g))
@@ -101,7 +117,7 @@ SIZES = [(128, 128, 128), (256, 256, 256), (1, 128, 128), (300, 520, 384), (5, 2
 def test_nt(M, N, K, rows):
     a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda())
     A, B = values64(a), values64(b)
-    near(fp8._mm_nt(a, b, BF), A @ B.t(), A.abs() @ B.abs().t(), K)
+    near(product("nt", a, b, M, N), A @ B.t(), A.abs() @ B.abs().t(), K)
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -109,7 +125,7 @@ def test_nt(M, N, K, rows):
 def test_nt_residual(M, N, K, rows):
     a, b, c = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda()), sample(M, N, seed=7).cuda()
     A, B = values64(a), values64(b)
-    near(fp8._mm_nt(a, b, BF, c), c.double() + A @ B.t(), A.abs() @ B.abs().t() + c.double().abs(), K)
+    near(product("nt", a, b, M, N, c), c.double() + A @ B.t(), A.abs() @ B.abs().t() + c.double().abs(), K)
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -117,14 +133,14 @@ def test_nt_residual(M, N, K, rows):
 def test_nn(M, N, K, rows):
     a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(K, N).cuda())
     A, B = values64(a), values64(b)
-    near(fp8._mm_nn(a, b, BF), A @ B, A.abs() @ B.abs(), K)
+    near(product("nn", a, b, M, N), A @ B, A.abs() @ B.abs(), K)
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_tn(M, N, K):
     a, b = ops.pack_fp8(sample(K, M).cuda()), ops.pack_fp8(sample(K, N, seed=5).cuda())
     A, B = values64(a), values64(b)
-    near(fp8._mm_tn(a, b, BF), A.t() @ B, A.abs().t() @ B.abs(), K)
+    near(product("tn", a, b, M, N), A.t() @ B, A.abs().t() @ B.abs(), K)
 
 
 def packed_near(q, want, magnitude, n, rows):
@@ -145,7 +161,7 @@ def test_relu_sq_packed(M, N, K, rows):
     a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda())
     A, B = values64(a), values64(b)
     pre, mag = A @ B.t(), A.abs() @ B.abs().t()
-    packed_near(fp8._hidden(a, b, rows), torch.relu(pre) ** 2, 2 * pre.abs() * mag + 1e-30, K, rows)
+    packed_near(packed_product("nt_relu_sq", a, b, M, N, rows), torch.relu(pre) ** 2, 2 * pre.abs() * mag + 1e-30, K, rows)
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -154,7 +170,7 @@ def test_relu_sq_grad_packed(M, N, K, rows):
     d, w = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(K, N).cuda())
     h = ops.pack_fp8((torch.relu(sample(M, N, seed=3).float()) ** 2).to(BF).cuda(), rows=rows)
     D, W, slope = values64(d), values64(w), 2 * values64(h).sqrt()
-    packed_near(fp8._hidden_grad(d, w, h), (D @ W) * slope, (D.abs() @ W.abs()) * slope + 1e-30, K + 64, rows)
+    packed_near(packed_product("nn_relu_sq_grad", d, w, M, N, rows, h), (D @ W) * slope, (D.abs() @ W.abs()) * slope + 1e-30, K + 64, rows)
 
 
 def test_long_contraction_and_many_tiles():
@@ -163,14 +179,14 @@ def test_long_contraction_and_many_tiles():
     for rows in (1, 128):
         a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda())
         A, B = values64(a), values64(b)
-        near(fp8._mm_nt(a, b, BF), A @ B.t(), A.abs() @ B.abs().t(), K)
-        q = fp8._hidden(a, b, rows)
+        near(product("nt", a, b, M, N), A @ B.t(), A.abs() @ B.abs().t(), K)
+        q = packed_product("nt_relu_sq", a, b, M, N, rows)
         pre = A @ B.t()
         packed_near(q, torch.relu(pre) ** 2, 2 * pre.abs() * (A.abs() @ B.abs().t()) + 1e-30, K, rows)
     b = ops.pack_fp8(weights(M, N, 4).cuda())
     a = ops.pack_fp8(sample(M, K).cuda())
     A, B = values64(a), values64(b)
-    near(fp8._mm_tn(a, b, BF), A.t() @ B, A.abs().t() @ B.abs(), M)
+    near(product("tn", a, b, K, N), A.t() @ B, A.abs().t() @ B.abs(), M)
 
 
 def test_non_finite_blocks_reach_exactly_their_products():
@@ -212,8 +228,8 @@ def test_channel_mix_autograd(M, C, H, frozen):
     x, res = sample(M, C).cuda().requires_grad_(), sample(M, C, seed=2).cuda().requires_grad_()
     wk, wv, dy = weights(H, C).cuda(), weights(C, H, 3).cuda(), sample(M, C, seed=9).cuda()
     x8, k8, v8, d8 = ops.pack_fp8(x, rows), ops.pack_fp8(wk), ops.pack_fp8(wv), ops.pack_fp8(dy, rows)
-    h8 = fp8._hidden(x8, k8, rows)                # these two are compared with their 64-bit values above
-    p8 = fp8._hidden_grad(d8, v8, h8)
+    h8 = packed_product("nt_relu_sq", x8, k8, M, H, rows)                # these two are compared with their 64-bit values above
+    p8 = packed_product("nn_relu_sq_grad", d8, v8, M, H, rows, h8)
     X, K, V, D, Hd, P = (values64(t) for t in (x8, k8, v8, d8, h8, p8))
     args = (k8, v8) if frozen else (wk.requires_grad_(), wv.requires_grad_())
     y = ops.fp8_channel_mix_ffn(x, *args, res)
