@@ -87,6 +87,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(ROW_THREADS)
 fp8_pack_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
                      int R, int C, int ldv, int lde, int blocks) {
+  rwkv_chain_trigger();       // a chained decode product may fetch its weights meanwhile
   const long long units = (long long)R * blocks, stride = (long long)gridDim.x * (ROW_THREADS / 8);
   const int part = threadIdx.x & 7;
   const long long rounds = (units + stride - 1) / stride;          // the same for every thread: the shuffles need whole warps

@@ -2,7 +2,7 @@
 #pragma once
 #include "common.cuh"
 
-enum Fp8StepKind : int { FP8_STEP_PACK = 0, FP8_STEP_UNPACK = 1, FP8_STEP_GEMM = 2 };
+enum Fp8StepKind : int { FP8_STEP_PACK = 0, FP8_STEP_UNPACK = 1, FP8_STEP_GEMM = 2, FP8_STEP_DECODE = 3 };
 
 struct Fp8Step {
   int kind;
@@ -10,7 +10,8 @@ struct Fp8Step {
   int a_rows, q_rows;        // rows of a block of A (unpack: of the input) and of the packed result
   int dtype;                 // pack, unpack: type of the plain side (0 bf16, 1 fp16, 2 fp32)
   int a_mn, b_mn, epilogue;  // gemm: see gemm_fp8_tcgen05.cu
-  int reserved[2];
+  int chained;               // decode: may start before its predecessor has finished (see gemm_fp8_decode.cu)
+  int reserved;
   long long ldx, ldc, ldr;   // row strides of x (pack), c and the residual
   const void* x;
   const void *a_val, *a_exp, *b_val, *b_exp;
@@ -22,3 +23,4 @@ struct Fp8Step {
 };
 
 int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t stream);
+int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t stream);

@@ -189,7 +189,14 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the loads into v.  The empty statements make every later use of v depend on something behind the wait: without
+// them the compiler may copy a destination register before its value has arrived.
+template <int COUNT>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[COUNT]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) asm volatile("" : "+r"(v[i]));
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -392,7 +399,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
               }
             }
           }
-          tmem_wait_ld();
+          tmem_wait_ld(v);
           if (i == 0) {
             tc_fence_before();
             if (lane == 0) mbar_arrive_cluster(free_leader);
@@ -448,7 +455,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) tmem_ld32(t_row + half * 128 + j * 32, v + j * 32);
-          tmem_wait_ld();
+          tmem_wait_ld(v);
           if (i == 0) {
             tc_fence_before();
             if (lane == 0) mbar_arrive_cluster(free_leader);
@@ -515,6 +522,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     if (elected) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
+  __syncwarp();
+  if (warp == WARP_TMA && *reinterpret_cast<volatile int*>(&bars->abort_flag)) {
+    const unsigned long long until = globaltimer_ns() + 1000000ull;      // loads in flight land before the memory is given up
+    while (globaltimer_ns() < until) {}
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();            // neither CTA leaves (or frees tensor memory) while the other may still signal or read it

@@ -17,8 +17,8 @@ With ``P`` for packing, ``x [M, K]``, ``W [N, K]``::
 Sums are formed in fp32 and rounded once.  The gradients are those of the products of the packed operands: packing itself
 counts as the identity.  Backward keeps ``P(x)``, ``h`` and the packed weights, one byte a value, and nothing in 16 bits.
 
-CUDA tensors run the kernels of ``csrc/fp8_blocks.cu`` and ``csrc/gemm_fp8_tcgen05.cu`` (bf16 activations; packing also
-takes fp16 and fp32).  CPU tensors of any of the three types run the same definitions in plain fp32.
+CUDA tensors run the kernels of ``csrc/fp8_blocks.cu``, ``csrc/gemm_fp8_tcgen05.cu`` and, for at most 128 rows against a
+frozen weight, ``csrc/gemm_fp8_decode.cu`` (bf16 activations; packing also takes fp16 and fp32).  CPU tensors of any of the three types run the same definitions in plain fp32.
 """
 from __future__ import annotations
 
@@ -123,6 +123,11 @@ class _HostRun:
     def tn(self, a, b, out):
         out.copy_(_f32(a).t() @ _f32(b))
 
+    def nt_frozen(self, x, w, out, hidden=None):
+        (x8,) = _room(x.device, (*x.shape, 1))
+        self.pack(x, x8)
+        self.nt(x8, w, out) if hidden is None else self.nt_relu_sq(x8, w, hidden)
+
     def nt_relu_sq(self, a, b, q):
         self.pack(torch.relu(_f32(a) @ _f32(b).t()) ** 2, q)
 
@@ -154,9 +159,34 @@ class _DeviceRun:
             self.steps.append(self.native.unpack(p, out))
 
     def nt(self, a, b, out, residual=None):
-        if a.R:
+        if not a.R:
+            return
+        if a.rows == 1 and self.native.decode_form(a.R, b.R, b.C, True):
+            # its predecessor is the step that packed `a`, which does not write the weights
+            self.steps.append(self.native.decode(a, b, out, residual, chained=bool(self.steps)))
+        else:
             self.steps.append(self.native.mm_nt(a, b, out, residual))
-            self.keep.append(residual)
+        self.keep.append(residual)
+
+    def nt_frozen(self, x, w, out, hidden=None):
+        """``out = P(x) w^T`` or ``hidden = P(relu(P(x) w^T)^2)`` with ``x`` packed row by row."""
+        if not x.shape[0]:
+            return
+        form = self.native.decode_form(x.shape[0], w.R, w.C)
+        if form == 2:
+            x = self.native.decode_input(x)
+            self.keep.append(x)
+            self.steps.append(self.native.decode(x, w, out, q=hidden))
+            return
+        (x8,) = _room(x.device, (*x.shape, 1))
+        self.keep.append(x8)
+        self.pack(x, x8)
+        if hidden is None:
+            self.nt(x8, w, out)
+        elif form:
+            self.steps.append(self.native.decode(x8, w, q=hidden, chained=True))
+        else:
+            self.nt_relu_sq(x8, w, hidden)
 
     def nn(self, a, b, out):
         if a.R:
@@ -299,11 +329,9 @@ class _LinearFrozen(torch.autograd.Function):
 
 def _linear_frozen(x, w8):
     x2 = _rows_of(x)
-    (x8,) = _room(x.device, (*x2.shape, 1))
     y = torch.empty(*x.shape[:-1], w8.R, dtype=x.dtype, device=x.device)
     run = _run_on(x)
-    run.pack(x2, x8)
-    run.nt(x8, w8, _rows_of(y))
+    run.nt_frozen(x2, w8, _rows_of(y))
     run.go()
     return y
 
@@ -425,12 +453,10 @@ class _ChannelMixFrozen(torch.autograd.Function):
 
 def _channel_mix_frozen(x, k8, v8, residual):
     x2 = _rows_of(x)
-    (x8,) = _room(x.device, (*x2.shape, 1))
     (h8,) = _room(x.device, (x2.shape[0], k8.R, 1))
     y = torch.empty(residual.shape, dtype=x.dtype, device=x.device)
     run = _run_on(x)
-    run.pack(x2, x8)
-    run.nt_relu_sq(x8, k8, h8)
+    run.nt_frozen(x2, k8, None, h8)
     run.nt(h8, v8, _rows_of(y), _rows_of(residual))
     run.go()
     return y, h8

@@ -173,6 +173,50 @@ def test_relu_sq_grad_packed(M, N, K, rows):
     packed_near(packed_product("nn_relu_sq_grad", d, w, M, N, rows, h), (D @ W) * slope, (D.abs() @ W.abs()) * slope + 1e-30, K + 64, rows)
 
 
+@pytest.mark.parametrize("N,K", [(128, 128), (40, 24), (200, 264), (2048, 2048), (640, 8192), (130, 1000), (8192, 512), (20000, 128)])
+@pytest.mark.parametrize("M", [1, 2, 16, 17, 64, 100, 128])
+def test_few_rows(M, N, K):
+    """The decode kernel: bf16 tokens packed inside it, packed tokens, and its three epilogues."""
+    from rwkvtune_b200.ops import fp8_native as native
+
+    x, w8 = sample(M, K).cuda(), ops.pack_fp8(weights(N, K).cuda())
+    x8, res = ops.pack_fp8(x, rows=1), sample(M, N, seed=7).cuda()
+    A, B = values64(x8), values64(w8)
+    pre, mag = A @ B.t(), A.abs() @ B.abs().t()
+    assert native.decode_form(M, N, K, True) == 1 and native.decode_form(M, N, K) == (2 if M <= 16 and K % 8 == 0 else 1)
+    forms = [x8] + ([x] if native.decode_form(M, N, K) == 2 else [])
+    for t in forms:
+        out, out_r = (torch.full((M, N), math.nan, dtype=BF, device="cuda") for _ in range(2))
+        (q,) = fp8._room(x.device, (M, N, 1))
+        native.run(x.device, [native.decode(t, w8, out), native.decode(t, w8, out_r, res), native.decode(t, w8, q=q)])
+        near(out, pre, mag, K)
+        near(out_r, res.double() + pre, mag + res.double().abs(), K)
+        packed_near(q, torch.relu(pre) ** 2, 2 * pre.abs() * mag + 1e-30, K, 1)
+    if len(forms) == 2:
+        out2 = torch.empty_like(out)
+        native.run(x.device, [native.decode(x8, w8, out2)])
+        assert torch.equal(out, out2)
+
+
+def test_few_rows_of_strided_inputs():
+    w8 = ops.pack_fp8(weights(200, 256).cuda())
+    base = sample(40, 600).cuda()
+    for x in (base[:3, 1:257], base[:16, 8:264], base[::4, :256], base[:2, :512:2], base[0, :256].expand(5, 256), base[7, 3:259]):
+        assert torch.equal(ops.fp8_linear(x, w8), ops.fp8_linear(x.contiguous().clone(), w8))
+
+
+def test_weights_packed_just_before_a_chained_product():
+    """Fresh weights every time: a product that fetched them before they were written would show old bytes."""
+    x, res = sample(20, 512).cuda(), sample(20, 512, seed=3).cuda()
+    for seed in range(6):
+        wk, wv = weights(1024, 512, seed).cuda(), weights(512, 1024, seed + 50).cuda()
+        torch.cuda.synchronize()
+        k8, v8 = ops.pack_fp8(wk), ops.pack_fp8(wv)
+        y = ops.fp8_channel_mix_ffn(x, k8, v8, res)
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.fp8_channel_mix_ffn(x, k8, v8, res))
+
+
 def test_long_contraction_and_many_tiles():
     """More tiles than SM pairs, more scale sets than the ring holds, 8-bit scales that differ from block to block."""
     M, N, K = 2600, 2100, 5000
@@ -243,13 +287,15 @@ def test_channel_mix_autograd(M, C, H, frozen):
 
 
 def test_frozen_rows_do_not_depend_on_the_batch():
+    """Bit for bit among batches of at most 128 rows, and among larger ones; the two sum in different orders."""
     w8 = ops.pack_fp8(weights(384, 640).cuda())
     k8, v8 = ops.pack_fp8(weights(512, 640, 5).cuda()), ops.pack_fp8(weights(640, 512, 6).cuda())
     x, res = sample(300, 640).cuda(), sample(300, 640, seed=8).cuda()
     for f in (lambda a, r: ops.fp8_linear(a, w8), lambda a, r: ops.fp8_channel_mix_ffn(a, k8, v8, r)):
-        whole = f(x, res)
-        for i in (0, 1, 127, 128, 255, 299):
-            assert torch.equal(f(x[i:i + 1], res[i:i + 1]), whole[i:i + 1])
+        few, many = f(x[:128], res[:128]), f(x, res)
+        for i in (0, 1, 63, 127):
+            assert torch.equal(f(x[i:i + 1], res[i:i + 1]), few[i:i + 1])
+        assert torch.equal(f(x[:20], res[:20]), few[:20]) and torch.equal(f(x[:129], res[:129]), many[:129])
 
 
 def test_same_bits_twice_and_on_other_streams():
