@@ -19,7 +19,8 @@
 //
 // Tensor memory holds two 256-column accumulators that overlap by 64 columns plus four 16-column sets of scales.  The
 // epilogue of a tile reads the shared 64 columns first and releases them; the products of the next tile start there, so
-// the overlap costs one 64-column read per tile instead of a whole drained accumulator.
+// the overlap costs one 64-column read per tile instead of a whole drained accumulator.  Two groups of four warps drain a
+// tile, 128 columns each.
 //
 // Every mbarrier wait is bounded as in gemm_tcgen05_2cta.cu: on expiry a code goes to `status`, all roles leave, the CTAs
 // meet, tensor memory is released and the kernel returns.
@@ -44,7 +45,8 @@ constexpr int SF_STAGES = 4;
 constexpr int SF_GROUP = 4;                    // scale blocks per set
 constexpr int SF_BYTES = 512 * 3;              // 128 rows of A, 256 of B, four bytes each
 constexpr int WARP_TMA = 0, WARP_MMA = 1, WARP_SCALE = 2, WARP_EPI = 3;
-constexpr int NUM_THREADS = 32 * (WARP_EPI + 4);
+constexpr int EPI_GROUPS = 2;                  // each drains 128 columns of the tile
+constexpr int NUM_THREADS = 32 * (WARP_EPI + 4 * EPI_GROUPS);
 constexpr int TMEM_COLS = 512, ACC1_COL = 192, SF_COL = 448, SF_COLS = 16, SF_B_OFFSET = 8;
 constexpr unsigned long long WAIT_NS = 4000000000ull;
 
@@ -56,10 +58,11 @@ struct Barriers {
   uint64_t sf_full[SF_STAGES];   // leader: both CTAs' scale warps have written the set
   uint64_t sf_empty[SF_STAGES];  // every CTA: the products that use the set are done
   uint64_t acc_full[2];          // every CTA: accumulator complete
-  uint64_t acc_free;             // leader: the shared columns of the tile's accumulator have been read (eight warps)
+  uint64_t acc_free;             // leader: the shared columns of the tile, and all of the tile before, have been read
+  uint64_t in_full[EPI_GROUPS];  // every CTA: the tile that the epilogue reads (kept activation) has landed in its staging buffer
   uint32_t tmem_base;
   int abort_flag;
-  uint32_t block_max[2][4];      // epilogue: maxima of the four warps, two blocks in flight
+  uint32_t block_max[EPI_GROUPS][2][4];   // epilogue: maxima of a group's four warps, two tiles in flight
 };
 
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * OUT_BYTES + SF_STAGES * SF_BYTES + 512 + 1024;
@@ -74,9 +77,8 @@ struct Args {
   bf16* c;
   const bf16* residual;
   long long ldc, ldr;
-  int direct;                    // rows of C or of the residual do not start on 16 bytes
-  const uint8_t* h_val;          // kept activation, packed like the result
-  const uint8_t* h_exp;
+  int direct;                    // rows of C or of the residual do not start on 16 bytes: no TMA for either
+  const uint8_t* h_exp;          // exponents of the kept activation, packed like the result
   uint8_t* q_exp;
   long long q_ldv, q_lde;        // leading dimensions of the packed result (and of h)
   int* status;
@@ -102,15 +104,31 @@ __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+// Arrive on an mbarrier of either CTA of the pair.  At CTA scope: what is announced is read by the tensor core (shared memory
+// of the writer's own CTA, behind a proxy fence) or has left tensor memory.  A release at cluster scope waits for the
+// thread's earlier stores all the way and costs 1650 cycles between two tiles' products (32768 x 2048 x 8192: 405 -> 490 us).
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.b32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok));
+  return ok != 0;
+}
+// What these barriers announce is read by the tensor core and the copy engine, or lies in tensor memory: an acquire at
+// cluster scope would only slow the issuing warp (NN 32768 x 2048 x 8192: 387 against 381 us).
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n"
       ".reg .pred p;\n"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
       "selp.b32 %0, 1, 0, p;\n"
       "}\n"
       : "=r"(ok)
@@ -139,10 +157,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, Barrie
   if (status) atomicCAS(status, 0, code);
   return false;
 }
+// the same answer in every lane of a warp whose lanes all wait
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Barriers* bars, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, bars, status, code));
+}
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(map), "r"(bar_cluster_addr), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
       : "memory");
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
@@ -199,7 +227,33 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[COUNT]) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// barrier of a group; true if `ok` holds in all its threads
+__device__ __forceinline__ bool epi_all(int group, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.b32 p, %1, 0;\n"
+      "barrier.cta.red.and.pred q, %2, 128, p;\n"
+      "selp.b32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(1 + group)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void epi_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
+// a tile of 128 rows by 128 bytes into a staging buffer, once the store out of that buffer has been read
+__device__ __forceinline__ void fetch_input(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  mbar_expect_tx(bar, OUT_BYTES);
+  tma_load_2d(dst, map, bar, x, y);
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -207,7 +261,8 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& v) {
 template <bool A_MN, bool B_MN, int EPI, int Q_ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ Args g) {
+                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_in,
+                const __grid_constant__ Args g) {
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t raw = smem_u32(smem_dyn);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -229,7 +284,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     for (int s = 0; s < SF_STAGES; ++s) { mbar_init(&bars->sf_full[s], 2); mbar_init(&bars->sf_empty[s], 1); }
     mbar_init(&bars->acc_full[0], 1);
     mbar_init(&bars->acc_full[1], 1);
-    mbar_init(&bars->acc_free, 8);
+    for (int i = 0; i < EPI_GROUPS; ++i) mbar_init(&bars->in_full[i], 1);
+    mbar_init(&bars->acc_free, 2 * 4 * EPI_GROUPS);
     bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -265,7 +321,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
     }
   } else if (warp == WARP_MMA) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {           // the whole warp runs the loop, one elected thread issues: operands stay in uniform registers
       // kind::mxf8f6f4: A and B e4m3 (0), E8M0 scales (bit 23), directions, N = 256, M = 256 across the pair
       constexpr uint32_t idesc = ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(TN >> 3) << 17) | (1u << 23) |
                                  ((uint32_t)((2 * TM) >> 7) << 27);
@@ -275,247 +331,260 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       uint32_t phase = 0, sf_phase = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += n_pairs, ++local) {
-        if (local > 0 && !mbar_wait(&bars->acc_free, (local - 1) & 1, bars, status, 212)) { ok = false; break; }
-        tc_fence_after();
         const uint32_t d_tmem = tmem_base + (local & 1) * ACC1_COL;
         for (int kb = 0; kb < num_kb; ++kb) {
           const uint32_t sfa = tmem_base + SF_COL + sf * SF_COLS, sfb = sfa + SF_B_OFFSET;
           const uint32_t id = kb % SF_GROUP;
-          if (id == 0) {
-            if (!mbar_wait(&bars->sf_full[sf], sf_phase, bars, status, 213)) { ok = false; break; }
+          if (id == 0) {       // (a tile's first set does not wait for the accumulator)
+            if (!warp_wait(&bars->sf_full[sf], sf_phase, bars, status, 213)) { ok = false; break; }
             tc_fence_after();
-            const uint32_t src = sf_stage + sf * SF_BYTES;
-            scales_to_tmem(sfa, scale_desc(src));
-            scales_to_tmem(sfb, scale_desc(src + 512));
-            scales_to_tmem(sfb + 4, scale_desc(src + 1024));
+            if (elect_one()) {
+              const uint32_t src = sf_stage + sf * SF_BYTES;
+              scales_to_tmem(sfa, scale_desc(src));
+              scales_to_tmem(sfb, scale_desc(src + 512));
+              scales_to_tmem(sfb + 4, scale_desc(src + 1024));
+            }
+            __syncwarp();
           }
-          if (!mbar_wait(&bars->full[stage], phase, bars, status, 214)) { ok = false; break; }
+          if (!warp_wait(&bars->full[stage], phase, bars, status, 214)) { ok = false; break; }
+          if (kb == 0 && local > 0 && !warp_wait(&bars->acc_free, (local - 1) & 1, bars, status, 212)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = base + stage * STAGE_BYTES;
-          const uint64_t adesc = operand_desc(sa), bdesc = operand_desc(sa + OP_BYTES);
-          const uint32_t desc = idesc | (id << 4) | (id << 29);
+          if (elect_one()) {
+            const uint32_t sa = base + stage * STAGE_BYTES;
+            const uint64_t adesc = operand_desc(sa), bdesc = operand_desc(sa + OP_BYTES);
+            const uint32_t desc = idesc | (id << 4) | (id << 29);
 #pragma unroll
-          for (int k = 0; k < TK / 32; ++k)
-            umma_pair(d_tmem, adesc + (uint64_t)(k * a_adv), bdesc + (uint64_t)(k * b_adv), desc, sfa, sfb, (kb | k) ? 1u : 0u);
-          umma_commit_pair(&bars->empty[stage]);
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
-          if (id == SF_GROUP - 1 || kb == num_kb - 1) {
-            umma_commit_pair(&bars->sf_empty[sf]);
-            if (++sf == SF_STAGES) { sf = 0; sf_phase ^= 1; }
+            for (int k = 0; k < TK / 32; ++k)
+              umma_pair(d_tmem, adesc + (uint64_t)(k * a_adv), bdesc + (uint64_t)(k * b_adv), desc, sfa, sfb, (kb | k) ? 1u : 0u);
+            umma_commit_pair(&bars->empty[stage]);
+            if (id == SF_GROUP - 1 || kb == num_kb - 1) umma_commit_pair(&bars->sf_empty[sf]);
+            if (kb == num_kb - 1) umma_commit_pair(&bars->acc_full[local & 1]);
           }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (id == SF_GROUP - 1 || kb == num_kb - 1)
+            if (++sf == SF_STAGES) { sf = 0; sf_phase ^= 1; }
         }
-        if (ok) umma_commit_pair(&bars->acc_full[local & 1]);
       }
     }
   } else if (warp == WARP_SCALE) {
     // Sets of scales: word r of an operand holds the bytes of rows r (128 of A, 256 of B) for four blocks of the
     // contraction; word r goes to lane r % 32, column r / 32.
+    const bool by_row = !A_MN && g.a_rows == 1;
+    const int sets = (num_kb + SF_GROUP - 1) / SF_GROUP;
     int sf = 0;
     uint32_t sf_phase = 0;
-    bool ok = true;
-    for (int tile = pair; tile < num_tiles && ok; tile += n_pairs) {
+    // lanes 0-3: A, 4-7 and 8-11: the two column blocks of B; blocks of one row: four rows a lane
+    auto fetch = [&](int tile, int set, uint32_t& byte, uint32_t (&rows4)[4]) {
       const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM, n0 = (tile % tiles_n) * TN;
-      for (int kb0 = 0; kb0 < num_kb; kb0 += SF_GROUP) {
-        // lanes 0-3: A, 4-7 and 8-11: the two column blocks of B
-        uint32_t byte = 0;
-        const int which = lane >> 2, kb = kb0 + (lane & 3);
-        if (kb < num_kb) {
-          if (which == 0 && g.a_rows == 128 && m0 < M) byte = g.a_exp[(long long)(m0 >> 7) * g.a_sm + (long long)kb * g.a_sk];
-          if ((which == 1 || which == 2) && n0 + (which - 1) * 128 < N)
-            byte = g.b_exp[(long long)((n0 >> 7) + which - 1) * g.b_sn + (long long)kb * g.b_sk];
-        }
-        uint32_t rows4[4] = {0, 0, 0, 0};
-        if (!A_MN && g.a_rows == 1) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (kb0 + i < num_kb && m0 + 4 * lane < g.a_ld)
-              rows4[i] = __ldg(reinterpret_cast<const uint32_t*>(g.a_exp + (long long)(kb0 + i) * g.a_ld + m0 + 4 * lane));
-        }
-        if (!mbar_wait(&bars->sf_empty[sf], sf_phase ^ 1, bars, status, 215)) { ok = false; break; }
-        byte <<= 8 * (lane & 3);
-        byte |= __shfl_xor_sync(0xffffffffu, byte, 1);
-        byte |= __shfl_xor_sync(0xffffffffu, byte, 2);
-        const uint32_t wa = __shfl_sync(0xffffffffu, byte, 0), wb0 = __shfl_sync(0xffffffffu, byte, 4),
-                       wb1 = __shfl_sync(0xffffffffu, byte, 8);
-        const uint32_t dst = sf_stage + sf * SF_BYTES;
-        if (!A_MN && g.a_rows == 1) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {      // word of row 4 * lane + i: byte i of the four blocks
-            const uint32_t lo = __byte_perm(rows4[0], rows4[1], i | ((4 + i) << 4));
-            const uint32_t hi = __byte_perm(rows4[2], rows4[3], i | ((4 + i) << 4));
-            const int r = 4 * lane + i;
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (r & 31) * 16 + (r >> 5) * 4), "r"(__byte_perm(lo, hi, 0x5410))
-                         : "memory");
-          }
-        } else {
-          st_shared16(dst + lane * 16, make_uint4(wa, wa, wa, wa));
-        }
-        st_shared16(dst + 512 + lane * 16, make_uint4(wb0, wb0, wb0, wb0));
-        st_shared16(dst + 1024 + lane * 16, make_uint4(wb1, wb1, wb1, wb1));
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&bars->sf_full[sf]), 0));
-        if (++sf == SF_STAGES) { sf = 0; sf_phase ^= 1; }
+      const int which = lane >> 2, kb = set * SF_GROUP + (lane & 3);
+      byte = 0;
+      if (kb < num_kb) {
+        if (which == 0 && !by_row && m0 < M) byte = __ldg(g.a_exp + (long long)(m0 >> 7) * g.a_sm + (long long)kb * g.a_sk);
+        if ((which == 1 || which == 2) && n0 + (which - 1) * 128 < N)
+          byte = __ldg(g.b_exp + (long long)((n0 >> 7) + which - 1) * g.b_sn + (long long)kb * g.b_sk);
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        rows4[i] = 0;
+        if (by_row && set * SF_GROUP + i < num_kb && m0 + 4 * lane < g.a_ld)
+          rows4[i] = __ldg(reinterpret_cast<const uint32_t*>(g.a_exp + (long long)(set * SF_GROUP + i) * g.a_ld + m0 + 4 * lane));
+      }
+    };
+    uint32_t next_byte, next_rows[4];
+    int tile = pair, set = 0;
+    if (tile < num_tiles) fetch(tile, 0, next_byte, next_rows);
+    while (tile < num_tiles) {
+      uint32_t byte = next_byte, rows4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rows4[i] = next_rows[i];
+      if (++set == sets) { set = 0; tile += n_pairs; }
+      if (tile < num_tiles) fetch(tile, set, next_byte, next_rows);      // one set ahead of the one that is written
+      if (!warp_wait(&bars->sf_empty[sf], sf_phase ^ 1, bars, status, 215)) break;
+      byte <<= 8 * (lane & 3);
+      byte |= __shfl_xor_sync(0xffffffffu, byte, 1);
+      byte |= __shfl_xor_sync(0xffffffffu, byte, 2);
+      const uint32_t wa = __shfl_sync(0xffffffffu, byte, 0), wb0 = __shfl_sync(0xffffffffu, byte, 4),
+                     wb1 = __shfl_sync(0xffffffffu, byte, 8);
+      const uint32_t dst = sf_stage + sf * SF_BYTES;
+      if (by_row) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {      // word of row 4 * lane + i: byte i of the four blocks
+          const uint32_t lo = __byte_perm(rows4[0], rows4[1], i | ((4 + i) << 4));
+          const uint32_t hi = __byte_perm(rows4[2], rows4[3], i | ((4 + i) << 4));
+          const int r = 4 * lane + i;
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (r & 31) * 16 + (r >> 5) * 4), "r"(__byte_perm(lo, hi, 0x5410))
+                       : "memory");
+        }
+      } else {
+        st_shared16(dst + lane * 16, make_uint4(wa, wa, wa, wa));
+      }
+      st_shared16(dst + 512 + lane * 16, make_uint4(wb0, wb0, wb0, wb0));
+      st_shared16(dst + 1024 + lane * 16, make_uint4(wb1, wb1, wb1, wb1));
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(map_to_cta(smem_u32(&bars->sf_full[sf]), 0));
+      if (++sf == SF_STAGES) { sf = 0; sf_phase ^= 1; }
     }
   } else {
     const int quarter = warp & 3;                 // tensor-memory lanes [32q, 32q + 32)
     const int row = quarter * 32 + lane;          // row of this CTA's 128 owned by this thread
-    const bool elected = threadIdx.x == 32 * WARP_EPI;
-    int local = 0, buf = 0;
+    const int group = (warp - WARP_EPI) >> 2;     // columns [128 * group, 128 * group + 128) of the tile
+    const bool elected = threadIdx.x == 32 * (WARP_EPI + 4 * group);
+    const uint32_t stage_addr = out_stage + group * OUT_BYTES;
+    const uint32_t free_leader = map_to_cta(smem_u32(&bars->acc_free), 0);
+    int local = 0;
     for (int tile = pair; tile < num_tiles; tile += n_pairs, ++local) {
-      const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM, n0 = (tile % tiles_n) * TN;
+      const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM, gn0 = (tile % tiles_n) * TN + group * 128;
       const int gm = m0 + row;
       const int acc = local & 1;
-      mbar_wait(&bars->acc_full[acc], (local >> 1) & 1, bars, status, 216);
-      epi_sync();
-      if (*reinterpret_cast<volatile int*>(&bars->abort_flag)) break;
+      const bool shared_columns = group != acc;    // accumulator 0 shares its last 64 columns, accumulator 1 its first
+      // What the epilogue reads - the kept activation, or the first half of the residual - is fetched while the products run
+      // and replaced in place by the result.
+      const bool residual_by_tma = EPI == EPI_RESIDUAL && !g.direct;
+      if ((EPI == EPI_RELU_SQ_GRAD || residual_by_tma) && elected)
+        fetch_input(stage_addr, &map_in, &bars->in_full[group], gn0 + (EPI == EPI_RESIDUAL && acc == 0 ? 64 : 0), m0);
+      if (!epi_all(group, mbar_wait(&bars->acc_full[acc], (local >> 1) & 1, bars, status, 216))) break;
       tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * ACC1_COL;
-      const uint32_t free_leader = map_to_cta(smem_u32(&bars->acc_free), 0);
+      // a group without shared columns arrives at once: it has read all of the tile before
+      if (!shared_columns && lane == 0) mbar_arrive_at(free_leader);
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * ACC1_COL + group * 128;
       if constexpr (EPI == EPI_STORE || EPI == EPI_RESIDUAL) {
 #pragma unroll 1
-        for (int i = 0; i < TN / 64; ++i) {
-          const int chunk = acc == 0 ? TN / 64 - 1 - i : i;      // the columns shared with the other accumulator first
-          const int gn0 = n0 + chunk * 64;
+        for (int i = 0; i < 2; ++i) {
+          const int chunk = acc == 0 ? 1 - i : i;      // the columns shared with the other accumulator first
+          const int c0 = gn0 + chunk * 64;
           uint32_t v[64];
           tmem_ld32(t_row + chunk * 64, v);
           tmem_ld32(t_row + chunk * 64 + 32, v + 32);
-          uint4 cin[EPI == EPI_RESIDUAL ? 8 : 1];
-          if (EPI == EPI_RESIDUAL) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              cin[j] = make_uint4(0u, 0u, 0u, 0u);
-              if (gm < M && gn0 + j * 8 < N) {
-                const bf16* p = g.residual + (long long)gm * g.ldr + gn0 + j * 8;
-                if (!g.direct) {
-                  cin[j] = __ldcs(reinterpret_cast<const uint4*>(p));
-                } else {
-                  float t[8];
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) t[e] = gn0 + j * 8 + e < N ? __bfloat162float(p[e]) : 0.f;
-                  cin[j] = pack8(t);
-                }
-              }
-            }
-          }
+          if (residual_by_tma && i == 1 && elected) fetch_input(stage_addr, &map_in, &bars->in_full[group], c0, m0);
           tmem_wait_ld(v);
-          if (i == 0) {
+          if (i == 0 && shared_columns) {
             tc_fence_before();
-            if (lane == 0) mbar_arrive_cluster(free_leader);
+            if (lane == 0) mbar_arrive_at(free_leader);
           }
-          if (elected) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          epi_sync();
-          const uint32_t stage_addr = out_stage + buf * OUT_BYTES;
+          if (residual_by_tma) {
+            if (!epi_all(group, mbar_wait(&bars->in_full[group], i, bars, status, 217))) break;
+          } else {
+            if (elected) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            epi_sync(group);
+          }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            float f[8], prev[8];
-            if (EPI == EPI_RESIDUAL) unpack8(cin[j], prev);
+            const uint32_t at = stage_addr + row * 128 + ((j ^ (row & 7)) << 4);
+            float f[8];
+            if (residual_by_tma) {
+              unpack8(ld_shared16(at), f);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j * 8 + e]) + (EPI == EPI_RESIDUAL ? prev[e] : 0.f);
-            st_shared16(stage_addr + row * 128 + ((j ^ (row & 7)) << 4), pack8(f));
+              for (int e = 0; e < 8; ++e)
+                f[e] = EPI == EPI_RESIDUAL && gm < M && c0 + j * 8 + e < N
+                           ? __bfloat162float(g.residual[(long long)gm * g.ldr + c0 + j * 8 + e]) : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] += __uint_as_float(v[j * 8 + e]);
+            st_shared16(at, pack8(f));
           }
           if (!g.direct) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            epi_sync();
-            if (elected && m0 < M) {
-              tma_store_2d(&map_out, stage_addr, gn0, m0);
+            epi_sync(group);
+            if (elected && m0 < M && c0 < N) {
+              tma_store_2d(&map_out, stage_addr, c0, m0);
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
           } else {                                                // unaligned rows: copied out value by value
-            epi_sync();
+            epi_sync(group);
             for (int r = quarter; r < TM && m0 + r < M; r += 4)
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const int col = lane + h * 32;
                 uint16_t val;
                 asm volatile("ld.shared.u16 %0, [%1];" : "=h"(val)
-                             : "r"(stage_addr + r * 128 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2));
-                if (gn0 + col < N) reinterpret_cast<uint16_t*>(g.c)[(long long)(m0 + r) * g.ldc + gn0 + col] = val;
+                             : "r"(stage_addr + r * 128 + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2)
+                             : "memory");
+                if (c0 + col < N) reinterpret_cast<uint16_t*>(g.c)[(long long)(m0 + r) * g.ldc + c0 + col] = val;
               }
           }
-          buf ^= 1;
         }
       } else {
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          const int half = acc == 0 ? 1 - i : i;
-          const int gn0 = n0 + half * 128, nb = gn0 >> 7;
-          uint32_t v[128];
-          uint4 hv[EPI == EPI_RELU_SQ_GRAD ? 8 : 1];
-          uint32_t he = 0;
+        const int nb = gn0 >> 7;
+        const bool partial = m0 + TM > M || gn0 + 128 > N;
+        float c_in = 1.f, c_out = 0.f;             // 2 sqrt(q 2^s) = c_out sqrt(c_in q)
+        if (EPI == EPI_RELU_SQ_GRAD && gm < M && gn0 < N) {
+          const uint32_t he = Q_ROWS == 1 ? g.h_exp[(long long)nb * g.q_lde + gm] : g.h_exp[(long long)(m0 >> 7) * g.q_lde + nb];
+          const int s = (int)he - 127;
+          c_in = s & 1 ? 2.f : 1.f;
+          c_out = __uint_as_float((uint32_t)((s >> 1) + 1 + 127) << 23);
+        }
+        uint32_t v[128];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tmem_ld32(t_row + j * 32, v + j * 32);
+        tmem_wait_ld(v);
+        if (shared_columns) {
+          tc_fence_before();
+          if (lane == 0) mbar_arrive_at(free_leader);
+        }
+        if (EPI == EPI_RELU_SQ_GRAD && !epi_all(group, mbar_wait(&bars->in_full[group], local & 1, bars, status, 217))) break;
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float h[16];
           if (EPI == EPI_RELU_SQ_GRAD) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              hv[j] = gm < M && gn0 + j * 16 < g.q_ldv
-                          ? __ldcs(reinterpret_cast<const uint4*>(g.h_val + (long long)gm * g.q_ldv + gn0 + j * 16))
-                          : make_uint4(0u, 0u, 0u, 0u);
-            if (gm < M && gn0 < N)
-              he = Q_ROWS == 1 ? g.h_exp[(long long)nb * g.q_lde + gm] : g.h_exp[(long long)(m0 >> 7) * g.q_lde + nb];
+            const uint4 q = ld_shared16(stage_addr + row * 128 + ((j ^ (row & 7)) << 4));
+            fp8_unpack4(q.x, h); fp8_unpack4(q.y, h + 4); fp8_unpack4(q.z, h + 8); fp8_unpack4(q.w, h + 12);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) tmem_ld32(t_row + half * 128 + j * 32, v + j * 32);
-          tmem_wait_ld(v);
-          if (i == 0) {
-            tc_fence_before();
-            if (lane == 0) mbar_arrive_cluster(free_leader);
-          }
-          uint32_t top = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float h[16];
-            if (EPI == EPI_RELU_SQ_GRAD) {
-              fp8_unpack4(hv[j].x, h); fp8_unpack4(hv[j].y, h + 4); fp8_unpack4(hv[j].z, h + 8); fp8_unpack4(hv[j].w, h + 12);
+          for (int e = 0; e < 16; ++e) {
+            float x = __uint_as_float(v[j * 16 + e]);
+            if (EPI == EPI_RELU_SQ) {
+              x = x < 0.f ? 0.f : x;             // a NaN stays one
+              x *= x;
+            } else {
+              x *= c_out * sqrtf(h[e] * c_in);
             }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float x = __uint_as_float(v[j * 16 + e]);
-              if (EPI == EPI_RELU_SQ) {
-                x = x < 0.f ? 0.f : x;             // a NaN stays one
-                x *= x;
-              } else {
-                x *= 2.f * sqrtf(fp8_scaled(h[e], he));
-              }
-              if (gm >= M || gn0 + j * 16 + e >= N) x = 0.f;
-              v[j * 16 + e] = __float_as_uint(x);
-              top = max(top, __float_as_uint(x) & 0x7fffffffu);
-            }
+            v[j * 16 + e] = __float_as_uint(x);
           }
-          if (Q_ROWS == 128) {
+        }
+        if (partial) {
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (lane == 0) bars->block_max[buf][quarter] = top;
-          }
-          if (elected) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          epi_sync();
-          if (Q_ROWS == 128)
-            top = max(max(bars->block_max[buf][0], bars->block_max[buf][1]), max(bars->block_max[buf][2], bars->block_max[buf][3]));
-          const uint32_t e = fp8_block_exponent(top);
-          const float s = fp8_inverse_scale(e == 255u ? 127u : e);
-          const uint32_t stage_addr = out_stage + buf * OUT_BYTES;
+          for (int e = 0; e < 128; ++e)
+            if (gm >= M || gn0 + e >= N) v[e] = 0u;
+        }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint32_t w[4];
+        for (int e = 0; e < 128; ++e) top = max(top, v[e] & 0x7fffffffu);
+        if (Q_ROWS == 128) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const uint32_t* p = v + j * 16 + t * 4;
-              w[t] = e == 255u ? 0x7f7f7f7fu
-                               : fp8_pack4(__uint_as_float(p[0]) * s, __uint_as_float(p[1]) * s, __uint_as_float(p[2]) * s,
-                                           __uint_as_float(p[3]) * s);
-            }
-            st_shared16(stage_addr + row * 128 + ((j ^ (row & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+          for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (lane == 0) bars->block_max[group][acc][quarter] = top;
+        }
+        if (EPI == EPI_RELU_SQ && elected) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        epi_sync(group);
+        if (Q_ROWS == 128) {
+          const uint32_t* b = bars->block_max[group][acc];
+          top = max(max(b[0], b[1]), max(b[2], b[3]));
+        }
+        const uint32_t e = fp8_block_exponent(top);
+        const float s = fp8_inverse_scale(e == 255u ? 127u : e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t w[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t* p = v + j * 16 + t * 4;
+            w[t] = fp8_pack4(__uint_as_float(p[0]) * s, __uint_as_float(p[1]) * s, __uint_as_float(p[2]) * s, __uint_as_float(p[3]) * s);
+            if (e == 255u) w[t] = 0x7f7f7f7fu;
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          epi_sync();
-          if (m0 < M && gn0 < N) {
-            if (elected) {
-              tma_store_2d(&map_out, stage_addr, gn0, m0);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-              if (Q_ROWS == 128) g.q_exp[(long long)(m0 >> 7) * g.q_lde + nb] = (uint8_t)e;
-            }
-            if (Q_ROWS == 1 && gm < M) g.q_exp[(long long)nb * g.q_lde + gm] = (uint8_t)e;
+          st_shared16(stage_addr + row * 128 + ((j ^ (row & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        epi_sync(group);
+        if (m0 < M && gn0 < N) {
+          if (elected) {
+            tma_store_2d(&map_out, stage_addr, gn0, m0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            if (Q_ROWS == 128) g.q_exp[(long long)(m0 >> 7) * g.q_lde + nb] = (uint8_t)e;
           }
-          buf ^= 1;
+          if (Q_ROWS == 1 && gm < M) g.q_exp[(long long)nb * g.q_lde + gm] = (uint8_t)e;
         }
       }
     }
@@ -555,7 +624,7 @@ int encode(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* ptr
 }
 
 template <bool A_MN, bool B_MN, int EPI, int Q_ROWS>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Args& g, cudaStream_t st) {
+int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const CUtensorMap& mi, const Args& g, cudaStream_t st) {
   auto kern = gemm_fp8_kernel<A_MN, B_MN, EPI, Q_ROWS>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -571,7 +640,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
   const long long tiles = (long long)((g.M + 2 * TM - 1) / (2 * TM)) * ((g.N + TN - 1) / TN);
   if (tiles > 0x3fffffff) return RWKV_ERR_TOO_LARGE;
   const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
-  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, st>>>(ma, mb, mo, g);
+  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, st>>>(ma, mb, mo, mi, g);
   return rwkv_launch_status();
 }
 
@@ -594,7 +663,7 @@ int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t st) {
                     : (!s.q_val || !s.q_exp || !(q_rows == 1 || q_rows == 128) ||
                        (epilogue == 3 && (!s.h_val || !s.h_exp || ((uintptr_t)s.h_val & 15)))))
     return RWKV_ERR_BAD_SHAPE;
-  CUtensorMap ma, mb, mo;
+  CUtensorMap ma, mb, mo, mi;
   const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int r = a_mn ? encode(&ma, u8, 1, s.a_val, K, M, up(M, 16)) : encode(&ma, u8, 1, s.a_val, M, K, up(K, 16));
   if (r) return r;
@@ -609,12 +678,12 @@ int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t st) {
   g.a_sm = a_mn ? 1 : kb_n; g.a_sk = a_mn ? mb_n : 1;
   g.b_sn = b_mn ? 1 : kb_n; g.b_sk = b_mn ? nb_n : 1;
   g.c = (bf16*)s.c; g.residual = (const bf16*)s.residual; g.ldc = s.ldc; g.ldr = s.ldr;
-  g.h_val = (const uint8_t*)s.h_val; g.h_exp = (const uint8_t*)s.h_exp; g.q_exp = (uint8_t*)s.q_exp;
+  g.h_exp = (const uint8_t*)s.h_exp; g.q_exp = (uint8_t*)s.q_exp;
   g.q_ldv = up(N, 16);
   g.q_lde = q_rows == 1 ? up(M, 16) : nb_n;
   g.status = (int*)s.status;
   if (epilogue <= 1) {
-    g.direct = ((uintptr_t)s.c & 15) || (s.ldc & 7) || (epilogue == 1 && (((uintptr_t)s.residual & 15) || (s.ldr & 7) || (N & 7)));
+    g.direct = ((uintptr_t)s.c & 15) || (s.ldc & 7) || (epilogue == 1 && (((uintptr_t)s.residual & 15) || (s.ldr & 7)));
     if (g.direct) {
       mo = ma;               // never read
     } else {
@@ -624,20 +693,24 @@ int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t st) {
     r = encode(&mo, u8, 1, s.q_val, M, N, g.q_ldv);
   }
   if (r) return r;
+  mi = mo;
+  if (epilogue == 3) r = encode(&mi, u8, 1, s.h_val, M, N, g.q_ldv);
+  if (epilogue == 1 && !g.direct) r = encode(&mi, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, s.residual, M, N, s.ldr);
+  if (r) return r;
   if (epilogue == 2) {
     if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
-    return q_rows == 1 ? launch<false, false, EPI_RELU_SQ, 1>(ma, mb, mo, g, st) : launch<false, false, EPI_RELU_SQ, 128>(ma, mb, mo, g, st);
+    return q_rows == 1 ? launch<false, false, EPI_RELU_SQ, 1>(ma, mb, mo, mi, g, st) : launch<false, false, EPI_RELU_SQ, 128>(ma, mb, mo, mi, g, st);
   }
   if (epilogue == 3) {
     if (a_mn || !b_mn) return RWKV_ERR_BAD_SHAPE;
-    return q_rows == 1 ? launch<false, true, EPI_RELU_SQ_GRAD, 1>(ma, mb, mo, g, st)
-                       : launch<false, true, EPI_RELU_SQ_GRAD, 128>(ma, mb, mo, g, st);
+    return q_rows == 1 ? launch<false, true, EPI_RELU_SQ_GRAD, 1>(ma, mb, mo, mi, g, st)
+                       : launch<false, true, EPI_RELU_SQ_GRAD, 128>(ma, mb, mo, mi, g, st);
   }
   if (epilogue == 1) {
     if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
-    return launch<false, false, EPI_RESIDUAL, 0>(ma, mb, mo, g, st);
+    return launch<false, false, EPI_RESIDUAL, 0>(ma, mb, mo, mi, g, st);
   }
-  if (a_mn && b_mn) return launch<true, true, EPI_STORE, 0>(ma, mb, mo, g, st);
+  if (a_mn && b_mn) return launch<true, true, EPI_STORE, 0>(ma, mb, mo, mi, g, st);
   if (a_mn) return RWKV_ERR_BAD_SHAPE;
-  return b_mn ? launch<false, true, EPI_STORE, 0>(ma, mb, mo, g, st) : launch<false, false, EPI_STORE, 0>(ma, mb, mo, g, st);
+  return b_mn ? launch<false, true, EPI_STORE, 0>(ma, mb, mo, mi, g, st) : launch<false, false, EPI_STORE, 0>(ma, mb, mo, mi, g, st);
 }
