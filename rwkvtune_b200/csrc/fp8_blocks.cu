@@ -1,11 +1,12 @@
 // Packing to and from the 8-bit block format (fp8_format.cuh): activation checkpoints, and the operands of the 8-bit GEMMs.
 //
-// Both directions are bound by memory: 2 + 1 bytes a value for bf16.  A thread owns 16 neighbouring values (two 16-byte
-// loads, one 16-byte store for bf16), eight threads a block of 128 columns.  The values stay in registers between the
-// maximum and the rounding, so the input is read once:
-//   rows = 1  : the maximum is three shuffles among the eight threads of a block;
-//   rows = 128: a CTA of 512 threads owns a tile, 32 values a thread; warp maxima meet in shared memory.
-// Loads and stores take the widest of 16 / 8 / 4 / 2 bytes that the row pitch and the address allow.
+// Both directions are bound by memory: 2 + 1 bytes a value for bf16.  Eight threads own the 128 columns of a block's row, 16
+// values each, in pieces as wide as the row pitch and the address allow (32 to 2 bytes), neighbouring threads on
+// neighbouring pieces.  The values stay in registers between the maximum and the rounding, so the input is read once:
+//   rows = 1  : the maximum is three shuffles among the eight threads; one block a thread and many CTAs (two or four blocks
+//               a thread in flight were slower: 32768 x 2048 in 35.0, 39.1 and 46.0 us);
+//   rows = 128: a CTA of 512 threads walks over tiles with the next one's loads in flight; warp maxima meet in shared
+//               memory (one CTA a tile: 43.2 us, walking: 33.3 us, 6.06 TB/s).
 //
 // Arithmetic in the rest of the library flushes numbers below 2^-126 to zero, and so do these kernels.
 #include <cuda_fp16.h>
@@ -26,45 +27,111 @@ template <typename T> __device__ __forceinline__ float largest();
 template <> __device__ __forceinline__ float largest<bf16>() { return 3.3895313892515355e38f; }
 template <> __device__ __forceinline__ float largest<__half>() { return 65504.f; }
 template <> __device__ __forceinline__ float largest<float>() { return 3.4028234663852886e38f; }
+// smallest exponent byte of a block with a value of T's largest power of two or more: 256 * 2^(E - 127) reaches it
+template <typename T> __device__ __forceinline__ constexpr uint32_t first_overflow() { return 127 + 127 - 8; }
+template <> __device__ __forceinline__ constexpr uint32_t first_overflow<__half>() { return 127 + 15 - 8; }
 
-template <int BYTES> struct Word;
-template <> struct Word<2> { typedef uint16_t type; };
-template <> struct Word<4> { typedef uint32_t type; };
-template <> struct Word<8> { typedef uint2 type; };
-template <> struct Word<16> { typedef uint4 type; };
+// 16 neighbouring values as they lie in memory
+template <typename T> struct Raw16 {
+  union {
+    uint32_t w[4 * sizeof(T)];
+    T t[16];
+  };
+};
+template <int V> __device__ __forceinline__ void load_word(const void* p, uint32_t* w);
+template <> __device__ __forceinline__ void load_word<4>(const void* p, uint32_t* w) { w[0] = __ldcs((const uint32_t*)p); }
+template <> __device__ __forceinline__ void load_word<8>(const void* p, uint32_t* w) {
+  const uint2 v = __ldcs((const uint2*)p);
+  w[0] = v.x; w[1] = v.y;
+}
+template <> __device__ __forceinline__ void load_word<16>(const void* p, uint32_t* w) {
+  const uint4 v = __ldcs((const uint4*)p);
+  w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+}
+template <> __device__ __forceinline__ void load_word<32>(const void* p, uint32_t* w) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+template <int V> __device__ __forceinline__ void store_word(void* p, const uint32_t* w);
+template <> __device__ __forceinline__ void store_word<4>(void* p, const uint32_t* w) { *(uint32_t*)p = w[0]; }
+template <> __device__ __forceinline__ void store_word<8>(void* p, const uint32_t* w) { *(uint2*)p = make_uint2(w[0], w[1]); }
+template <> __device__ __forceinline__ void store_word<16>(void* p, const uint32_t* w) {
+  *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <> __device__ __forceinline__ void store_word<32>(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 
-// 16 values from p, the first n of them in range (n may be <= 0 or above 16); V: bytes of one load
+// A thread's 16 values of a block's row: pieces of PER values, piece i of thread `part` at (8 i + part) PER.
+// The first n values of the row are in range (n may be <= 0 or above 128), the others read as zero.
 template <typename T, int V>
-__device__ __forceinline__ void load16(const T* p, int n, float* f) {
+__device__ __forceinline__ void load16(const T* p, int part, int n, Raw16<T>& r) {
   constexpr int PER = V / (int)sizeof(T);
-  union { typename Word<V>::type w[16 / PER]; T t[16]; } u;
 #pragma unroll
   for (int i = 0; i < 16 / PER; ++i) {
-    if ((i + 1) * PER <= n) {
-      u.w[i] = __ldcs(reinterpret_cast<const typename Word<V>::type*>(p) + i);
+    const int at = (8 * i + part) * PER;
+    if (V > 2 && at + PER <= n) {
+      load_word<(V > 2 ? V : 4)>(p + at, r.w + i * V / 4);
     } else {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) u.t[i * PER + j] = i * PER + j < n ? p[i * PER + j] : from_f32<T>(0.f);
+      for (int j = 0; j < PER; ++j) r.t[i * PER + j] = at + j < n ? p[at + j] : from_f32<T>(0.f);
     }
   }
+}
+template <typename T>
+__device__ __forceinline__ void widen16(const Raw16<T>& r, float* f) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = to_f32(u.t[i]);
+  for (int i = 0; i < 16; ++i) f[i] = to_f32(r.t[i]);
 }
 template <typename T, int V>
-__device__ __forceinline__ void store16(T* p, int n, const float* f) {
+__device__ __forceinline__ void store16(T* p, int part, int n, const float* f) {
   constexpr int PER = V / (int)sizeof(T);
-  union { typename Word<V>::type w[16 / PER]; T t[16]; } u;
+  Raw16<T> r;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) u.t[i] = from_f32<T>(f[i]);
+  for (int i = 0; i < 16; ++i) r.t[i] = from_f32<T>(f[i]);
 #pragma unroll
   for (int i = 0; i < 16 / PER; ++i) {
-    if ((i + 1) * PER <= n) {
-      reinterpret_cast<typename Word<V>::type*>(p)[i] = u.w[i];
+    const int at = (8 * i + part) * PER;
+    if (V > 2 && at + PER <= n) {
+      store_word<(V > 2 ? V : 4)>(p + at, r.w + i * V / 4);
     } else {
 #pragma unroll
       for (int j = 0; j < PER; ++j)
-        if (i * PER + j < n) p[i * PER + j] = u.t[i * PER + j];
+        if (at + j < n) p[at + j] = r.t[i * PER + j];
     }
+  }
+}
+// the same pieces of a packed row, n columns of which exist (a multiple of 16)
+union Packed16 {
+  uint32_t w[4];
+  uint16_t h[8];
+  uint8_t b[16];
+};
+template <int PER>
+__device__ __forceinline__ void store_packed(uint8_t* p, int part, int n, const Packed16& q) {
+#pragma unroll
+  for (int i = 0; i < 16 / PER; ++i) {
+    const int at = (8 * i + part) * PER;
+    if (at >= n) continue;
+    if constexpr (PER >= 4) store_word<(PER >= 4 ? PER : 4)>(p + at, q.w + i * PER / 4);
+    if constexpr (PER == 2) *reinterpret_cast<uint16_t*>(p + at) = q.h[i];
+    if constexpr (PER == 1) p[at] = q.b[i];
+  }
+}
+template <int PER>
+__device__ __forceinline__ void load_packed(const uint8_t* p, int part, int n, Packed16& q) {
+#pragma unroll
+  for (int i = 0; i < 16 / PER; ++i) {
+    const int at = (8 * i + part) * PER;
+    const bool live = at < n;
+    if constexpr (PER >= 4) {
+      if (live) load_word<(PER >= 4 ? PER : 4)>(p + at, q.w + i * PER / 4);
+    }
+    if constexpr (PER == 2) q.h[i] = live ? *reinterpret_cast<const uint16_t*>(p + at) : 0;
+    if constexpr (PER == 1) q.b[i] = live ? p[at] : 0;
   }
 }
 
@@ -74,11 +141,13 @@ __device__ __forceinline__ uint32_t abs_bits16(const float* f) {
   for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
   return m;
 }
-__device__ __forceinline__ uint4 quantise16(const float* f, uint32_t e) {
-  if (e == 255u) return make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-  const float s = fp8_inverse_scale(e);
-  return make_uint4(fp8_pack4(f[0] * s, f[1] * s, f[2] * s, f[3] * s), fp8_pack4(f[4] * s, f[5] * s, f[6] * s, f[7] * s),
-                    fp8_pack4(f[8] * s, f[9] * s, f[10] * s, f[11] * s), fp8_pack4(f[12] * s, f[13] * s, f[14] * s, f[15] * s));
+__device__ __forceinline__ Packed16 quantise16(const float* f, uint32_t e) {
+  Packed16 q;
+  const float s = fp8_inverse_scale(e == 255u ? 127u : e);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q.w[i] = e == 255u ? 0x7f7f7f7fu : fp8_pack4(f[4 * i] * s, f[4 * i + 1] * s, f[4 * i + 2] * s, f[4 * i + 3] * s);
+  return q;
 }
 
 constexpr int ROW_THREADS = 256;
@@ -86,24 +155,31 @@ constexpr int ROW_THREADS = 256;
 template <typename T, int V>
 __global__ void __launch_bounds__(ROW_THREADS)
 fp8_pack_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
-                     int R, int C, int ldv, int lde, int blocks) {
+                     uint32_t units, int C, int ldv, int lde, uint32_t blocks) {
   rwkv_chain_trigger();       // a chained decode product may fetch its weights meanwhile
-  const long long units = (long long)R * blocks, stride = (long long)gridDim.x * (ROW_THREADS / 8);
   const int part = threadIdx.x & 7;
-  const long long rounds = (units + stride - 1) / stride;          // the same for every thread: the shuffles need whole warps
-  long long u = (long long)blockIdx.x * (ROW_THREADS / 8) + (threadIdx.x >> 3);
-  for (long long i = 0; i < rounds; ++i, u += stride) {
-    const bool live = u < units;
-    const int row = live ? (int)(u / blocks) : 0, kb = live ? (int)(u % blocks) : 0;
-    const int col = kb * FP8_BLOCK + part * 16;
+  const uint32_t step = gridDim.x * (ROW_THREADS / 8);
+  Raw16<T> next;
+  auto fetch = [&](uint32_t u) {
+    const uint32_t row = u < units ? u / blocks : 0, col = u < units ? (u - row * blocks) * FP8_BLOCK : 0;
+    load16<T, V>(x + row * ldx + col, part, u < units ? C - (int)col : 0, next);
+  };
+  // the first block of a warp decides for all of it: the shuffles need whole warps
+  uint32_t base = blockIdx.x * (ROW_THREADS / 8) + (threadIdx.x >> 5) * 4;
+  const uint32_t mine = (threadIdx.x >> 3) & 3;
+  if (base < units) fetch(base + mine);
+  for (; base < units; base += step) {
     float f[16];
-    load16<T, V>(x + row * ldx + col, live ? C - col : 0, f);
+    widen16(next, f);
+    if (base + step < units) fetch(base + step + mine);
     uint32_t m = abs_bits16(f);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t e = fp8_block_exponent(m);
-    if (live) {
-      if (col < ldv) *reinterpret_cast<uint4*>(values + (long long)row * ldv + col) = quantise16(f, e);
+    const uint32_t u = base + mine, e = fp8_block_exponent(m);
+    if (u < units) {
+      const uint32_t row = u / blocks, kb = u - row * blocks;
+      const int col = kb * FP8_BLOCK;
+      store_packed<V / sizeof(T)>(values + (long long)row * ldv + col, part, ldv - col, quantise16(f, e));
       if (part == 0) exps[(long long)kb * lde + row] = (uint8_t)e;
     }
   }
@@ -111,107 +187,153 @@ fp8_pack_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict
 
 constexpr int TILE_THREADS = 512;
 
+// A CTA walks over tiles and has the next one in flight while it works on the present one.
 template <typename T, int V>
-__global__ void __launch_bounds__(TILE_THREADS)
+__global__ void __launch_bounds__(TILE_THREADS, 2)
 fp8_pack_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
-                      int R, int C, int ldv, int blocks) {
-  __shared__ uint32_t warp_max[TILE_THREADS / 32];
-  const int rb = (int)(blockIdx.x / blocks), kb = (int)(blockIdx.x % blocks);
-  const int col = kb * FP8_BLOCK + (threadIdx.x & 7) * 16;
-  const int row0 = rb * FP8_BLOCK + (threadIdx.x >> 3);
-  float f[2][16];
+                      int R, int C, int ldv, uint32_t tiles, uint32_t blocks) {
+  rwkv_chain_trigger();
+  __shared__ uint32_t warp_max[2][TILE_THREADS / 32];
+  Raw16<T> next[2];
+  auto fetch = [&](uint32_t tile) {
+    const int row0 = (int)(tile / blocks) * FP8_BLOCK + (threadIdx.x >> 3), col = (int)(tile % blocks) * FP8_BLOCK;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = row0 + i * (TILE_THREADS / 8);
-    load16<T, V>(x + (long long)min(row, R - 1) * ldx + col, row < R ? C - col : 0, f[i]);
+    for (int i = 0; i < 2; ++i) {
+      const int row = row0 + i * (TILE_THREADS / 8);
+      load16<T, V>(x + (long long)min(row, R - 1) * ldx + col, threadIdx.x & 7, row < R ? C - col : 0, next[i]);
+    }
+  };
+  uint32_t tile = blockIdx.x;
+  if (tile < tiles) fetch(tile);
+  for (int turn = 0; tile < tiles; turn ^= 1) {
+    float f[2][16];
+    widen16(next[0], f[0]);
+    widen16(next[1], f[1]);
+    const uint32_t now = tile;
+    tile += gridDim.x;
+    if (tile < tiles) fetch(tile);
+    uint32_t m = max(abs_bits16(f[0]), abs_bits16(f[1]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) warp_max[turn][threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = warp_max[turn][threadIdx.x & (TILE_THREADS / 32 - 1)];
+#pragma unroll
+    for (int o = TILE_THREADS / 64; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t e = fp8_block_exponent(m);
+    const int row0 = (int)(now / blocks) * FP8_BLOCK + (threadIdx.x >> 3), col = (int)(now % blocks) * FP8_BLOCK;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = row0 + i * (TILE_THREADS / 8);
+      if (row < R)
+        store_packed<V / sizeof(T)>(values + (long long)row * ldv + col, threadIdx.x & 7, ldv - col, quantise16(f[i], e));
+    }
+    if (threadIdx.x == 0) exps[now] = (uint8_t)e;
   }
-  uint32_t m = max(abs_bits16(f[0]), abs_bits16(f[1]));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
-  __syncthreads();
-  m = warp_max[threadIdx.x & (TILE_THREADS / 32 - 1)];
-#pragma unroll
-  for (int o = TILE_THREADS / 64; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const uint32_t e = fp8_block_exponent(m);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = row0 + i * (TILE_THREADS / 8);
-    if (row < R && col < ldv) *reinterpret_cast<uint4*>(values + (long long)row * ldv + col) = quantise16(f[i], e);
-  }
-  if (threadIdx.x == 0) exps[blockIdx.x] = (uint8_t)e;
 }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(ROW_THREADS)
 fp8_unpack_kernel(const uint8_t* __restrict__ values, const uint8_t* __restrict__ exps, T* __restrict__ y, long long ldy,
-                  int R, int C, int ldv, int lde, int rows, int chunks) {
-  const long long units = (long long)R * chunks, stride = (long long)gridDim.x * ROW_THREADS;
-  for (long long u = (long long)blockIdx.x * ROW_THREADS + threadIdx.x; u < units; u += stride) {
-    const int row = (int)(u / chunks), col = (int)(u % chunks) * 16, kb = col / FP8_BLOCK;
-    const uint4 q = __ldcs(reinterpret_cast<const uint4*>(values + (long long)row * ldv + col));
+                  uint32_t units, int C, int ldv, int lde, int rows, uint32_t blocks) {
+  const int part = threadIdx.x & 7;
+  for (uint32_t u = blockIdx.x * (ROW_THREADS / 8) + (threadIdx.x >> 3); u < units; u += gridDim.x * (ROW_THREADS / 8)) {
+    const uint32_t row = u / blocks, kb = u - row * blocks;
+    const int col = kb * FP8_BLOCK;
     const uint32_t e = rows == 1 ? exps[(long long)kb * lde + row] : exps[(long long)(row / FP8_BLOCK) * lde + kb];
+    Packed16 q;
+    load_packed<V / sizeof(T)>(values + (long long)row * ldv + col, part, ldv - col, q);
     float f[16];
-    fp8_unpack4(q.x, f); fp8_unpack4(q.y, f + 4); fp8_unpack4(q.z, f + 8); fp8_unpack4(q.w, f + 12);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      f[i] = fp8_scaled(f[i], e);
-      if (e < 255u) f[i] = fminf(fmaxf(f[i], -largest<T>()), largest<T>());
+    for (int i = 0; i < 4; ++i) fp8_unpack4(q.w[i], f + 4 * i);
+    // one multiplication, but for blocks whose scale is no normal number and for those that may end above the largest one
+    if (e != 0u && e < first_overflow<T>()) {
+      const float s = __uint_as_float(e << 23);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] *= s;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        f[i] = fp8_scaled(f[i], e);
+        if (e < 255u) f[i] = fminf(fmaxf(f[i], -largest<T>()), largest<T>());
+      }
     }
-    store16<T, V>(y + row * ldy + col, C - col, f);
+    store16<T, V>(y + row * ldy + col, part, C - col, f);
   }
 }
 
 // widest access that every row start allows
-int access_bytes(const void* p, long long pitch_bytes, int elem) {
-  for (int v = 16; v > elem; v /= 2)
+int access_bytes(const void* p, long long pitch_bytes) {
+  for (int v = 32; v > 2; v /= 2)
     if ((uintptr_t)p % v == 0 && pitch_bytes % v == 0) return v;
-  return elem;
+  return 2;
 }
-unsigned grid_for(long long ctas) { return (unsigned)(ctas < 148 * 8 * 4 ? ctas : 148 * 8 * 4); }
+inline int up(int n, int m) { return (n + m - 1) / m * m; }
+int grid_for(long long ctas, int per_sm) { return (int)(ctas < 148 * per_sm ? ctas : 148 * per_sm); }
+// Rows of one launch: the kernels count in 32 bits.
+int rows_at_once(int R, int per_row) {
+  const long long most = 0x40000000ll / per_row / FP8_BLOCK * FP8_BLOCK;
+  return R < most ? R : (int)most;
+}
 
 template <typename T, int V>
-int pack_v(const void* x, long long ld, uint8_t* values, uint8_t* exps, int R, int C, int rows, cudaStream_t st) {
-  const int blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK, ldv = (C + 15) / 16 * 16;
-  if (rows == 1) {
-    const int lde = (R + 15) / 16 * 16;
-    const long long ctas = ((long long)R * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
-    fp8_pack_rows_kernel<T, V><<<grid_for(ctas), ROW_THREADS, 0, st>>>((const T*)x, ld, values, exps, R, C, ldv, lde, blocks);
-  } else {
-    const long long tiles = (long long)((R + FP8_BLOCK - 1) / FP8_BLOCK) * blocks;
-    if (tiles > 0x7fffffffll) return RWKV_ERR_TOO_LARGE;
-    fp8_pack_tiles_kernel<T, V><<<(unsigned)tiles, TILE_THREADS, 0, st>>>((const T*)x, ld, values, exps, R, C, ldv, blocks);
+int pack_v(const T* x, long long ld, uint8_t* values, uint8_t* exps, int R, int C, int rows, cudaStream_t st) {
+  const int blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK, ldv = up(C, 16);
+  const int most = rows_at_once(R, blocks);
+  for (int r0 = 0; r0 < R; r0 += most) {
+    const int n = R - r0 < most ? R - r0 : most;
+    const T* src = x + r0 * ld;
+    uint8_t* dst = values + (long long)r0 * ldv;
+    if (rows == 1) {
+      const long long ctas = ((long long)n * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
+      fp8_pack_rows_kernel<T, V><<<grid_for(ctas, 16), ROW_THREADS, 0, st>>>(src, ld, dst, exps + r0, (uint32_t)n * blocks, C, ldv,
+                                                                            up(R, 16), blocks);
+    } else {
+      const uint32_t tiles = (uint32_t)((n + FP8_BLOCK - 1) / FP8_BLOCK) * blocks;
+      fp8_pack_tiles_kernel<T, V><<<grid_for(tiles, 2), TILE_THREADS, 0, st>>>(
+          src, ld, dst, exps + (long long)(r0 / FP8_BLOCK) * blocks, n, C, ldv, tiles, blocks);
+    }
   }
   return rwkv_launch_status();
 }
 template <typename T>
 int pack_t(const void* x, long long ld, uint8_t* values, uint8_t* exps, int R, int C, int rows, cudaStream_t st) {
-  switch (access_bytes(x, ld * (long long)sizeof(T), sizeof(T))) {
-    case 16: return pack_v<T, 16>(x, ld, values, exps, R, C, rows, st);
-    case 8: return pack_v<T, 8>(x, ld, values, exps, R, C, rows, st);
-    case 4: return pack_v<T, 4>(x, ld, values, exps, R, C, rows, st);
-    default: return pack_v<T, sizeof(T)>(x, ld, values, exps, R, C, rows, st);
+  const T* p = (const T*)x;
+  switch (access_bytes(x, ld * (long long)sizeof(T))) {
+    case 32: return pack_v<T, 32>(p, ld, values, exps, R, C, rows, st);
+    case 16: return pack_v<T, 16>(p, ld, values, exps, R, C, rows, st);
+    case 8: return pack_v<T, 8>(p, ld, values, exps, R, C, rows, st);
+    case 4: return pack_v<T, 4>(p, ld, values, exps, R, C, rows, st);
+    default: return pack_v<T, sizeof(T)>(p, ld, values, exps, R, C, rows, st);
   }
 }
 template <typename T, int V>
-int unpack_v(const uint8_t* values, const uint8_t* exps, void* y, long long ldy, int R, int C, int rows, cudaStream_t st) {
-  const int ldv = (C + 15) / 16 * 16, chunks = ldv / 16;
-  const int lde = rows == 1 ? (R + 15) / 16 * 16 : (C + FP8_BLOCK - 1) / FP8_BLOCK;
-  const long long ctas = ((long long)R * chunks + ROW_THREADS - 1) / ROW_THREADS;
-  fp8_unpack_kernel<T, V><<<grid_for(ctas), ROW_THREADS, 0, st>>>(values, exps, (T*)y, ldy, R, C, ldv, lde, rows, chunks);
+int unpack_v(const uint8_t* values, const uint8_t* exps, T* y, long long ldy, int R, int C, int rows, cudaStream_t st) {
+  const int ldv = up(C, 16), blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK;
+  const int lde = rows == 1 ? up(R, 16) : blocks;
+  const int most = rows_at_once(R, blocks);
+  for (int r0 = 0; r0 < R; r0 += most) {
+    const int n = R - r0 < most ? R - r0 : most;
+    const long long ctas = ((long long)n * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
+    fp8_unpack_kernel<T, V><<<grid_for(ctas, 32), ROW_THREADS, 0, st>>>(
+        values + (long long)r0 * ldv, exps + (rows == 1 ? r0 : (long long)(r0 / FP8_BLOCK) * blocks), y + r0 * ldy, ldy,
+        (uint32_t)n * blocks, C, ldv, lde, rows, blocks);
+  }
   return rwkv_launch_status();
 }
 template <typename T>
 int unpack_t(const uint8_t* values, const uint8_t* exps, void* y, long long ldy, int R, int C, int rows, cudaStream_t st) {
-  switch (access_bytes(y, ldy * (long long)sizeof(T), sizeof(T))) {
-    case 16: return unpack_v<T, 16>(values, exps, y, ldy, R, C, rows, st);
-    case 8: return unpack_v<T, 8>(values, exps, y, ldy, R, C, rows, st);
-    case 4: return unpack_v<T, 4>(values, exps, y, ldy, R, C, rows, st);
-    default: return unpack_v<T, sizeof(T)>(values, exps, y, ldy, R, C, rows, st);
+  T* p = (T*)y;
+  switch (access_bytes(y, ldy * (long long)sizeof(T))) {
+    case 32: return unpack_v<T, 32>(values, exps, p, ldy, R, C, rows, st);
+    case 16: return unpack_v<T, 16>(values, exps, p, ldy, R, C, rows, st);
+    case 8: return unpack_v<T, 8>(values, exps, p, ldy, R, C, rows, st);
+    case 4: return unpack_v<T, 4>(values, exps, p, ldy, R, C, rows, st);
+    default: return unpack_v<T, sizeof(T)>(values, exps, p, ldy, R, C, rows, st);
   }
 }
 bool args_ok(const void* values, long long ld, int dtype, int R, int C, int rows) {
-  return R > 0 && C > 0 && C <= 0x7fffff00 && ld >= C && (rows == 1 || rows == FP8_BLOCK) && dtype >= 0 && dtype <= 2 &&
+  return R > 0 && C > 0 && C <= 0x3fffff00 && ld >= C && (rows == 1 || rows == FP8_BLOCK) && dtype >= 0 && dtype <= 2 &&
          (uintptr_t)values % 16 == 0;
 }
 
