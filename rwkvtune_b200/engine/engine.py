@@ -31,6 +31,13 @@ def resolve_stage(strategy: str) -> int:
     return STRATEGY_STAGE[strategy]
 
 
+def check_8bit_options(ffn_precision: str, grad_cp_bits: int) -> None:
+    if ffn_precision not in ("bf16", "fp8"):
+        raise ValueError(f"ffn_precision must be 'bf16' or 'fp8', got {ffn_precision!r}")
+    if grad_cp_bits not in (8, 16):
+        raise ValueError(f"grad_cp_bits must be 8 or 16, got {grad_cp_bits!r}")
+
+
 @dataclass
 class EngineConfig:
     lr_init: float = 3e-4
@@ -50,6 +57,8 @@ class EngineConfig:
     transport: str = "auto"   # "p2p": fused kernels over symmetric memory; "nccl": library collectives; "auto": p2p on multi-GPU CUDA when symmetric memory can be set up
     l2wrap: bool = True
     grad_cp_layers: Optional[object] = None   # None = all layers when grad_cp=1; int k = first k layers; "auto"
+    ffn_precision: str = "bf16"   # "fp8": the feed-forward products of training in 8 bits, its activations kept in 8 bits
+    grad_cp_bits: int = 16        # 8: inputs of recomputed blocks kept in 8 bits
     cuda_graph: bool = False   # replay forward+backward of a micro-batch (or of one infctx chunk) from a CUDA graph
 
 
@@ -61,12 +70,22 @@ class TrainEngine:
             dtype = torch.float32
         self.model = model.to(device=ctx.device, dtype=dtype)
         self.model.config.grad_cp = cfg.grad_cp
+        check_8bit_options(cfg.ffn_precision, cfg.grad_cp_bits)
+        self.model.config.ffn_precision, self.model.config.grad_cp_bits = cfg.ffn_precision, cfg.grad_cp_bits
+        if cfg.ffn_precision == "fp8":
+            if ctx.device.type == "cuda" and dtype != torch.bfloat16:
+                raise ValueError("ffn_precision='fp8' trains bf16 parameters on a GPU (precision='bf16')")
+            if not all(b.ffn._plain() for b in self.model.blocks):
+                raise ValueError("ffn_precision='fp8' needs plain feed-forward projections: leave ffn.key and ffn.value out "
+                                 "of the adapter's targets")
         if isinstance(cfg.grad_cp_layers, int):
             self.model.config.grad_cp_layers = cfg.grad_cp_layers
         if cfg.train_type == "infctx":
             as_infctx(self.model)
         self.model.train()
         stage = resolve_stage(cfg.strategy)
+        if stage == 3 and cfg.ffn_precision == "fp8":
+            raise ValueError("ffn_precision='fp8' does not run on ZeRO-3 weight panels: use stage 2 or below")
         self.zero3 = None
         if stage == 3 and ctx.world_size > 1 and ctx.device.type == "cuda" and dtype == torch.bfloat16:
             from ..parallel.zero3 import Zero3ShardedLinears

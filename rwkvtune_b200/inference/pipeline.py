@@ -16,7 +16,9 @@ from .batch_generator import BatchGenerator, GenerationConfig
 class InferencePipeline:
     def __init__(self, model_path: Optional[str] = None, model_config: Optional[str] = None, device: str = "cuda",
                  precision: str = "bf16", vocab_path: Optional[str] = None, debug_output: bool = False,
-                 model=None, tokenizer=None):
+                 model=None, tokenizer=None, ffn_8bit: bool = False):
+        """``ffn_8bit``: hold the feed-forward weights in 8 bits as well and decode with those
+        (:meth:`RWKV7Model.pack_ffn`)."""
         self.device = torch.device(device)
         self.precision = precision
         self.debug_output = debug_output
@@ -44,6 +46,8 @@ class InferencePipeline:
             self.model.load_state_dict(sd)
             self.model = self.model.to(device=self.device, dtype=dtype)
         self.model.eval()
+        if ffn_8bit:
+            self.model.pack_ffn()
         if tokenizer is not None:
             self.tokenizer = tokenizer
         elif model_path and os.path.isdir(model_path) and os.path.exists(os.path.join(model_path, "vocab.txt")):

@@ -293,8 +293,34 @@ class RWKV7ChannelMix(nn.Module):
             self.key.weight.uniform_(-0.5 * s, 0.5 * s)
             self.value.weight.zero_()
 
+    def _plain(self) -> bool:
+        """True when key and value are unwrapped, unsharded ``Linear`` layers (no adapter, no ZeRO-3 panels)."""
+        return all(type(m) is Linear and getattr(m, "_sharded", None) is None for m in (self.key, self.value))
+
+    def _weights_stamp(self):
+        return self.key.weight._version, self.value.weight._version, ops.param_epoch()
+
+    def pack(self) -> None:
+        """Hold key and value in 8 bits beside the weights; forward passes without autograd use those from now on."""
+        if not self._plain():
+            raise ValueError("8-bit feed-forward weights need plain projections (merge the adapter; no ZeRO-3 panels)")
+        packed = ops.pack_fp8(self.key.weight), ops.pack_fp8(self.value.weight)
+        object.__setattr__(self, "_packed", (self._weights_stamp(), packed))
+
+    def unpack(self) -> None:
+        object.__setattr__(self, "_packed", None)
+
     def forward(self, x, ln_w, ln_b, x_prev=None, want_state: bool = False):
         (xk,), last, x = ops.ln_shift_mix_unbound(x, ln_w, ln_b, self.x_k, x_prev)
+        held = getattr(self, "_packed", None)
+        if held is not None and not torch.is_grad_enabled():
+            if held[0] != self._weights_stamp():
+                raise RuntimeError("the feed-forward weights have changed since pack_ffn(): call it again, or unpack_ffn()")
+            return ops.fp8_channel_mix_ffn(xk, *held[1], x), (last if want_state else None)
+        if getattr(self.config, "ffn_precision", "bf16") == "fp8" and not _decoding(xk):
+            if not self._plain():
+                raise RuntimeError("ffn_precision='fp8' needs plain feed-forward projections (no adapter, no ZeRO-3 panels)")
+            return ops.fp8_channel_mix_ffn(xk, self.key.weight, self.value.weight, x), (last if want_state else None)
         if _decoding(xk):
             spec = _decode_spec(self.key, xk, "relu_sq")
             out = ops.decode_projection_set([spec], (), _weights_of(self.value)) if spec is not None else None
@@ -302,8 +328,7 @@ class RWKV7ChannelMix(nn.Module):
                 nxt = getattr(self, "_decode_next", None)      # the time-mix half of the next block
                 hint = _weights_of(*(getattr(nxt, n, None) for n in ("receptance", "key", "value"))) if nxt is not None else None
                 return _project_add(self.value, out[0][0], x, hint), (last if want_state else None)
-        plain = all(type(m) is Linear and getattr(m, "_sharded", None) is None for m in (self.key, self.value))
-        if plain:
+        if self._plain():
             return ops.channel_mix_ffn(xk, self.key.weight, self.value.weight, x), (last if want_state else None)
         if type(self.key) is Linear and getattr(self.key, "_sharded", None) is None:
             hidden = ops.linear_relu_sq(xk, self.key.weight)
@@ -370,21 +395,34 @@ class _Recompute(torch.autograd.Function):
     (``rwkvtune/models/rwkv7/model.py:454-455`` wraps every block) without the per-saved-tensor pack/unpack hooks of
     the non-reentrant implementation, which cost more host time than the kernels of a small block.  ``anchor`` is an
     empty tensor that requires grad, so the node is part of the graph even when no real input requires grad (frozen
-    embedding under LoRA); parameter gradients accumulate into ``.grad`` during the inner backward."""
+    embedding under LoRA); parameter gradients accumulate into ``.grad`` during the inner backward.
+
+    ``bits=8`` keeps the residual stream (the first input, different for every block) in 8 bits with one scale per token
+    and 128 channels; the second run then starts from the rounded values.  The other inputs are shared by all blocks
+    (``v_first``) or small (carried states) and kept as they are."""
 
     @staticmethod
-    def forward(ctx, fn, block, anchor, *tensors):
+    def forward(ctx, fn, block, anchor, bits, *tensors):
         ctx.fn, ctx.block = fn, block
         ctx.req = [t is not None and t.requires_grad for t in tensors]
         ctx.none = [t is None for t in tensors]
-        ctx.save_for_backward(*[t for t in tensors if t is not None])
+        ctx.packed = None
+        keep = [t for t in tensors if t is not None]
+        if bits == 8:
+            p = ops.pack_fp8(keep[0], rows=1)
+            ctx.packed = p.offset, p.R, p.C, p.rows, p.shape, p.dtype
+            keep[0] = p.data
+        ctx.save_for_backward(*keep)
         with torch.no_grad():
             outs = fn(block, *tensors)
         return tuple(outs)
 
     @staticmethod
     def backward(ctx, *grads):
-        saved = iter(ctx.saved_tensors)
+        saved = list(ctx.saved_tensors)
+        if ctx.packed is not None:
+            saved[0] = ops.unpack_fp8(ops.Fp8Blocks(saved[0], *ctx.packed))
+        saved = iter(saved)
         inputs = [None if is_none else next(saved).detach().requires_grad_(req)
                   for is_none, req in zip(ctx.none, ctx.req)]
         with torch.enable_grad():
@@ -392,7 +430,7 @@ class _Recompute(torch.autograd.Function):
         pairs = [(o, g) for o, g in zip(outs, grads) if isinstance(o, torch.Tensor) and o.requires_grad and g is not None]
         if pairs:
             torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
-        return (None, None, None) + tuple(t.grad if t is not None and t.requires_grad else None for t in inputs)
+        return (None, None, None, None) + tuple(t.grad if t is not None and t.requires_grad else None for t in inputs)
 
 
 def _has_active_dropout(block: nn.Module) -> bool:
@@ -401,10 +439,13 @@ def _has_active_dropout(block: nn.Module) -> bool:
 
 def _checkpoint_block(fn, block, *tensors):
     """Recompute-in-backward wrapper for one block (random-number state is only preserved by the library path)."""
+    bits = getattr(block.config, "grad_cp_bits", 16)
     if _has_active_dropout(block):
+        if bits == 8:
+            raise RuntimeError("grad_cp_bits=8 does not keep the random-number state that active dropout needs")
         return _checkpoint(fn, block, *tensors, use_reentrant=False)
     anchor = torch.empty(0, device=tensors[0].device, requires_grad=True)
-    return _Recompute.apply(fn, block, anchor, *tensors)
+    return _Recompute.apply(fn, block, anchor, bits, *tensors)
 
 
 class RWKV7Model(GenerationMixin, nn.Module):
@@ -476,6 +517,21 @@ class RWKV7Model(GenerationMixin, nn.Module):
         if hasattr(head, "base_layer"):  # LoRA-wrapped heads are merged on the fly
             return head.effective_weight()
         return head.weight
+
+    # ------------------------------------------------------------------ 8-bit feed-forward weights for inference
+    def pack_ffn(self) -> "RWKV7Model":
+        """Hold every block's feed-forward weights in 8 bits as well (half their bf16 size again): passes without autograd -
+        decoding, prefill, evaluation - then run those products in 8 bits.  A token's result does not depend on the batch
+        it is in.  Call it again after changing the weights; a stale copy is refused.  A captured decode graph keeps the
+        form that the weights had when it was captured."""
+        for block in self.blocks:
+            block.ffn.pack()
+        return self
+
+    def unpack_ffn(self) -> "RWKV7Model":
+        for block in self.blocks:
+            block.ffn.unpack()
+        return self
 
     # ------------------------------------------------------------------ stateful paths
     def init_state(self, batch_size: int) -> List[Dict[str, torch.Tensor]]:

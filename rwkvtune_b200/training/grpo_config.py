@@ -98,8 +98,13 @@ class GRPOConfig:
     gradient_checkpointing: bool = False
     log_entropy: bool = True
     ctx_len: int = 0
+    ffn_precision: str = "bf16"   # "fp8": feed-forward products and activations of training in 8 bits
+    grad_cp_bits: int = 16        # 8: inputs of recomputed blocks kept in 8 bits
 
     def __post_init__(self) -> None:
+        from ..engine.engine import check_8bit_options
+
+        check_8bit_options(self.ffn_precision, self.grad_cp_bits)
         if self.epsilon_high is None:
             self.epsilon_high = self.epsilon
         if self.num_generations <= 0:

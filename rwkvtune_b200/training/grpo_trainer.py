@@ -339,11 +339,13 @@ class GRPOTrainer:
                            grad_clip=a.grad_clip, accumulate_grad_batches=a.accumulate_grad_batches, strategy=a.strategy,
                            precision=a.precision if a.accelerator != "cpu" else "fp32", grad_cp=a.grad_cp,
                            lr_2x_patterns=("att.w0",), transport=os.environ.get("RWKVTUNE_TRANSPORT", "auto"),
+                           ffn_precision=a.ffn_precision, grad_cp_bits=a.grad_cp_bits,
                            cuda_graph=os.environ.get("RWKVTUNE_CUDA_GRAPH", "0") == "1")
         self.engine = eng = TrainEngine(self.model, cfg, ctx)
         self.model = eng.model
         if self.ref_model is not None:
             self.ref_model = self.ref_model.to(device=ctx.device, dtype=eng.model.dtype).eval()
+            self.ref_model.config.ffn_precision = a.ffn_precision      # the KL term compares like with like
             for p in self.ref_model.parameters():
                 p.requires_grad_(False)
         self.generator = GRPOBatchGenerator(eng.model, self.processing_class, ctx.device,

@@ -66,8 +66,13 @@ class SFTConfig:
     run_name: str = ""
     profile_steps: int = 0   # > 0: record that many steps (after 3 warm-up steps) with torch.profiler and write <proj_dir>/profile_kernels.txt
     log_every_n_steps: int = 1
+    ffn_precision: str = "bf16"   # "fp8": feed-forward products and activations of training in 8 bits
+    grad_cp_bits: int = 16        # 8: inputs of recomputed blocks kept in 8 bits
 
     def __post_init__(self) -> None:
+        from ..engine.engine import check_8bit_options
+
+        check_8bit_options(self.ffn_precision, self.grad_cp_bits)
         if self.train_type not in ("normal", "infctx"):
             raise ValueError(f"train_type must be 'normal' or 'infctx', got {self.train_type!r}")
         if self.train_type == "infctx":

@@ -100,6 +100,7 @@ class SupervisedTrainer:
                             lr_2x_patterns=("att.w0",) if a.train_type == "infctx" else (),
                             train_type=a.train_type, chunk_ctx=a.chunk_ctx, truncated_bptt=a.truncated_bptt,
                             transport=os.environ.get("RWKVTUNE_TRANSPORT", "auto"),
+                            ffn_precision=a.ffn_precision, grad_cp_bits=a.grad_cp_bits,
                            cuda_graph=os.environ.get("RWKVTUNE_CUDA_GRAPH", "0") == "1")
 
     # ------------------------------------------------------------------ public

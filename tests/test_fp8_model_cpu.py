@@ -1,0 +1,192 @@
+"""The 8-bit operators inside the model, the engine and the trainers' settings, on the CPU."""
+import copy
+
+import pytest
+import torch
+
+from rwkvtune_b200 import ops
+from rwkvtune_b200.engine.engine import EngineConfig, TrainEngine
+from rwkvtune_b200.models import RWKV7Model, RWKVConfig
+from rwkvtune_b200.parallel.bootstrap import DistContext
+from rwkvtune_b200.peft import LoraConfig, get_peft_model
+from rwkvtune_b200.training.grpo_config import GRPOConfig
+from rwkvtune_b200.training.sft_config import SFTConfig
+
+
+def make(**kw):
+    torch.manual_seed(0)
+    m = RWKV7Model(RWKVConfig(n_layer=2, n_embd=64, vocab_size=128, dim_att_lora=16, dim_gate_lora=16, dim_mv_lora=16))
+    with torch.no_grad():
+        for b in m.blocks:      # the value projection starts at zero, which would hide it
+            b.ffn.value.weight.normal_(0, 0.05)
+            b.att.output.weight.normal_(0, 0.05)
+    for k, v in kw.items():
+        setattr(m.config, k, v)
+    return m
+
+
+def batch(B=3, T=40):
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, 128, (B, T), generator=g)
+    return ids, torch.randint(0, 128, (B, T), generator=g)
+
+
+def grads(m, ids, labels):
+    m.train()
+    loss = m.loss(ids, labels)
+    loss.backward()
+    return loss.item(), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}
+
+
+def test_the_ffn_of_a_model_in_8_bits_is_the_operator():
+    m, ids = make(ffn_precision="fp8"), batch()[0]
+    calls = []
+    real = ops.fp8_channel_mix_ffn
+    try:
+        ops.fp8_channel_mix_ffn = lambda *a: calls.append(a) or real(*a)
+        m(ids)
+    finally:
+        ops.fp8_channel_mix_ffn = real
+    assert len(calls) == 2 and calls[0][1] is m.blocks[0].ffn.key.weight
+    # the packed operands move every product's terms by at most (1 + 2^-4)^2 - 1: the result is another one, but near
+    a, b = make()(ids), m(ids)
+    assert not torch.equal(a, b) and (a - b).norm() < ((1 + 2 ** -4) ** 2 - 1) * 2 * a.norm()
+
+
+def test_a_recomputed_block_sees_the_packed_input():
+    """With inputs that packing leaves as they are, 8-bit checkpoints change nothing; with others the gradients are those of
+    the block at the packed input."""
+    m = make(grad_cp=1, grad_cp_bits=8)
+    block = m.blocks[0].train()
+    from rwkvtune_b200.models.rwkv7.model import _block_plain, _checkpoint_block
+
+    x = torch.randn(2, 16, 64)
+    v = torch.zeros_like(x)
+    exact = ops.unpack_fp8(ops.pack_fp8(x, rows=1))
+    out = {}
+    for name, inp in (("packed", exact), ("given", x)):
+        a = inp.clone().requires_grad_()
+        y, _ = _checkpoint_block(_block_plain, block, a, v)
+        dy = torch.ones_like(y)
+        (out[name],) = torch.autograd.grad(y, [a], dy)
+    a = exact.clone().requires_grad_()
+    y, _ = _block_plain(block, a, v)
+    (want,) = torch.autograd.grad(y, [a], torch.ones_like(y))
+    assert torch.equal(out["packed"], want) and torch.equal(out["given"], want)
+
+
+def test_checkpoints_in_8_bits_keep_the_loss_and_the_last_block():
+    ids, labels = batch()
+    l16, g16 = grads(make(grad_cp=1), ids, labels)
+    l8, g8 = grads(make(grad_cp=1, grad_cp_bits=8), ids, labels)
+    assert l8 == l16 and set(g8) == set(g16)                  # the forward pass is not rounded
+    assert torch.equal(g8["head.weight"], g16["head.weight"]) and torch.equal(g8["ln_out.weight"], g16["ln_out.weight"])
+    k = "blocks.0.ffn.key.weight"
+    assert not torch.equal(g8[k], g16[k]) and torch.isfinite(g8[k]).all()
+
+
+def test_infinite_context_chunks_with_8_bit_checkpoints():
+    from rwkvtune_b200.models.rwkv7.model_infctx import as_infctx
+
+    ids, labels = batch(2, 32)
+    got = {}
+    for bits in (16, 8):
+        m = as_infctx(make(grad_cp=1, grad_cp_bits=bits, ffn_precision="fp8")).train()
+        L, H = 2, 1
+        shift, wkv = torch.zeros(L, 2, 2, 64), torch.zeros(L, 2, H, 64, 64)
+        x, shift, wkv = m.forward_hidden_infctx(ids, shift, wkv, checkpoint=True)
+        (x.square().mean() + wkv.square().mean()).backward()
+        got[bits] = m.blocks[0].ffn.value.weight.grad
+    assert got[8].abs().sum() > 0 and torch.isfinite(got[8]).all()
+
+
+def test_dropout_and_8_bit_checkpoints_are_refused():
+    m = get_peft_model(make(), LoraConfig(r=4, lora_alpha=8, lora_dropout=0.5))
+    m.config.grad_cp, m.config.grad_cp_bits = 1, 8
+    m.train()
+    with pytest.raises(RuntimeError, match="dropout"):
+        m.loss(*batch())
+
+
+def test_packed_weights_serve_passes_without_autograd():
+    m, ids = make().eval(), batch()[0]
+    with torch.no_grad():
+        plain = m(ids)
+        m.pack_ffn()
+        y = m(ids)
+        state_y, st = m.forward_with_state(ids[:, :30])
+        more, _ = m.forward_with_state(ids[:, 30:], st)
+    ffn = m.blocks[0].ffn
+    x = torch.randn(1, 5, 64)
+    with torch.no_grad():
+        got, _ = ffn(x, torch.ones(64), torch.zeros(64))
+        (xk,), _, _ = ops.ln_shift_mix_unbound(x, torch.ones(64), torch.zeros(64), ffn.x_k, None)
+        assert torch.equal(got, ops.fp8_channel_mix_ffn(xk, ops.pack_fp8(ffn.key.weight), ops.pack_fp8(ffn.value.weight), x))
+    assert not torch.equal(y, plain)
+    # blocks of one row: cutting the sequence in two leaves the packed operands as they are (the recurrence sums differently)
+    torch.testing.assert_close(torch.cat([state_y, more], 1), y, rtol=1e-3, atol=1e-3)
+    m.unpack_ffn()
+    with torch.no_grad():
+        assert torch.equal(m(ids), plain)
+
+
+def test_stale_packed_weights_are_refused():
+    m, ids = make().eval().pack_ffn(), batch()[0]
+    with torch.no_grad():
+        m.blocks[1].ffn.key.weight.add_(1.0)
+        with pytest.raises(RuntimeError, match="pack_ffn"):
+            m(ids)
+        m.pack_ffn()
+        m(ids)
+        ops.bump_param_epoch()                     # the optimiser kernels write without a version count
+        with pytest.raises(RuntimeError, match="pack_ffn"):
+            m(ids)
+    m.train().loss(*batch()).backward()            # training uses the weights themselves
+
+
+def test_packing_wrapped_projections_is_refused():
+    m = get_peft_model(make(), LoraConfig(r=4, lora_alpha=8))
+    if any(not b.ffn._plain() for b in m.blocks):
+        with pytest.raises(ValueError):
+            m.pack_ffn()
+
+
+def test_engine_trains_with_both():
+    ids, labels = batch()
+    eng = TrainEngine(make(), EngineConfig(lr_init=1e-3, precision="fp32", grad_cp=1, ffn_precision="fp8", grad_cp_bits=8),
+                      DistContext())
+    before = copy.deepcopy(eng.model.state_dict())
+    out = eng.train_step(ids, labels, 1e-3) if hasattr(eng, "train_step") else None
+    after = eng.model.state_dict()
+    assert eng.model.config.ffn_precision == "fp8" and eng.model.config.grad_cp_bits == 8
+    if out is not None:
+        assert any(not torch.equal(before[k], after[k]) for k in before)
+
+
+@pytest.mark.parametrize("config", [SFTConfig, GRPOConfig, EngineConfig])
+def test_settings(config):
+    c = config(ffn_precision="fp8", grad_cp_bits=8)
+    assert (c.ffn_precision, c.grad_cp_bits) == ("fp8", 8)
+    assert (config().ffn_precision, config().grad_cp_bits) == ("bf16", 16)
+
+
+def test_settings_refusals():
+    for kw in ({"ffn_precision": "int8"}, {"grad_cp_bits": 4}):
+        with pytest.raises(ValueError):
+            SFTConfig(**kw)
+        with pytest.raises(ValueError):
+            GRPOConfig(**kw)
+        with pytest.raises(ValueError):
+            TrainEngine(make(), EngineConfig(precision="fp32", **kw), DistContext())
+    m = get_peft_model(make(), LoraConfig(r=4, lora_alpha=8, target_modules=["key", "value"]))
+    with pytest.raises(ValueError):
+        TrainEngine(m, EngineConfig(precision="fp32", ffn_precision="fp8"), DistContext())
+    with pytest.raises(ValueError):
+        TrainEngine(make(), EngineConfig(precision="fp32", ffn_precision="fp8", strategy="deepspeed_stage_3"), DistContext())
+
+
+def test_pipeline_switch():
+    from rwkvtune_b200.inference.pipeline import InferencePipeline
+
+    pipe = InferencePipeline(model=make(), device="cpu", tokenizer=object(), ffn_8bit=True)
+    assert all(b.ffn._packed is not None for b in pipe.model.blocks)

@@ -1,0 +1,126 @@
+"""The 8-bit operators as the model, the engine and the rollout generator use them on a GPU."""
+import pytest
+import torch
+
+from rwkvtune_b200.engine.engine import EngineConfig, TrainEngine
+from rwkvtune_b200.models import RWKV7Model, RWKVConfig
+from rwkvtune_b200.ops import _ext, gemm_native
+from rwkvtune_b200.parallel.bootstrap import DistContext
+
+pytestmark = pytest.mark.gpu
+
+
+def make(**kw):
+    torch.manual_seed(0)
+    m = RWKV7Model(RWKVConfig(n_layer=2, n_embd=256, vocab_size=1024, dim_att_lora=32, dim_gate_lora=64, dim_mv_lora=32, ctx_len=512))
+    with torch.no_grad():
+        for b in m.blocks:
+            b.ffn.value.weight.normal_(0, 0.02)
+            b.att.output.weight.normal_(0, 0.02)
+    for k, v in kw.items():
+        setattr(m.config, k, v)
+    return m.cuda().to(torch.bfloat16)
+
+
+def batch(B=2, T=272):
+    g = torch.Generator().manual_seed(1)
+    return [torch.randint(0, 1024, (B, T), generator=g).cuda() for _ in range(2)]
+
+
+def run(m, **kw):
+    """Loss and gradients of one model under the given settings."""
+    for k, v in {"ffn_precision": "bf16", "grad_cp": 0, "grad_cp_bits": 16, **kw}.items():
+        setattr(m.config, k, v)
+    m.train().zero_grad(set_to_none=True)
+    loss = m.loss(*batch())
+    loss.backward()
+    return loss.item(), {n: p.grad.float() for n, p in m.named_parameters()}
+
+
+def test_training_pass_runs_the_8_bit_kernels_and_stays_near():
+    """The packed operands move each feed-forward product's terms by at most 2^-4 each; a gradient's direction stays."""
+    m = make()
+    l16, g16 = run(m)
+    before = _ext.launch_count()
+    l8, g8 = run(m, ffn_precision="fp8")
+    assert _ext.launch_count() > before and abs(l8 - l16) < 2 ** -4 * abs(l16)
+    for name in ("blocks.0.ffn.key.weight", "blocks.1.ffn.value.weight", "emb.weight", "blocks.0.att.key.weight"):
+        a, b = g8[name].flatten(), g16[name].flatten()
+        assert torch.isfinite(a).all() and torch.dot(a, b) > 0.9 * a.norm() * b.norm(), name
+    torch.cuda.synchronize()
+    assert gemm_native.check_status() == 0
+
+
+def test_checkpoints_in_8_bits():
+    m = make()
+    l16, g16 = run(m, grad_cp=1)
+    l8, g8 = run(m, grad_cp=1, grad_cp_bits=8)
+    assert l8 == l16 and torch.equal(g8["head.weight"], g16["head.weight"])
+    for name in g16:
+        a, b = g8[name].flatten(), g16[name].flatten()
+        if b.norm() > 0:
+            assert torch.isfinite(a).all() and torch.dot(a, b) > 0.9 * a.norm() * b.norm(), name
+
+
+def test_a_checkpoint_takes_half_the_memory():
+    from rwkvtune_b200.models.rwkv7.model import _checkpoint_block
+
+    class Id(torch.nn.Module):
+        def __init__(self, bits):
+            super().__init__()
+            self.config = type("C", (), {"grad_cp_bits": bits})()
+
+    kept = {}
+    for bits in (16, 8):
+        torch.cuda.synchronize()
+        start = torch.cuda.memory_allocated()
+        x = torch.randn(4096, 1024, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        (y,) = _checkpoint_block(lambda b, t: (t * 2,), Id(bits), x * 1.0)
+        kept[bits] = torch.cuda.memory_allocated() - start
+        del x, y
+    assert kept[16] - kept[8] > 0.45 * 4096 * 1024 * 2
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_engine_steps_with_both(graph):
+    eng = TrainEngine(make(), EngineConfig(lr_init=1e-3, precision="bf16", grad_cp=1, ffn_precision="fp8", grad_cp_bits=8,
+                                           cuda_graph=graph), DistContext(device=torch.device("cuda", 0)))
+    ids, labels = batch()
+    losses = [float(eng.train_step(ids, labels, 1e-3)) for _ in range(4)]
+    assert all(v == v for v in losses) and len(set(losses)) > 1
+    torch.cuda.synchronize()
+    assert gemm_native.check_status() == 0
+
+
+def test_captured_steps_repeat_the_eager_ones():
+    got = []
+    for graph in (False, True):
+        eng = TrainEngine(make(), EngineConfig(lr_init=1e-3, precision="bf16", ffn_precision="fp8", cuda_graph=graph),
+                          DistContext(device=torch.device("cuda", 0)))
+        ids, labels = batch()
+        got.append([float(eng.train_step(ids, labels, 1e-3)) for _ in range(3)])
+    assert got[0] == got[1]
+
+
+def test_packed_decode_steps():
+    """Prefill and decoding on packed weights, eager and from the rollout generator's captured step."""
+    from rwkvtune_b200.inference import GRPOBatchGenerator
+
+    m = make().eval().pack_ffn()
+    prompts = [[5, 6, 7, 8], [9, 10, 11], [12] * 6]
+    outs = []
+    for use_graph in (False, True):
+        gen = GRPOBatchGenerator(m, None, torch.device("cuda", 0), eos_token_id=0, use_cuda_graph=use_graph)
+        out = gen.generate(input_ids=prompts, max_new_tokens=12, num_generations=2, temperature=1.0, top_p=1.0, seed=3)
+        outs.append(out["completion_ids"].cpu())
+    assert torch.equal(outs[0], outs[1])
+    torch.cuda.synchronize()
+    assert gemm_native.check_status() == 0
+
+
+def test_packed_and_plain_logits_are_near():
+    m, (ids, _) = make().eval(), batch()
+    with torch.no_grad():
+        plain = m(ids).float()
+        packed = m.pack_ffn()(ids).float()
+    assert (packed - plain).norm() < ((1 + 2 ** -4) ** 2 - 1) * 2 * plain.norm() and not torch.equal(packed, plain)
