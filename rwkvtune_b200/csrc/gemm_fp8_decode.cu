@@ -2,9 +2,10 @@
 //
 // Bound by streaming W once, one byte a weight, and below a few megabytes by latency.  As in gemm_decode_tcgen05.cu the
 // weight tile is the 128-row operand A of the instruction and the tokens are its columns (M rounded up to 16), so the
-// accumulator's lanes are full whatever M is; a column block of 128 weights is one CTA's, its contraction is cut over a
-// cluster of S CTAs, and the partial tiles are summed through distributed shared memory in a fixed order.  S depends on N
-// and K alone, so a row's result does not depend on how many others there are.
+// accumulator's lanes are full whatever M is; a column block of 128 weights is one CTA's and its contraction is cut over a
+// cluster of S CTAs.  Token m of the sum belongs to CTA m % S: the others write their partial rows into its shared memory,
+// and after one cluster barrier it adds them in a fixed order.  S depends on N and K alone, so a row's result does not
+// depend on how many others there are.
 //
 // The tokens come either in bf16 - then each CTA packs its part of the contraction itself, row by row, into the
 // shared-memory tiles the tensor core reads, which saves a launch and a round trip - or already packed, fetched by TMA in
@@ -35,20 +36,24 @@ constexpr int THREADS = 32 * (WORKERS + 2);
 constexpr int W_BYTES = 128 * 128;
 constexpr int MAX_STAGES = 8;
 constexpr int MAX_GROUPS = 16;                   // sets of four scale blocks: 64 blocks of the contraction per CTA
-constexpr int TMEM_COLS = 256, SF_COL = 128;     // accumulator in columns 0..127, eight columns of scales per set behind it
+// Tensor memory: accumulator in columns 0..127 (two in turn if mpad <= 64), then the scales: four columns per set of tokens
+// and four per set and column block of weights, all of them resident.
+constexpr int TMEM_COLS = 256, SF_COL = 128, MAX_SETS = (TMEM_COLS - SF_COL) / 4;
 constexpr int SMEM_MIN = 112 * 1024, SMEM_MAX = 224 * 1024;
 constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 struct Barriers {
   uint64_t full[MAX_STAGES], empty[MAX_STAGES];
   uint64_t x_ready[MAX_GROUPS];                  // tokens (or their scales) of a set are in shared memory
-  uint64_t acc_full;
+  uint64_t acc_full[2], acc_free[2];
   uint32_t tmem_base;
   int abort_flag;
 };
 
 struct Args {
-  int M, N, K, mpad, stages, split;
+  int M, N, K, mpad, stages;
+  int tiles;                                     // column blocks of a CTA, one after another (S = 1)
+  int split_log, m_log;                          // log2 of S, and of M rounded up to a power of two
   const uint8_t* w_exp;
   const bf16* x;                                 // null: packed tokens
   long long ldx;
@@ -147,138 +152,238 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.b32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok));
+  return ok != 0;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 enum Epilogue { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_RELU_SQ = 2 };
 
-// grid: (column blocks of 128, S), clusters of (1, S, 1)
+// Tokens z, z + S, ... of a column block: sums the S partial rows, applies the epilogue and stores; one warp a token, four
+// columns a lane.
+template <int EPI>
+__device__ __forceinline__ void finish(const Args& g, uint32_t part, int slab, int warp, int lane, int z, int slog, int own_tokens) {
+  const int n = slab * 128 + lane * 4;
+  for (int m = z + (warp << slog); m < g.M; m += WORKERS << slog) {
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < 1 << slog; ++r) {
+      float4 p;
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
+                   : "r"(part + (r * own_tokens + (m >> slog)) * 512 + lane * 16) : "memory");
+      f[0] += p.x; f[1] += p.y; f[2] += p.z; f[3] += p.w;
+    }
+    if (EPI == EPI_RELU_SQ) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[e] = f[e] < 0.f || n + e >= g.N ? 0.f : f[e];
+        f[e] *= f[e];
+        top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const uint32_t e = fp8_block_exponent(top);
+      const float s = fp8_inverse_scale(e == 255u ? 127u : e);
+      if (n < g.q_ldv)
+        *reinterpret_cast<uint32_t*>(g.q_val + (long long)m * g.q_ldv + n) =
+            e == 255u ? 0x7f7f7f7fu : fp8_pack4(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
+      if (lane == 0) g.q_exp[(long long)slab * g.q_lde + m] = (uint8_t)e;
+    } else if (g.vec) {
+      if (n < g.N) {
+        if (EPI == EPI_RESIDUAL) {
+          const uint2 p = *reinterpret_cast<const uint2*>(g.residual + m * g.ldr + n);
+          f[0] += bf16_lo(p.x); f[1] += bf16_hi(p.x); f[2] += bf16_lo(p.y); f[3] += bf16_hi(p.y);
+        }
+        *reinterpret_cast<uint2*>(g.c + m * g.ldc + n) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < g.N)
+          g.c[m * g.ldc + n + e] =
+              __float2bfloat16_rn(f[e] + (EPI == EPI_RESIDUAL ? __bfloat162float(g.residual[m * g.ldr + n + e]) : 0.f));
+    }
+  }
+}
+
+// grid: (column blocks of 128 / tiles, S), clusters of (1, S, 1)
 template <bool PACKED, int EPI>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 fp8_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                   const __grid_constant__ Args g) {
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t raw = smem_u32(smem_dyn);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int S = g.split, z = (int)blockIdx.y, n0 = (int)blockIdx.x * 128;
-  const int all_kb = (g.K + 127) / 128, kb0 = (int)((long long)all_kb * z / S), nkb = (int)((long long)all_kb * (z + 1) / S) - kb0;
-  const int groups = (nkb + 3) / 4, x_bytes = g.mpad * 128;
+  const int slog = g.split_log, S = 1 << slog, z = (int)blockIdx.y;
+  // column blocks of this CTA: tiles of them, the last CTA's may be fewer
+  const int slab0 = (int)blockIdx.x * g.tiles, slabs = (g.N + 127) >> 7, tiles = min(g.tiles, slabs - slab0);
+  const int accs = g.mpad <= 64 ? 2 : 1;          // accumulators in turn, mpad <= 64 columns apart
+  // the first all_kb % S CTAs of a cluster take one block of the contraction more
+  const int all_kb = (g.K + 127) >> 7, more = all_kb & (S - 1), kb0 = z * (all_kb >> slog) + min(z, more);
+  const int nkb = (all_kb >> slog) + (z < more ? 1 : 0);
+  const int groups = (nkb + 3) >> 2, x_bytes = g.mpad * 128;
   const int stage_bytes = W_BYTES + (PACKED ? x_bytes : 0);
   const uint32_t xs = base + g.stages * stage_bytes;                       // tokens packed here (not PACKED)
-  const int max_kb = (all_kb + S - 1) / S;
-  const uint32_t sf = xs + (PACKED ? 0 : max_kb * x_bytes);                // 512 bytes of A, 512 of B per set
-  Barriers* bars = reinterpret_cast<Barriers*>(smem_dyn + (sf - raw) + (max_kb + 3) / 4 * 1024);
+  const int max_kb = (all_kb + S - 1) >> slog;
+  const int max_groups = (max_kb + 3) >> 2;
+  const uint32_t sf = xs + (PACKED ? 0 : max_kb * x_bytes);                // 512 bytes per set: tokens, then weights by block
+  const uint32_t part = sf + max_groups * (1 + g.tiles) * 512;             // [CTA][own token][128 columns] in fp32
+  const int own_tokens = (g.mpad + S - 1) >> slog;
+  Barriers* bars = reinterpret_cast<Barriers*>(smem_dyn + (part - raw) + own_tokens * S * 512);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < g.stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    for (int i = 0; i < groups; ++i) mbar_init(&bars->x_ready[i], WORKERS);
-    mbar_init(&bars->acc_full, 1);
-    bars->abort_flag = 0;
+  rwkv_chain_trigger();
+  if (warp == WARP_TMA) {                        // a lane a barrier
+    if (lane < MAX_STAGES) { mbar_init(&bars->full[lane], 1); mbar_init(&bars->empty[lane], 1); }
+    if (lane < MAX_GROUPS) mbar_init(&bars->x_ready[lane], WORKERS);
+    if (lane >= MAX_GROUPS && lane < MAX_GROUPS + 2) {
+      mbar_init(&bars->acc_full[lane - MAX_GROUPS], 1);
+      mbar_init(&bars->acc_free[lane - MAX_GROUPS], WORKERS);
+    }
+    if (lane == 31) bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == WARP_MMA) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)),
-                 "r"(TMEM_COLS));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  // scales of the weights, one byte per block: requested before anything is waited for
+  uint32_t w_scale = 0;
+  const int w_sets = groups * tiles;                            // set i: column block i / groups, blocks of the contraction i % groups
+  const auto weight_scale = [&](int i) {
+    const int t = i / groups, kb = kb0 + (i - t * groups) * 4 + (lane & 3);
+    return kb < all_kb ? (uint32_t)g.w_exp[(long long)(slab0 + t) * all_kb + kb] << (8 * (lane & 3)) : 0u;
+  };
+  if (warp < WORKERS && warp < w_sets) w_scale = weight_scale(warp);
+  // tokens: eight threads a block of 128, DEEP blocks a thread in flight; the first set's are requested before the barrier
+  constexpr int DEEP = 4;
+  const int sub = lane & 7;
+  uint4 v[DEEP][2];
+  const auto fetch = [&](int i, int u0) {
+    const int units = (nkb - i * 4 < 4 ? nkb - i * 4 : 4) << g.m_log;
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      const int u = u0 + d * WORKERS * 4, row = u & ((1 << g.m_log) - 1), col = (kb0 + i * 4 + (u >> g.m_log)) * 128 + sub * 16;
+      v[d][0] = v[d][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (u < units && row < g.M) {
+        const uint4* p = reinterpret_cast<const uint4*>(g.x + row * g.ldx + col);
+        if (col < g.K) v[d][0] = p[0];
+        if (col + 8 < g.K) v[d][1] = p[1];
+      }
+    }
+  };
+  if (!PACKED && warp < WORKERS) {
+    rwkv_chain_wait();
+    fetch(0, warp * 4 + (lane >> 3));
   }
-  rwkv_chain_trigger();
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  if (S > 1) cluster_arrive_relaxed();       // waited for before the first write to another CTA: it has started by then
 
   if (warp == WARP_TMA) {
     if (lane == 0) {
-      const int first = nkb < g.stages ? nkb : g.stages;
+      const int all = nkb * tiles, first = all < g.stages ? all : g.stages;
+      int kb = 0, n0 = slab0 * 128;
       for (int i = 0; i < first; ++i) {
         mbar_expect_tx(&bars->full[i], stage_bytes);
-        tma_load_2d(base + i * stage_bytes, &map_w, &bars->full[i], (kb0 + i) * 128, n0);
+        tma_load_2d(base + i * stage_bytes, &map_w, &bars->full[i], (kb0 + kb) * 128, n0);
+        if (++kb == nkb) { kb = 0; n0 += 128; }
       }
       rwkv_chain_wait();
       if (PACKED)
-        for (int i = 0; i < first; ++i)
-          tma_load_2d(base + i * stage_bytes + W_BYTES, &map_x, &bars->full[i], (kb0 + i) * 128, 0);
-      for (int i = first; i < nkb; ++i) {
-        const int s = i % g.stages;
-        if (!mbar_wait(&bars->empty[s], (i / g.stages - 1) & 1, bars, g.status, 221)) break;
+        for (int i = 0, k = 0; i < first; ++i) {
+          tma_load_2d(base + i * stage_bytes + W_BYTES, &map_x, &bars->full[i], (kb0 + k) * 128, 0);
+          if (++k == nkb) k = 0;
+        }
+      int s = 0;
+      uint32_t phase = 0;
+      for (int i = first; i < all; ++i) {
+        if (!mbar_wait(&bars->empty[s], phase, bars, g.status, 221)) break;
         mbar_expect_tx(&bars->full[s], stage_bytes);
-        tma_load_2d(base + s * stage_bytes, &map_w, &bars->full[s], (kb0 + i) * 128, n0);
-        if (PACKED) tma_load_2d(base + s * stage_bytes + W_BYTES, &map_x, &bars->full[s], (kb0 + i) * 128, 0);
+        tma_load_2d(base + s * stage_bytes, &map_w, &bars->full[s], (kb0 + kb) * 128, n0);
+        if (PACKED) tma_load_2d(base + s * stage_bytes + W_BYTES, &map_x, &bars->full[s], (kb0 + kb) * 128, 0);
+        if (++kb == nkb) { kb = 0; n0 += 128; }
+        if (++s == g.stages) { s = 0; phase ^= 1; }
       }
     }
   } else if (warp == WARP_MMA) {
-    if (lane == 0) {
-      // kind::mxf8f6f4: e4m3 operands, both K-major, E8M0 scales, M = 128, N = mpad
-      const uint32_t idesc = ((uint32_t)(g.mpad >> 3) << 17) | (1u << 23) | (1u << 27);
-      bool ok = true;
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem_base)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    __syncwarp();
+    tc_fence_before();
+    asm volatile("bar.arrive 2, 288;" ::: "memory");           // the workers read the address before they read the accumulator
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+    // kind::mxf8f6f4: e4m3 operands, both K-major, E8M0 scales, M = 128, N = mpad
+    const uint32_t idesc = ((uint32_t)(g.mpad >> 3) << 17) | (1u << 23) | (1u << 27);
+    bool ok = true;
+    int s = 0;
+    uint32_t phase = 0;
+    for (int t = 0; t < tiles && ok; ++t) {
+      const int a = t & (accs - 1);
+      const uint32_t d = tmem + a * 64;
+      if (t >= accs) ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_free[a], ((t - accs) / accs) & 1, bars, g.status, 225));
       for (int i = 0; i < nkb && ok; ++i) {
-        const int s = i % g.stages;
-        const uint32_t id = i & 3, sfa = tmem + SF_COL + (i >> 2) * 8, sfb = sfa + 4;
-        if (id == 0) {
-          if (!mbar_wait(&bars->x_ready[i >> 2], 0, bars, g.status, 222)) break;
-          tc_fence_after();
-          scales_to_tmem(sfa, scale_desc(sf + (i >> 2) * 1024));
-          scales_to_tmem(sfb, scale_desc(sf + (i >> 2) * 1024 + 512));
-        }
-        ok = mbar_wait(&bars->full[s], (i / g.stages) & 1, bars, g.status, 223);
+        const uint32_t id = i & 3, set = i >> 2, sfb = tmem + SF_COL + set * 4, w_set = max_groups + t * groups + set;
+        const uint32_t sfa = tmem + SF_COL + w_set * 4;
+        if (id == 0 && t == 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->x_ready[set], 0, bars, g.status, 222));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[s], phase, bars, g.status, 223));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t sa = base + s * stage_bytes, sb = PACKED ? sa + W_BYTES : xs + i * x_bytes;
+        if (elect_one()) {
+          if (id == 0) {
+            scales_to_tmem(sfa, scale_desc(sf + w_set * 512));
+            if (t == 0) scales_to_tmem(sfb, scale_desc(sf + set * 512));
+          }
+          const uint32_t sa = base + s * stage_bytes, sb = PACKED ? sa + W_BYTES : xs + i * x_bytes;
+          const uint64_t da = operand_desc(sa), db = operand_desc(sb);
+          const uint32_t desc = idesc | (id << 4) | (id << 29);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma(tmem, operand_desc(sa) + k * 2, operand_desc(sb) + k * 2, idesc | (id << 4) | (id << 29), sfa, sfb, (i | k) ? 1u : 0u);
-        umma_commit(&bars->empty[s]);
+          for (int k = 0; k < 4; ++k) umma(d, da + k * 2, db + k * 2, desc, sfa, sfb, (i | k) ? 1u : 0u);
+          umma_commit(&bars->empty[s]);
+          if (i == nkb - 1) umma_commit(&bars->acc_full[a]);
+        }
+        __syncwarp();
+        if (++s == g.stages) { s = 0; phase ^= 1; }
       }
-      umma_commit(&bars->acc_full);
     }
   } else {
-    // ---- scales of the weights: one byte per block, the same for all 128 rows
-    for (int i = warp; i < groups; i += WORKERS) {
-      const int kb = kb0 + i * 4 + (lane & 3);
-      uint32_t w = kb < all_kb ? (uint32_t)g.w_exp[(long long)blockIdx.x * all_kb + kb] << (8 * (lane & 3)) : 0u;
+    for (int i = warp; i < w_sets; i += WORKERS) {
+      uint32_t w = i == warp ? w_scale : weight_scale(i);
       w |= __shfl_xor_sync(0xffffffffu, w, 1);
       w |= __shfl_xor_sync(0xffffffffu, w, 2);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sf + i * 1024 + lane * 16), "r"(w) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sf + (max_groups + i) * 512 + lane * 16), "r"(w) : "memory");
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    rwkv_chain_wait();
     if (PACKED) {
       // ---- scales of the tokens: word of row r holds the bytes of four blocks
-      for (int u = threadIdx.x; u < groups * g.M; u += 32 * WORKERS) {
-        const int i = u / g.M, r = u % g.M;
+      rwkv_chain_wait();
+      for (int u = threadIdx.x; u < groups << g.m_log; u += 32 * WORKERS) {
+        const int i = u >> g.m_log, r = u & ((1 << g.m_log) - 1);
+        if (r >= g.M) continue;
         uint32_t w = 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
           if (i * 4 + b < nkb) w |= (uint32_t)g.x_exp[(long long)(kb0 + i * 4 + b) * g.x_lde + r] << (8 * b);
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(sf + i * 1024 + 512 + (r & 31) * 16 + (r >> 5) * 4), "r"(w) : "memory");
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(sf + i * 512 + (r & 31) * 16 + (r >> 5) * 4), "r"(w) : "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0)
         for (int i = 0; i < groups; ++i) mbar_arrive(&bars->x_ready[i]);
     } else {
-      // ---- pack the tokens: eight threads a block of 128, four blocks a thread in flight
-      constexpr int DEEP = 4;
-      const int part = lane & 7;
       for (int i = 0; i < groups; ++i) {
-        const int blocks = nkb - i * 4 < 4 ? nkb - i * 4 : 4, units = blocks * g.M;
+        const int units = (nkb - i * 4 < 4 ? nkb - i * 4 : 4) << g.m_log;
         for (int u0 = warp * 4 + (lane >> 3); u0 - (lane >> 3) < units; u0 += WORKERS * 4 * DEEP) {
-          uint4 v[DEEP][2];
+          if (i > 0 || u0 >= WORKERS * 4) fetch(i, u0);
 #pragma unroll
           for (int d = 0; d < DEEP; ++d) {
-            const int u = u0 + d * WORKERS * 4, row = u % g.M, kb = kb0 + i * 4 + u / g.M, col = kb * 128 + part * 16;
-            v[d][0] = v[d][1] = make_uint4(0u, 0u, 0u, 0u);
-            if (u < units) {
-              const uint4* p = reinterpret_cast<const uint4*>(g.x + row * g.ldx + col);
-              if (col < g.K) v[d][0] = p[0];
-              if (col + 8 < g.K) v[d][1] = p[1];
-            }
-          }
-#pragma unroll
-          for (int d = 0; d < DEEP; ++d) {
-            const int u = u0 + d * WORKERS * 4, row = u % g.M, b = u / g.M;
+            const int u = u0 + d * WORKERS * 4, row = u & ((1 << g.m_log) - 1), b = u >> g.m_log;
             float f[16];
             unpack8(v[d][0], f);
             unpack8(v[d][1], f + 8);
@@ -287,7 +392,7 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (u < units) {
+            if (u < units && row < g.M) {
               const uint32_t e = fp8_block_exponent(top);
               uint32_t q[4];
               const float s = fp8_inverse_scale(e == 255u ? 127u : e);
@@ -295,11 +400,11 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
               for (int j = 0; j < 4; ++j)
                 q[j] = e == 255u ? 0x7f7f7f7fu : fp8_pack4(f[4 * j] * s, f[4 * j + 1] * s, f[4 * j + 2] * s, f[4 * j + 3] * s);
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                           ::"r"(xs + (i * 4 + b) * x_bytes + row * 128 + ((part ^ (row & 7)) << 4)), "r"(q[0]), "r"(q[1]), "r"(q[2]),
+                           ::"r"(xs + (i * 4 + b) * x_bytes + row * 128 + ((sub ^ (row & 7)) << 4)), "r"(q[0]), "r"(q[1]), "r"(q[2]),
                              "r"(q[3])
                            : "memory");
-              if (part == 0)
-                asm volatile("st.shared.u8 [%0], %1;" ::"r"(sf + i * 1024 + 512 + (row & 31) * 16 + (row >> 5) * 4 + b), "r"(e)
+              if (sub == 0)
+                asm volatile("st.shared.u8 [%0], %1;" ::"r"(sf + i * 512 + (row & 31) * 16 + (row >> 5) * 4 + b), "r"(e)
                              : "memory");
             }
           }
@@ -309,20 +414,45 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         if (lane == 0) mbar_arrive(&bars->x_ready[i]);
       }
     }
-    // ---- this CTA's partial tile, [token][128 columns] in fp32, over the ring (every load of it has been consumed)
-    mbar_wait(&bars->acc_full, 0, bars, g.status, 224);
-    __syncwarp();
-    tc_fence_after();
+    asm volatile("bar.sync 2, 288;" ::: "memory");
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
     const int quarter = warp & 3;
-    // All mpad rows are stored: with the store under a test of the row, nvcc 12.9 dropped that of the last row of an unrolled
-    // iteration.
+    const uint32_t column = (quarter * 32 + lane) * 4;
+    for (int t = 0; t < tiles; ++t) {
+      // ---- partial rows to the CTAs that own the tokens (all mpad of them: rows beyond M are never read)
+      const int a = t & (accs - 1);
+      const bool ok = mbar_wait(&bars->acc_full[a], (t / accs) & 1, bars, g.status, 224);
+      __syncwarp();
+      tc_fence_after();
+      if (S > 1) cluster_wait();                 // (S > 1: one column block)
 #pragma unroll 1
-    for (int m = (warp >> 2) * 8; m < g.mpad; m += 16) {
-      float v[8];
-      tmem_ld8(tmem + ((uint32_t)(quarter * 32) << 16) + m, v);
+      for (int m = (warp >> 2) * 8; m < g.mpad; m += 16) {
+        float p[8];
+        tmem_ld8(tmem + ((uint32_t)(quarter * 32) << 16) + a * 64 + m, p);
+        if (S == 1) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + (m + e) * 512 + (quarter * 32 + lane) * 4), "f"(v[e]) : "memory");
+          for (int e = 0; e < 8; ++e) asm volatile("st.shared.f32 [%0], %1;" ::"r"(part + (m + e) * 512 + column), "f"(p[e]) : "memory");
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int at = z * own_tokens + ((m + e) >> slog);
+            uint32_t dst;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(part + at * 512 + column), "r"((m + e) & (S - 1)));
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(p[e]) : "memory");
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->acc_free[a]);
+      if (S > 1) {
+        cluster_arrive();
+        cluster_wait();
+      } else {
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      if (ok) finish<EPI>(g, part, slab0 + t, warp, lane, z, slog, own_tokens);
+      if (t + 1 < tiles) asm volatile("bar.sync 1, 256;" ::: "memory");
     }
   }
 
@@ -331,58 +461,18 @@ fp8_decode_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     const unsigned long long until = globaltimer_ns() + 1000000ull;      // loads in flight land before the memory is given up
     while (globaltimer_ns() < until) {}
   }
+  if (S > 1 && warp >= WORKERS) {                // the other two warps' part in both cluster barriers
+    cluster_wait();
+    cluster_arrive();
+    cluster_wait();
+  }
   tc_fence_before();
-  if (S > 1) cluster_sync(); else __syncthreads();
+  __syncthreads();
   if (warp == WARP_MMA) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                 ::"r"(*reinterpret_cast<volatile uint32_t*>(&bars->tmem_base)), "r"(TMEM_COLS));
   }
-  if (warp < WORKERS && !*reinterpret_cast<volatile int*>(&bars->abort_flag)) {
-    // ---- tokens z, z + S, ... of the cluster's sum, one warp a token, four columns a lane
-    const int n = n0 + lane * 4;
-    for (int m = z + warp * S; m < g.M; m += WORKERS * S) {
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int r = 0; r < S; ++r) {
-        uint32_t at;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(base + m * 512 + lane * 16), "r"(r));
-        float4 p;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w) : "r"(at));
-        f[0] += p.x; f[1] += p.y; f[2] += p.z; f[3] += p.w;
-      }
-      if (EPI == EPI_RELU_SQ) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f[e] = f[e] < 0.f || n + e >= g.N ? 0.f : f[e];
-          f[e] *= f[e];
-          top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const uint32_t e = fp8_block_exponent(top);
-        const float s = fp8_inverse_scale(e == 255u ? 127u : e);
-        if (n < g.q_ldv)
-          *reinterpret_cast<uint32_t*>(g.q_val + (long long)m * g.q_ldv + n) =
-              e == 255u ? 0x7f7f7f7fu : fp8_pack4(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
-        if (lane == 0) g.q_exp[(long long)blockIdx.x * g.q_lde + m] = (uint8_t)e;
-      } else if (g.vec) {
-        if (n < g.N) {
-          if (EPI == EPI_RESIDUAL) {
-            const uint2 p = *reinterpret_cast<const uint2*>(g.residual + m * g.ldr + n);
-            f[0] += bf16_lo(p.x); f[1] += bf16_hi(p.x); f[2] += bf16_lo(p.y); f[3] += bf16_hi(p.y);
-          }
-          *reinterpret_cast<uint2*>(g.c + m * g.ldc + n) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < g.N)
-            g.c[m * g.ldc + n + e] =
-                __float2bfloat16_rn(f[e] + (EPI == EPI_RESIDUAL ? __bfloat162float(g.residual[m * g.ldr + n + e]) : 0.f));
-      }
-    }
-  }
-  if (S > 1) cluster_sync();           // no CTA leaves while another reads its partial tile
 }
 
 int encode(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
@@ -414,14 +504,14 @@ int launch(const CUtensorMap& mw, const CUtensorMap& mx, const Args& g, int smem
   }
   if (e != cudaSuccess) return RWKV_ERR_CUDA_BASE + (int)e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((g.N + 127) / 128), (unsigned)g.split);
+  cfg.gridDim = dim3((unsigned)(((g.N + 127) / 128 + g.tiles - 1) / g.tiles), 1u << g.split_log);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = g.split;
+  attr[0].val.clusterDim.y = 1u << g.split_log;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -438,20 +528,28 @@ int split_for(int N, int K) {
   while (s < 8 && slabs * s < 120 && s * 2 <= kb) s *= 2;
   return s;
 }
+// Column blocks of a CTA: with more blocks than two CTAs on every SM, a CTA takes several and its ring runs on from one to
+// the next, so the weights keep streaming through the epilogues.
+int tiles_for(int N, int K, int split) {
+  const int slabs = (N + 127) / 128, groups = ((K + 127) / 128 + 3) / 4;
+  if (split > 1) return 1;
+  const int fit = MAX_SETS / groups - 1, want = (slabs + 2 * 148 - 1) / (2 * 148);
+  return want < fit ? want : fit < 1 ? 1 : fit;
+}
 
 struct Layout {
   int stages, smem;          // stages = 0: does not fit
 };
-Layout layout_for(int mpad, int K, int split, bool packed) {
-  const int kb = ((K + 127) / 128 + split - 1) / split;
-  if ((kb + 3) / 4 > MAX_GROUPS) return {0, 0};
+Layout layout_for(int mpad, int K, int split, int tiles, bool packed) {
+  const int kb = ((K + 127) / 128 + split - 1) / split, groups = (kb + 3) / 4;
+  if (groups > MAX_GROUPS) return {0, 0};
   const int stage = W_BYTES + (packed ? mpad * 128 : 0);
-  const int fixed = (packed ? 0 : kb * mpad * 128) + (kb + 3) / 4 * 1024 + (int)sizeof(Barriers) + 1024 + 64;
-  const int need = mpad * 512;                                       // the partial tile lies over the ring
+  const int fixed = (packed ? 0 : kb * mpad * 128) + groups * (1 + tiles) * 512 + (mpad + split - 1) / split * split * 512 +
+                    (int)sizeof(Barriers) + 1024 + 64;
   for (int budget = SMEM_MIN; budget <= SMEM_MAX; budget += SMEM_MAX - SMEM_MIN) {
     int stages = (budget - fixed) / stage;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
-    if (stages >= 3 && stages * stage >= need) return {stages, budget};
+    if (stages >= (kb < 3 ? kb : 3)) return {stages, budget};
   }
   return {0, 0};
 }
@@ -462,9 +560,9 @@ Layout layout_for(int mpad, int K, int split, bool packed) {
 // 2 - on bf16 tokens that it packs itself (never if `packed`: the tokens are packed already).  Depends on sizes only.
 RWKV_EXPORT int rwkv_fp8_decode_form(int M, int N, int K, int packed) {
   if (M < 1 || M > 128 || N < 1 || K < 1 || N > 0x7ffffe00 || K > 0x7ffffe00) return 0;
-  const int mpad = (M + 15) / 16 * 16, split = split_for(N, K);
-  if (!packed && K % 8 == 0 && M <= 16 && layout_for(mpad, K, split, false).stages) return 2;
-  return layout_for(mpad, K, split, true).stages ? 1 : 0;
+  const int mpad = (M + 15) / 16 * 16, split = split_for(N, K), tiles = tiles_for(N, K, split);
+  if (!packed && K % 8 == 0 && M <= 16 && layout_for(mpad, K, split, tiles, false).stages) return 2;
+  return layout_for(mpad, K, split, tiles, true).stages ? 1 : 0;
 }
 
 // x: bf16 rows (16-byte aligned, K a multiple of 8) or, if null, packed tokens in (a_val, a_exp) with blocks of one row;
@@ -479,8 +577,8 @@ int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t st) {
   if (!packed && (((uintptr_t)s.x & 15) || s.ldx % 8)) return RWKV_ERR_BAD_ALIGNMENT;
   if (s.epilogue == 2 ? !s.q_val || !s.q_exp || s.q_rows != 1 : !s.c || s.ldc < N || (s.epilogue == 1 && (!s.residual || s.ldr < N)))
     return RWKV_ERR_BAD_SHAPE;
-  const int mpad = (M + 15) / 16 * 16, split = split_for(N, K);
-  const Layout lay = layout_for(mpad, K, split, packed);
+  const int mpad = (M + 15) / 16 * 16, split = split_for(N, K), tiles = tiles_for(N, K, split);
+  const Layout lay = layout_for(mpad, K, split, tiles, packed);
   if (!lay.stages) return RWKV_ERR_TOO_LARGE;
   const int ldk = (K + 15) / 16 * 16;
   CUtensorMap mw, mx;
@@ -489,7 +587,9 @@ int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t st) {
   if (packed) r = encode(&mx, s.a_val, M, K, ldk, mpad); else mx = mw;
   if (r) return r;
   Args g = {};
-  g.M = M; g.N = N; g.K = K; g.mpad = mpad; g.stages = lay.stages; g.split = split;
+  g.M = M; g.N = N; g.K = K; g.mpad = mpad; g.stages = lay.stages; g.tiles = tiles;
+  while ((1 << g.split_log) < split) ++g.split_log;
+  while ((1 << g.m_log) < M) ++g.m_log;
   g.w_exp = (const uint8_t*)s.b_exp;
   g.x = (const bf16*)s.x; g.ldx = s.ldx;
   g.x_exp = (const uint8_t*)s.a_exp; g.x_lde = (M + 15) / 16 * 16;

@@ -173,7 +173,8 @@ def test_relu_sq_grad_packed(M, N, K, rows):
     packed_near(packed_product("nn_relu_sq_grad", d, w, M, N, rows, h), (D @ W) * slope, (D.abs() @ W.abs()) * slope + 1e-30, K + 64, rows)
 
 
-@pytest.mark.parametrize("N,K", [(128, 128), (40, 24), (200, 264), (2048, 2048), (640, 8192), (130, 1000), (8192, 512), (20000, 128)])
+@pytest.mark.parametrize("N,K", [(128, 128), (40, 24), (200, 264), (2048, 2048), (640, 8192), (130, 1000), (8192, 512), (20000, 128),
+                                 (40100, 136), (77000, 640), (200, 33000)])
 @pytest.mark.parametrize("M", [1, 2, 16, 17, 64, 100, 128])
 def test_few_rows(M, N, K):
     """The decode kernel: bf16 tokens packed inside it, packed tokens, and its three epilogues."""
