@@ -27,6 +27,7 @@ from typing import Optional, Union
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import fp8_native as native
 from . import reference
 
 BLOCK = reference.FP8_BLOCK
@@ -45,12 +46,14 @@ class Fp8Blocks:
     ``offset`` in the byte buffer ``data``: values row by row, each row padded to 16 bytes, then the exponents
     (``[ceil(R/128)][ceil(C/128)]`` for tiles, ``[ceil(C/128)][R padded to 16]`` for row blocks)."""
 
-    __slots__ = ("data", "offset", "R", "C", "rows", "shape", "dtype", "exponent_offset")
+    __slots__ = ("data", "offset", "R", "C", "rows", "shape", "dtype", "exponent_offset", "address", "exponent_address")
 
     def __init__(self, data: torch.Tensor, offset: int, R: int, C: int, rows: int, shape=None, dtype=torch.bfloat16):
         self.data, self.offset, self.R, self.C, self.rows, self.dtype = data, offset, R, C, rows, dtype
         self.shape = (R, C) if shape is None else shape
         self.exponent_offset = R * (-(-C // 16) * 16)
+        self.address = data.data_ptr() + offset
+        self.exponent_address = self.address + self.exponent_offset
 
     @property
     def device(self) -> torch.device:
@@ -59,10 +62,6 @@ class Fp8Blocks:
     @property
     def nbytes(self) -> int:
         return sum(_sizes(self.R, self.C, self.rows))
-
-    @property
-    def address(self) -> int:
-        return self.data.data_ptr() + self.offset
 
     @property
     def values(self) -> torch.Tensor:
@@ -82,8 +81,16 @@ class Fp8Blocks:
         data = self.data.to(device)
         return self if data is self.data else Fp8Blocks(data, self.offset, self.R, self.C, self.rows, self.shape, self.dtype)
 
+    def __reduce__(self):
+        return Fp8Blocks, (self.data, self.offset, self.R, self.C, self.rows, self.shape, self.dtype)
+
     def __repr__(self) -> str:
         return f"Fp8Blocks(shape={tuple(self.shape)}, rows={self.rows}, dtype={self.dtype}, device={self.device})"
+
+
+def _matrix(device, R: int, C: int, rows: int, shape=None, dtype=torch.bfloat16) -> Fp8Blocks:
+    """An uninitialised packed matrix in a buffer of its own."""
+    return Fp8Blocks(torch.empty(sum(_sizes(R, C, rows)), dtype=torch.uint8, device=device), 0, R, C, rows, shape, dtype)
 
 
 def _room(device, *specs):
@@ -124,7 +131,7 @@ class _HostRun:
         out.copy_(_f32(a).t() @ _f32(b))
 
     def nt_frozen(self, x, w, out, hidden=None):
-        (x8,) = _room(x.device, (*x.shape, 1))
+        x8 = _matrix(x.device, *x.shape, 1)
         self.pack(x, x8)
         self.nt(x8, w, out) if hidden is None else self.nt_relu_sq(x8, w, hidden)
 
@@ -141,74 +148,74 @@ class _HostRun:
 class _DeviceRun:
     """The steps of an operator, collected and launched together."""
 
-    def __init__(self, device):
-        from . import fp8_native
+    __slots__ = ("device", "steps", "keep")
 
-        self.native, self.device, self.steps = fp8_native, device, []
+    def __init__(self, device):
+        self.device, self.steps = device, []
         self.keep = []                            # copies made on the way: their memory is not reused before the launch
 
     def pack(self, x, q):
         if q.R:
             if (q.C > 1 and x.stride(1) != 1) or (q.R > 1 and x.stride(0) < q.C):
                 x = x.contiguous()
-            self.steps.append(self.native.pack(x, q))
+            self.steps.append(native.pack(x, q))
             self.keep.append(x)
 
     def unpack(self, p, out):
         if p.R:
-            self.steps.append(self.native.unpack(p, out))
+            self.steps.append(native.unpack(p, out))
 
     def nt(self, a, b, out, residual=None):
         if not a.R:
             return
-        if a.rows == 1 and self.native.decode_form(a.R, b.R, b.C, True):
+        if a.rows == 1 and native.decode_form(a.R, b.R, b.C, True):
             # its predecessor is the step that packed `a`, which does not write the weights
-            self.steps.append(self.native.decode(a, b, out, residual, chained=bool(self.steps)))
+            self.steps.append(native.decode(a, b, out, residual, chained=bool(self.steps)))
         else:
-            self.steps.append(self.native.mm_nt(a, b, out, residual))
+            self.steps.append(native.mm_nt(a, b, out, residual))
         self.keep.append(residual)
 
     def nt_frozen(self, x, w, out, hidden=None):
         """``out = P(x) w^T`` or ``hidden = P(relu(P(x) w^T)^2)`` with ``x`` packed row by row."""
         if not x.shape[0]:
             return
-        form = self.native.decode_form(x.shape[0], w.R, w.C)
+        form = native.decode_form(x.shape[0], w.R, w.C)
         if form == 2:
-            x = self.native.decode_input(x)
+            x = native.decode_input(x)
             self.keep.append(x)
-            self.steps.append(self.native.decode(x, w, out, q=hidden))
+            self.steps.append(native.decode(x, w, out, q=hidden))
             return
-        (x8,) = _room(x.device, (*x.shape, 1))
+        x8 = _matrix(x.device, x.shape[0], x.shape[1], 1)
         self.keep.append(x8)
         self.pack(x, x8)
         if hidden is None:
             self.nt(x8, w, out)
         elif form:
-            self.steps.append(self.native.decode(x8, w, q=hidden, chained=True))
+            self.steps.append(native.decode(x8, w, q=hidden, chained=True))
         else:
             self.nt_relu_sq(x8, w, hidden)
 
     def nn(self, a, b, out):
         if a.R:
-            self.steps.append(self.native.mm_nn(a, b, out))
+            self.steps.append(native.mm_nn(a, b, out))
 
     def tn(self, a, b, out):
         if a.R:
-            self.steps.append(self.native.mm_tn(a, b, out))
+            self.steps.append(native.mm_tn(a, b, out))
         else:
             out.zero_()
 
     def nt_relu_sq(self, a, b, q):
         if a.R:
-            self.steps.append(self.native.mm_nt_relu_sq(a, b, q))
+            self.steps.append(native.mm_nt_relu_sq(a, b, q))
 
     def nn_relu_sq_grad(self, a, b, h, q):
         if a.R:
-            self.steps.append(self.native.mm_nn_relu_sq_grad(a, b, h, q))
+            self.steps.append(native.mm_nn_relu_sq_grad(a, b, h, q))
 
     def go(self):
         if self.steps:
-            self.native.run(self.device, self.steps)
+            native.run(self.device, self.steps)
 
 
 def _run_on(t: torch.Tensor):
@@ -229,8 +236,7 @@ def pack_fp8(x: torch.Tensor, rows: int = BLOCK) -> Fp8Blocks:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"pack_fp8: the last dimension must not be empty, got shape {tuple(x.shape)}")
     x2 = _rows_of(x.detach())
-    (p,) = _room(x.device, (*x2.shape, rows))
-    p.shape, p.dtype = x.shape, x.dtype
+    p = _matrix(x.device, x2.shape[0], x2.shape[1], rows, x.shape, x.dtype)
     run = _run_on(x)
     run.pack(x2, p)
     run.go()
@@ -290,7 +296,7 @@ class _Linear(torch.autograd.Function):
         (data,) = ctx.saved_tensors
         x8, w8 = (None if m is None else Fp8Blocks(data, *m) for m in ctx.meta)
         d2 = _rows_of(dy)
-        (d8,) = _room(dy.device, (*d2.shape, BLOCK))
+        d8 = _matrix(dy.device, d2.shape[0], d2.shape[1], BLOCK)
         run = _run_on(dy)
         run.pack(d2, d8)
         dx = dw = None
@@ -318,7 +324,7 @@ class _LinearFrozen(torch.autograd.Function):
     def backward(ctx, dy):
         w8 = Fp8Blocks(ctx.saved_tensors[0], *ctx.meta)
         d2 = _rows_of(dy)
-        (d8,) = _room(dy.device, (*d2.shape, 1))
+        d8 = _matrix(dy.device, d2.shape[0], d2.shape[1], 1)
         dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device)
         run = _run_on(dy)
         run.pack(d2, d8)
@@ -453,7 +459,7 @@ class _ChannelMixFrozen(torch.autograd.Function):
 
 def _channel_mix_frozen(x, k8, v8, residual):
     x2 = _rows_of(x)
-    (h8,) = _room(x.device, (x2.shape[0], k8.R, 1))
+    h8 = _matrix(x.device, x2.shape[0], k8.R, 1)
     y = torch.empty(residual.shape, dtype=x.dtype, device=x.device)
     run = _run_on(x)
     run.nt_frozen(x2, k8, None, h8)

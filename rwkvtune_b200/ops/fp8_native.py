@@ -19,39 +19,39 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _PACK, _UNPACK, _GEMM, _DECODE = 0, 1, 2, 3
 _STORE, _RESIDUAL, _RELU_SQ, _RELU_SQ_GRAD = 0, 1, 2, 3
 _record = struct.Struct("=12i3q12Q").pack      # Fp8Step, field by field
-_declared = False
+_launch = None                                 # rwkv_fp8_run, bound at the first call
+_status_address = {}
 
 
 def _status(device: torch.device) -> int:
-    return gemm_native._status(device).data_ptr()
+    at = _status_address.get(device.index)
+    if at is None:
+        at = _status_address[device.index] = gemm_native._status(device).data_ptr()
+    return at
 
 
 def pack(x: torch.Tensor, q) -> bytes:
     """``x [R, C]`` with unit inner stride -> ``q``."""
-    at = q.address
     return _record(_PACK, q.R, q.C, 0, 0, q.rows, _DTYPES[x.dtype], 0, 0, 0, 0, 0, x.stride(0) if q.R > 1 else q.C, 0, 0,
-                   x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, at, at + q.exponent_offset, 0)
+                   x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, q.address, q.exponent_address, 0)
 
 
 def unpack(p, out: torch.Tensor) -> bytes:
-    at = p.address
-    return _record(_UNPACK, p.R, p.C, 0, p.rows, 0, _DTYPES[out.dtype], 0, 0, 0, 0, 0, 0, p.C, 0, 0, at, at + p.exponent_offset,
-                   0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0)
+    return _record(_UNPACK, p.R, p.C, 0, p.rows, 0, _DTYPES[out.dtype], 0, 0, 0, 0, 0, 0, p.C, 0, 0, p.address,
+                   p.exponent_address, 0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0)
 
 
 def _product(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, out=None, residual=None, h=None, q=None) -> bytes:
-    pa, pb = a.address, b.address
-    ph = pq = he = qe = qr = pr = ldr = 0
+    ph = he = pq = qe = qr = pr = ldr = 0
     if h is not None:
-        ph = h.address
-        he = ph + h.exponent_offset
+        ph, he = h.address, h.exponent_address
     if q is not None:
-        pq, qr = q.address, q.rows
-        qe = pq + q.exponent_offset
+        pq, qe, qr = q.address, q.exponent_address, q.rows
     if residual is not None:
         pr, ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
-    return _record(_GEMM, M, N, K, a.rows, qr, 0, a_mn, b_mn, epilogue, 0, 0, 0, N, ldr, 0, pa, pa + a.exponent_offset,
-                   pb, pb + b.exponent_offset, 0 if out is None else out.data_ptr(), pr, ph, he, pq, qe, _status(a.data.device))
+    return _record(_GEMM, M, N, K, a.rows, qr, 0, a_mn, b_mn, epilogue, 0, 0, 0, N, ldr, 0, a.address, a.exponent_address,
+                   b.address, b.exponent_address, 0 if out is None else out.data_ptr(), pr, ph, he, pq, qe,
+                   _status(a.data.device))
 
 
 def mm_nt(a, b, out, residual=None) -> bytes:
@@ -95,26 +95,34 @@ def decode_input(x: torch.Tensor) -> torch.Tensor:
 
 def decode(x, b, out=None, residual=None, q=None, chained: bool = False) -> bytes:
     """``out = x @ b^T (+ residual)`` or ``q = packed relu(x @ b^T)^2`` for at most 128 rows; ``x`` is packed or bf16."""
-    packed = not isinstance(x, torch.Tensor)
-    pb = b.address
-    M, N, K = (x.R if packed else x.shape[0]), b.R, b.C
-    px, pa, ae, ldx = (0, x.address, x.address + x.exponent_offset, 0) if packed else \
-        (x.data_ptr(), 0, 0, x.stride(0) if M > 1 else K)
-    pq = 0 if q is None else q.address
-    return _record(_DECODE, M, N, K, 1, 1, 0, 0, 0, _RELU_SQ if q is not None else _STORE if residual is None else _RESIDUAL,
-                   int(chained), 0, ldx, N, 0 if residual is None else residual.stride(0) if M > 1 else N, px, pa, ae, pb,
-                   pb + b.exponent_offset, 0 if out is None else out.data_ptr(), 0 if residual is None else residual.data_ptr(),
-                   0, 0, pq, 0 if q is None else pq + q.exponent_offset, _status(b.data.device))
+    N, K = b.R, b.C
+    if isinstance(x, torch.Tensor):
+        M, px, pa, ae = x.shape[0], x.data_ptr(), 0, 0
+        ldx = x.stride(0) if M > 1 else K
+    else:
+        M, px, pa, ae, ldx = x.R, 0, x.address, x.exponent_address, 0
+    epilogue, po, pr, ldr, pq, qe = _STORE, 0, 0, 0, 0, 0
+    if q is not None:
+        epilogue, pq, qe = _RELU_SQ, q.address, q.exponent_address
+    else:
+        po = out.data_ptr()
+        if residual is not None:
+            epilogue, pr, ldr = _RESIDUAL, residual.data_ptr(), residual.stride(0) if M > 1 else N
+    return _record(_DECODE, M, N, K, 1, 1, 0, 0, 0, epilogue, chained, 0, ldx, N, ldr, px, pa, ae, b.address,
+                   b.exponent_address, po, pr, 0, 0, pq, qe, _status(b.data.device))
 
 
 def run(device: torch.device, steps) -> None:
     """Launch ``steps`` in order on the device's current stream."""
-    global _declared
-    if not _declared:
-        _ext.lib().rwkv_fp8_run.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p]
-        _declared = True
-    if device.index is not None and device.index != torch._C._cuda_getDevice():
+    global _launch
+    index = device.index
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return run(device, steps)
-    _ext.LAUNCH_COUNT += len(steps) - 1
-    _ext.call("rwkv_fp8_run", b"".join(steps), len(steps), _ext.stream())
+    if _launch is None:
+        _launch = _ext.lib().rwkv_fp8_run
+        _launch.argtypes, _launch.restype = [ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p], ctypes.c_int
+    _ext.LAUNCH_COUNT += len(steps)
+    status = _launch(b"".join(steps), len(steps), torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _ext.check(status, "rwkv_fp8_run")
