@@ -17,7 +17,13 @@ RWKV_EXPORT int rwkv_fp8_run(const Fp8Step* steps, int count, void* stream) {
     switch (s.kind) {
       case FP8_STEP_PACK: r = rwkv_fp8_pack(s.x, s.dtype, s.ldx, s.q_val, s.q_exp, s.M, s.N, s.q_rows, stream); break;
       case FP8_STEP_UNPACK: r = rwkv_fp8_unpack(s.a_val, s.a_exp, s.c, s.dtype, s.ldc, s.M, s.N, s.a_rows, stream); break;
-      case FP8_STEP_GEMM: r = rwkv_fp8_gemm(s, (cudaStream_t)stream); break;
+      case FP8_STEP_GEMM:
+        if (!s.with_next) {
+          r = rwkv_fp8_gemm(s, (cudaStream_t)stream);
+        } else if (i + 1 < count && steps[i + 1].kind == FP8_STEP_GEMM) {
+          r = rwkv_fp8_gemm_two(s, steps[++i], (cudaStream_t)stream);
+        }
+        break;
       case FP8_STEP_DECODE: r = rwkv_fp8_decode(s, (cudaStream_t)stream); break;
       default: break;
     }

@@ -11,7 +11,7 @@ struct Fp8Step {
   int dtype;                 // pack, unpack: type of the plain side (0 bf16, 1 fp16, 2 fp32)
   int a_mn, b_mn, epilogue;  // gemm: see gemm_fp8_tcgen05.cu
   int chained;               // decode: may start before its predecessor has finished (see gemm_fp8_decode.cu)
-  int reserved;
+  int with_next;             // gemm: this record and the next are one launch
   long long ldx, ldc, ldr;   // row strides of x (pack), c and the residual
   const void* x;
   const void *a_val, *a_exp, *b_val, *b_exp;
@@ -23,4 +23,5 @@ struct Fp8Step {
 };
 
 int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t stream);
+int rwkv_fp8_gemm_two(const Fp8Step& s, const Fp8Step& t, cudaStream_t stream);
 int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t stream);

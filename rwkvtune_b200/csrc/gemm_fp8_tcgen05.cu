@@ -83,6 +83,18 @@ struct Args {
   long long q_ldv, q_lde;        // leading dimensions of the packed result (and of h)
   int* status;
 };
+// One product, or two of the same kind in one launch: their tiles follow one another, so the second fills the SMs that the
+// first's last round leaves idle (the two weight gradients of a feed-forward half: 2 x 256 tiles of 74 at a time in 7 rounds
+// instead of 2 x 4).
+struct alignas(64) Problem {
+  CUtensorMap a, b, out, in;
+  Args g;
+  int tiles_n, tiles, num_kb, pad[1];
+};
+template <int COUNT>
+struct Problems {
+  Problem p[COUNT];
+};
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -258,11 +270,9 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-template <bool A_MN, bool B_MN, int EPI, int Q_ROWS>
+template <bool A_MN, bool B_MN, int EPI, int Q_ROWS, int COUNT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
-gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_in,
-                const __grid_constant__ Args g) {
+gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t raw = smem_u32(smem_dyn);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -274,10 +284,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();            // 0 = leader
   const int pair = (int)blockIdx.x >> 1, n_pairs = (int)gridDim.x >> 1;
-  const int M = g.M, N = g.N;
-  const int tiles_n = (N + TN - 1) / TN, num_tiles = ((M + 2 * TM - 1) / (2 * TM)) * tiles_n;
-  const int num_kb = (g.K + TK - 1) / TK;
-  int* const status = g.status;
+  const int tiles0 = all.p[0].tiles, num_tiles = tiles0 + (COUNT > 1 ? all.p[COUNT - 1].tiles : 0);
+  int* const status = all.p[0].g.status;
+  // the problem of a tile, its first row and its first column
+  const auto locate = [&](int tile, int& m0, int& n0) -> const Problem& {
+    const bool second = COUNT > 1 && tile >= tiles0;
+    const Problem& p = second ? all.p[COUNT - 1] : all.p[0];
+    if (second) tile -= tiles0;
+    m0 = (tile / p.tiles_n) * (2 * TM) + (int)rank * TM;
+    n0 = (tile % p.tiles_n) * TN;
+    return p;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
@@ -306,16 +323,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += n_pairs) {
-        const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM;
-        const int n0 = (tile % tiles_n) * TN + (int)rank * 128;
+        int m0, n0;
+        const Problem& p = locate(tile, m0, n0);
+        n0 += (int)rank * 128;
+        const int num_kb = p.num_kb;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&bars->empty[stage], phase ^ 1, bars, status, 211)) { ok = false; break; }
           if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * STAGE_BYTES);
           const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[stage]), 0);
           const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OP_BYTES;
           const int k0 = kb * TK;
-          tma_load_2d_pair(sa, &map_a, full_leader, A_MN ? m0 : k0, A_MN ? k0 : m0);
-          tma_load_2d_pair(sb, &map_b, full_leader, B_MN ? n0 : k0, B_MN ? k0 : n0);
+          tma_load_2d_pair(sa, &p.a, full_leader, A_MN ? m0 : k0, A_MN ? k0 : m0);
+          tma_load_2d_pair(sb, &p.b, full_leader, B_MN ? n0 : k0, B_MN ? k0 : n0);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -332,6 +351,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += n_pairs, ++local) {
         const uint32_t d_tmem = tmem_base + (local & 1) * ACC1_COL;
+        const int num_kb = COUNT > 1 && tile >= tiles0 ? all.p[COUNT - 1].num_kb : all.p[0].num_kb;
         for (int kb = 0; kb < num_kb; ++kb) {
           const uint32_t sfa = tmem_base + SF_COL + sf * SF_COLS, sfb = sfa + SF_B_OFFSET;
           const uint32_t id = kb % SF_GROUP;
@@ -370,18 +390,20 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   } else if (warp == WARP_SCALE) {
     // Sets of scales: word r of an operand holds the bytes of rows r (128 of A, 256 of B) for four blocks of the
     // contraction; word r goes to lane r % 32, column r / 32.
-    const bool by_row = !A_MN && g.a_rows == 1;
-    const int sets = (num_kb + SF_GROUP - 1) / SF_GROUP;
+    const bool by_row = !A_MN && COUNT == 1 && all.p[0].g.a_rows == 1;
     int sf = 0;
     uint32_t sf_phase = 0;
     // lanes 0-3: A, 4-7 and 8-11: the two column blocks of B; blocks of one row: four rows a lane
     auto fetch = [&](int tile, int set, uint32_t& byte, uint32_t (&rows4)[4]) {
-      const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM, n0 = (tile % tiles_n) * TN;
+      int m0, n0;
+      const Problem& p = locate(tile, m0, n0);
+      const Args& g = p.g;
+      const int num_kb = p.num_kb;
       const int which = lane >> 2, kb = set * SF_GROUP + (lane & 3);
       byte = 0;
       if (kb < num_kb) {
-        if (which == 0 && !by_row && m0 < M) byte = __ldg(g.a_exp + (long long)(m0 >> 7) * g.a_sm + (long long)kb * g.a_sk);
-        if ((which == 1 || which == 2) && n0 + (which - 1) * 128 < N)
+        if (which == 0 && !by_row && m0 < g.M) byte = __ldg(g.a_exp + (long long)(m0 >> 7) * g.a_sm + (long long)kb * g.a_sk);
+        if ((which == 1 || which == 2) && n0 + (which - 1) * 128 < g.N)
           byte = __ldg(g.b_exp + (long long)((n0 >> 7) + which - 1) * g.b_sn + (long long)kb * g.b_sk);
       }
 #pragma unroll
@@ -390,16 +412,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (by_row && set * SF_GROUP + i < num_kb && m0 + 4 * lane < g.a_ld)
           rows4[i] = __ldg(reinterpret_cast<const uint32_t*>(g.a_exp + (long long)(set * SF_GROUP + i) * g.a_ld + m0 + 4 * lane));
       }
+      return (num_kb + SF_GROUP - 1) / SF_GROUP;
     };
     uint32_t next_byte, next_rows[4];
-    int tile = pair, set = 0;
-    if (tile < num_tiles) fetch(tile, 0, next_byte, next_rows);
+    int tile = pair, set = 0, sets = 0;
+    if (tile < num_tiles) sets = fetch(tile, 0, next_byte, next_rows);
     while (tile < num_tiles) {
       uint32_t byte = next_byte, rows4[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) rows4[i] = next_rows[i];
       if (++set == sets) { set = 0; tile += n_pairs; }
-      if (tile < num_tiles) fetch(tile, set, next_byte, next_rows);      // one set ahead of the one that is written
+      if (tile < num_tiles) sets = fetch(tile, set, next_byte, next_rows);      // one set ahead of the one that is written
       if (!warp_wait(&bars->sf_empty[sf], sf_phase ^ 1, bars, status, 215)) break;
       byte <<= 8 * (lane & 3);
       byte |= __shfl_xor_sync(0xffffffffu, byte, 1);
@@ -435,7 +458,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t free_leader = map_to_cta(smem_u32(&bars->acc_free), 0);
     int local = 0;
     for (int tile = pair; tile < num_tiles; tile += n_pairs, ++local) {
-      const int m0 = (tile / tiles_n) * (2 * TM) + (int)rank * TM, gn0 = (tile % tiles_n) * TN + group * 128;
+      int m0, gn0;
+      const Problem& p = locate(tile, m0, gn0);
+      gn0 += group * 128;
+      const Args& g = p.g;
+      const int M = g.M, N = g.N;
       const int gm = m0 + row;
       const int acc = local & 1;
       const bool shared_columns = group != acc;    // accumulator 0 shares its last 64 columns, accumulator 1 its first
@@ -443,7 +470,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       // and replaced in place by the result.
       const bool residual_by_tma = EPI == EPI_RESIDUAL && !g.direct;
       if ((EPI == EPI_RELU_SQ_GRAD || residual_by_tma) && elected)
-        fetch_input(stage_addr, &map_in, &bars->in_full[group], gn0 + (EPI == EPI_RESIDUAL && acc == 0 ? 64 : 0), m0);
+        fetch_input(stage_addr, &p.in, &bars->in_full[group], gn0 + (EPI == EPI_RESIDUAL && acc == 0 ? 64 : 0), m0);
       if (!epi_all(group, mbar_wait(&bars->acc_full[acc], (local >> 1) & 1, bars, status, 216))) break;
       tc_fence_after();
       // a group without shared columns arrives at once: it has read all of the tile before
@@ -457,7 +484,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           uint32_t v[64];
           tmem_ld32(t_row + chunk * 64, v);
           tmem_ld32(t_row + chunk * 64 + 32, v + 32);
-          if (residual_by_tma && i == 1 && elected) fetch_input(stage_addr, &map_in, &bars->in_full[group], c0, m0);
+          if (residual_by_tma && i == 1 && elected) fetch_input(stage_addr, &p.in, &bars->in_full[group], c0, m0);
           tmem_wait_ld(v);
           if (i == 0 && shared_columns) {
             tc_fence_before();
@@ -489,7 +516,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             epi_sync(group);
             if (elected && m0 < M && c0 < N) {
-              tma_store_2d(&map_out, stage_addr, c0, m0);
+              tma_store_2d(&p.out, stage_addr, c0, m0);
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
           } else {                                                // unaligned rows: copied out value by value
@@ -580,7 +607,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         epi_sync(group);
         if (m0 < M && gn0 < N) {
           if (elected) {
-            tma_store_2d(&map_out, stage_addr, gn0, m0);
+            tma_store_2d(&p.out, stage_addr, gn0, m0);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             if (Q_ROWS == 128) g.q_exp[(long long)(m0 >> 7) * g.q_lde + nb] = (uint8_t)e;
           }
@@ -623,9 +650,9 @@ int encode(CUtensorMap* map, CUtensorMapDataType type, int elem, const void* ptr
   return r == CUDA_SUCCESS ? RWKV_OK : RWKV_ERR_CUDA_BASE + 900 + (int)r;
 }
 
-template <bool A_MN, bool B_MN, int EPI, int Q_ROWS>
-int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const CUtensorMap& mi, const Args& g, cudaStream_t st) {
-  auto kern = gemm_fp8_kernel<A_MN, B_MN, EPI, Q_ROWS>;
+template <bool A_MN, bool B_MN, int EPI, int Q_ROWS, int COUNT = 1>
+int launch(const Problems<COUNT>& all, cudaStream_t st) {
+  auto kern = gemm_fp8_kernel<A_MN, B_MN, EPI, Q_ROWS, COUNT>;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -637,14 +664,57 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, 
     if (e != cudaSuccess) return RWKV_ERR_CUDA_BASE + (int)e;
     configured.fetch_or(bit);
   }
-  const long long tiles = (long long)((g.M + 2 * TM - 1) / (2 * TM)) * ((g.N + TN - 1) / TN);
-  if (tiles > 0x3fffffff) return RWKV_ERR_TOO_LARGE;
+  long long tiles = 0;
+  for (int i = 0; i < COUNT; ++i) tiles += all.p[i].tiles;
   const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
-  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, st>>>(ma, mb, mo, mi, g);
+  kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, st>>>(all);
   return rwkv_launch_status();
 }
 
 inline int up(int n, int m) { return (n + m - 1) / m * m; }
+
+// Checks a record and fills in a problem.
+int describe(const Fp8Step& s, Problem& p) {
+  const int M = s.M, N = s.N, K = s.K, a_mn = s.a_mn, b_mn = s.b_mn, epilogue = s.epilogue, q_rows = s.q_rows;
+  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7ffffe00 || N > 0x7ffffe00 || K > 0x7ffffe00) return RWKV_ERR_BAD_SHAPE;
+  if (!(s.a_rows == 128 || (s.a_rows == 1 && !a_mn)) || epilogue < 0 || epilogue > 3) return RWKV_ERR_BAD_SHAPE;
+  if (epilogue <= 1 ? (!s.c || s.ldc < N || (epilogue == 1 && (!s.residual || s.ldr < N)))
+                    : (!s.q_val || !s.q_exp || !(q_rows == 1 || q_rows == 128) ||
+                       (epilogue == 3 && (!s.h_val || !s.h_exp || ((uintptr_t)s.h_val & 15)))))
+    return RWKV_ERR_BAD_SHAPE;
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, b16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  int r = a_mn ? encode(&p.a, u8, 1, s.a_val, K, M, up(M, 16)) : encode(&p.a, u8, 1, s.a_val, M, K, up(K, 16));
+  if (r) return r;
+  r = b_mn ? encode(&p.b, u8, 1, s.b_val, K, N, up(N, 16)) : encode(&p.b, u8, 1, s.b_val, N, K, up(K, 16));
+  if (r) return r;
+  const int mb_n = up(M, 128) / 128, nb_n = up(N, 128) / 128, kb_n = up(K, 128) / 128;
+  const long long tiles = (long long)(up(M, 2 * TM) / (2 * TM)) * (up(N, TN) / TN);
+  if (tiles > 0x1fffffff) return RWKV_ERR_TOO_LARGE;
+  p.tiles = (int)tiles; p.tiles_n = up(N, TN) / TN; p.num_kb = kb_n;
+  Args& g = p.g;
+  g = {};
+  g.M = M; g.N = N; g.K = K;
+  g.a_exp = (const uint8_t*)s.a_exp; g.b_exp = (const uint8_t*)s.b_exp;
+  g.a_rows = s.a_rows;
+  g.a_ld = up(M, 16);
+  g.a_sm = a_mn ? 1 : kb_n; g.a_sk = a_mn ? mb_n : 1;
+  g.b_sn = b_mn ? 1 : kb_n; g.b_sk = b_mn ? nb_n : 1;
+  g.c = (bf16*)s.c; g.residual = (const bf16*)s.residual; g.ldc = s.ldc; g.ldr = s.ldr;
+  g.h_exp = (const uint8_t*)s.h_exp; g.q_exp = (uint8_t*)s.q_exp;
+  g.q_ldv = up(N, 16);
+  g.q_lde = q_rows == 1 ? up(M, 16) : nb_n;
+  g.status = (int*)s.status;
+  p.out = p.in = p.a;                  // maps that the epilogue does not use are never read
+  if (epilogue <= 1) {
+    g.direct = ((uintptr_t)s.c & 15) || (s.ldc & 7) || (epilogue == 1 && (((uintptr_t)s.residual & 15) || (s.ldr & 7)));
+    if (!g.direct) r = encode(&p.out, b16, 2, s.c, M, N, s.ldc);
+    if (!r && epilogue == 1 && !g.direct) r = encode(&p.in, b16, 2, s.residual, M, N, s.ldr);
+  } else {
+    r = encode(&p.out, u8, 1, s.q_val, M, N, g.q_ldv);
+    if (!r && epilogue == 3) r = encode(&p.in, u8, 1, s.h_val, M, N, g.q_ldv);
+  }
+  return r;
+}
 
 }  // namespace
 
@@ -656,61 +726,30 @@ inline int up(int n, int m) { return (n + m - 1) / m * m; }
 //            the packed result and h are [M,N] with blocks of q_rows rows
 //   status: device int, set non-zero if a device-side wait expired
 int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t st) {
-  const int M = s.M, N = s.N, K = s.K, a_mn = s.a_mn, b_mn = s.b_mn, epilogue = s.epilogue, q_rows = s.q_rows;
-  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7ffffe00 || N > 0x7ffffe00 || K > 0x7ffffe00) return RWKV_ERR_BAD_SHAPE;
-  if (!(s.a_rows == 128 || (s.a_rows == 1 && !a_mn)) || epilogue < 0 || epilogue > 3) return RWKV_ERR_BAD_SHAPE;
-  if (epilogue <= 1 ? (!s.c || s.ldc < N || (epilogue == 1 && (!s.residual || s.ldr < N)))
-                    : (!s.q_val || !s.q_exp || !(q_rows == 1 || q_rows == 128) ||
-                       (epilogue == 3 && (!s.h_val || !s.h_exp || ((uintptr_t)s.h_val & 15)))))
-    return RWKV_ERR_BAD_SHAPE;
-  CUtensorMap ma, mb, mo, mi;
-  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  int r = a_mn ? encode(&ma, u8, 1, s.a_val, K, M, up(M, 16)) : encode(&ma, u8, 1, s.a_val, M, K, up(K, 16));
+  Problems<1> all;
+  const int r = describe(s, all.p[0]);
   if (r) return r;
-  r = b_mn ? encode(&mb, u8, 1, s.b_val, K, N, up(N, 16)) : encode(&mb, u8, 1, s.b_val, N, K, up(K, 16));
-  if (r) return r;
-  Args g = {};
-  g.M = M; g.N = N; g.K = K;
-  g.a_exp = (const uint8_t*)s.a_exp; g.b_exp = (const uint8_t*)s.b_exp;
-  g.a_rows = s.a_rows;
-  g.a_ld = up(M, 16);
-  const int mb_n = up(M, 128) / 128, nb_n = up(N, 128) / 128, kb_n = up(K, 128) / 128;
-  g.a_sm = a_mn ? 1 : kb_n; g.a_sk = a_mn ? mb_n : 1;
-  g.b_sn = b_mn ? 1 : kb_n; g.b_sk = b_mn ? nb_n : 1;
-  g.c = (bf16*)s.c; g.residual = (const bf16*)s.residual; g.ldc = s.ldc; g.ldr = s.ldr;
-  g.h_exp = (const uint8_t*)s.h_exp; g.q_exp = (uint8_t*)s.q_exp;
-  g.q_ldv = up(N, 16);
-  g.q_lde = q_rows == 1 ? up(M, 16) : nb_n;
-  g.status = (int*)s.status;
-  if (epilogue <= 1) {
-    g.direct = ((uintptr_t)s.c & 15) || (s.ldc & 7) || (epilogue == 1 && (((uintptr_t)s.residual & 15) || (s.ldr & 7)));
-    if (g.direct) {
-      mo = ma;               // never read
-    } else {
-      r = encode(&mo, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, s.c, M, N, s.ldc);
-    }
-  } else {
-    r = encode(&mo, u8, 1, s.q_val, M, N, g.q_ldv);
+  const bool a_mn = s.a_mn, b_mn = s.b_mn;
+  switch (s.epilogue) {
+    case EPI_RELU_SQ:
+      if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
+      return s.q_rows == 1 ? launch<false, false, EPI_RELU_SQ, 1>(all, st) : launch<false, false, EPI_RELU_SQ, 128>(all, st);
+    case EPI_RELU_SQ_GRAD:
+      if (a_mn || !b_mn) return RWKV_ERR_BAD_SHAPE;
+      return s.q_rows == 1 ? launch<false, true, EPI_RELU_SQ_GRAD, 1>(all, st) : launch<false, true, EPI_RELU_SQ_GRAD, 128>(all, st);
+    case EPI_RESIDUAL:
+      return a_mn || b_mn ? RWKV_ERR_BAD_SHAPE : launch<false, false, EPI_RESIDUAL, 0>(all, st);
+    default:
+      if (a_mn) return b_mn ? launch<true, true, EPI_STORE, 0>(all, st) : RWKV_ERR_BAD_SHAPE;
+      return b_mn ? launch<false, true, EPI_STORE, 0>(all, st) : launch<false, false, EPI_STORE, 0>(all, st);
   }
-  if (r) return r;
-  mi = mo;
-  if (epilogue == 3) r = encode(&mi, u8, 1, s.h_val, M, N, g.q_ldv);
-  if (epilogue == 1 && !g.direct) r = encode(&mi, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, s.residual, M, N, s.ldr);
-  if (r) return r;
-  if (epilogue == 2) {
-    if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
-    return q_rows == 1 ? launch<false, false, EPI_RELU_SQ, 1>(ma, mb, mo, mi, g, st) : launch<false, false, EPI_RELU_SQ, 128>(ma, mb, mo, mi, g, st);
-  }
-  if (epilogue == 3) {
-    if (a_mn || !b_mn) return RWKV_ERR_BAD_SHAPE;
-    return q_rows == 1 ? launch<false, true, EPI_RELU_SQ_GRAD, 1>(ma, mb, mo, mi, g, st)
-                       : launch<false, true, EPI_RELU_SQ_GRAD, 128>(ma, mb, mo, mi, g, st);
-  }
-  if (epilogue == 1) {
-    if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
-    return launch<false, false, EPI_RESIDUAL, 0>(ma, mb, mo, mi, g, st);
-  }
-  if (a_mn && b_mn) return launch<true, true, EPI_STORE, 0>(ma, mb, mo, mi, g, st);
-  if (a_mn) return RWKV_ERR_BAD_SHAPE;
-  return b_mn ? launch<false, true, EPI_STORE, 0>(ma, mb, mo, mi, g, st) : launch<false, false, EPI_STORE, 0>(ma, mb, mo, mi, g, st);
+}
+
+// Two products of the kind a^T b (a_mn = b_mn = 1, epilogue 0) in one launch.
+int rwkv_fp8_gemm_two(const Fp8Step& s, const Fp8Step& t, cudaStream_t st) {
+  if (!s.a_mn || !s.b_mn || s.epilogue || !t.a_mn || !t.b_mn || t.epilogue) return RWKV_ERR_BAD_SHAPE;
+  Problems<2> all;
+  int r = describe(s, all.p[0]);
+  if (!r) r = describe(t, all.p[1]);
+  return r ? r : launch<true, true, EPI_STORE, 0, 2>(all, st);
 }

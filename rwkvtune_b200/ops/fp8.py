@@ -127,7 +127,7 @@ class _HostRun:
     def nn(self, a, b, out):
         out.copy_(_f32(a) @ _f32(b))
 
-    def tn(self, a, b, out):
+    def tn(self, a, b, out, with_next=False):
         out.copy_(_f32(a).t() @ _f32(b))
 
     def nt_frozen(self, x, w, out, hidden=None):
@@ -199,9 +199,10 @@ class _DeviceRun:
         if a.R:
             self.steps.append(native.mm_nn(a, b, out))
 
-    def tn(self, a, b, out):
+    def tn(self, a, b, out, with_next=False):
+        """``with_next``: the next step is another of these and may run in the same launch."""
         if a.R:
-            self.steps.append(native.mm_tn(a, b, out))
+            self.steps.append(native.mm_tn(a, b, out, with_next))
         else:
             out.zero_()
 
@@ -423,7 +424,7 @@ class _ChannelMix(torch.autograd.Function):
                 run.nn(p8, k8, _rows_of(dx))
             if need_k:
                 dwk = torch.empty(p8.C, x8.C, dtype=ctx.types[1], device=dev)
-                run.tn(p8, x8, dwk)
+                run.tn(p8, x8, dwk, with_next=need_v)
             if need_v:
                 dwv = torch.empty(d8.C, h8.C, dtype=ctx.types[2], device=dev)
                 run.tn(d8, h8, dwv)

@@ -41,7 +41,8 @@ def unpack(p, out: torch.Tensor) -> bytes:
                    p.exponent_address, 0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0)
 
 
-def _product(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, out=None, residual=None, h=None, q=None) -> bytes:
+def _product(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, out=None, residual=None, h=None, q=None,
+             with_next: int = 0) -> bytes:
     ph = he = pq = qe = qr = pr = ldr = 0
     if h is not None:
         ph, he = h.address, h.exponent_address
@@ -49,7 +50,7 @@ def _product(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, 
         pq, qe, qr = q.address, q.exponent_address, q.rows
     if residual is not None:
         pr, ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
-    return _record(_GEMM, M, N, K, a.rows, qr, 0, a_mn, b_mn, epilogue, 0, 0, 0, N, ldr, 0, a.address, a.exponent_address,
+    return _record(_GEMM, M, N, K, a.rows, qr, 0, a_mn, b_mn, epilogue, 0, with_next, 0, N, ldr, 0, a.address, a.exponent_address,
                    b.address, b.exponent_address, 0 if out is None else out.data_ptr(), pr, ph, he, pq, qe,
                    _status(a.data.device))
 
@@ -64,9 +65,10 @@ def mm_nn(a, b, out) -> bytes:
     return _product(a, b, a.R, b.C, a.C, 0, 1, _STORE, out)
 
 
-def mm_tn(a, b, out) -> bytes:
-    """``out [M, N] = a [K, M]^T @ b [K, N]``, both in tiles"""
-    return _product(a, b, a.C, b.C, a.R, 1, 1, _STORE, out)
+def mm_tn(a, b, out, with_next: bool = False) -> bytes:
+    """``out [M, N] = a [K, M]^T @ b [K, N]``, both in tiles; ``with_next``: in one launch with the next record, another of
+    these"""
+    return _product(a, b, a.C, b.C, a.R, 1, 1, _STORE, out, with_next=int(with_next))
 
 
 def mm_nt_relu_sq(a, b, q) -> bytes:

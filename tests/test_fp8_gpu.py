@@ -234,6 +234,24 @@ def test_long_contraction_and_many_tiles():
     near(product("tn", a, b, K, N), A.t() @ B, A.abs().t() @ B.abs(), M)
 
 
+@pytest.mark.parametrize("first,second", [((300, 520, 384), (130, 90, 1000)), ((2048, 1024, 129), (1024, 2048, 129)),
+                                          ((1, 1, 1), (4100, 2600, 700))])
+def test_two_products_in_one_launch(first, second):
+    outs, wants = [], []
+    run = None
+    for i, (M, N, K) in enumerate((first, second)):
+        a, b = ops.pack_fp8(sample(K, M, seed=i).cuda()), ops.pack_fp8(sample(K, N, seed=5 + i).cuda())
+        outs.append(torch.full((M, N), math.nan, dtype=BF, device="cuda"))
+        run = run or fp8._run_on(a.data)
+        run.tn(a, b, outs[-1], with_next=i == 0)
+        run.keep += [a, b]
+        A, B = values64(a), values64(b)
+        wants.append((A.t() @ B, A.abs().t() @ B.abs(), K))
+    run.go()
+    for out, want in zip(outs, wants):
+        near(out, *want)
+
+
 def test_non_finite_blocks_reach_exactly_their_products():
     x, w = sample(300, 256), weights(64, 256)
     x[140, 3] = math.inf
