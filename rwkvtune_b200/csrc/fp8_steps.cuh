@@ -19,6 +19,7 @@ struct Fp8Step {
   const void* residual;
   const void *h_val, *h_exp;
   void *q_val, *q_exp;
+  void* workspace;           // gemm: see gemm_fp8_tcgen05.cu
   void* status;
 };
 

@@ -50,7 +50,7 @@ constexpr int NUM_THREADS = 32 * (WARP_EPI + 4 * EPI_GROUPS);
 constexpr int TMEM_COLS = 512, ACC1_COL = 192, SF_COL = 448, SF_COLS = 16, SF_B_OFFSET = 8;
 constexpr unsigned long long WAIT_NS = 4000000000ull;
 
-enum Epilogue { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_RELU_SQ = 2, EPI_RELU_SQ_GRAD = 3 };
+enum Epilogue { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_RELU_SQ = 2, EPI_RELU_SQ_GRAD = 3, EPI_PARTIAL = 4 };
 
 struct Barriers {
   uint64_t full[STAGES];         // leader: both CTAs' operand loads have landed
@@ -89,7 +89,8 @@ struct Args {
 struct alignas(64) Problem {
   CUtensorMap a, b, out, in;
   Args g;
-  int tiles_n, tiles, num_kb, pad[1];
+  int tiles_n, tiles, num_kb;
+  int splits, kb_split, rows_split;  // EPI_PARTIAL: slices of the contraction, blocks of a slice, rows of a slice in the workspace
 };
 template <int COUNT>
 struct Problems {
@@ -284,13 +285,22 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();            // 0 = leader
   const int pair = (int)blockIdx.x >> 1, n_pairs = (int)gridDim.x >> 1;
-  const int tiles0 = all.p[0].tiles, num_tiles = tiles0 + (COUNT > 1 ? all.p[COUNT - 1].tiles : 0);
+  constexpr bool SPLIT = EPI == EPI_PARTIAL;
+  const int tiles0 = all.p[0].tiles * (SPLIT ? all.p[0].splits : 1);
+  const int num_tiles = tiles0 + (COUNT > 1 ? all.p[COUNT - 1].tiles * (SPLIT ? all.p[COUNT - 1].splits : 1) : 0);
   int* const status = all.p[0].g.status;
-  // the problem of a tile, its first row and its first column
-  const auto locate = [&](int tile, int& m0, int& n0) -> const Problem& {
+  // the problem of a tile, its first row, its first column and (split: tile = slice * tiles + tile) its blocks of the contraction
+  const auto locate = [&](int tile, int& m0, int& n0, int& kb0, int& num_kb) -> const Problem& {
     const bool second = COUNT > 1 && tile >= tiles0;
     const Problem& p = second ? all.p[COUNT - 1] : all.p[0];
     if (second) tile -= tiles0;
+    kb0 = 0;
+    num_kb = p.num_kb;
+    if (SPLIT) {
+      kb0 = tile / p.tiles * p.kb_split;
+      num_kb = min(p.kb_split, p.num_kb - kb0);
+      tile %= p.tiles;
+    }
     m0 = (tile / p.tiles_n) * (2 * TM) + (int)rank * TM;
     n0 = (tile % p.tiles_n) * TN;
     return p;
@@ -323,16 +333,15 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += n_pairs) {
-        int m0, n0;
-        const Problem& p = locate(tile, m0, n0);
+        int m0, n0, kb0, num_kb;
+        const Problem& p = locate(tile, m0, n0, kb0, num_kb);
         n0 += (int)rank * 128;
-        const int num_kb = p.num_kb;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&bars->empty[stage], phase ^ 1, bars, status, 211)) { ok = false; break; }
           if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * STAGE_BYTES);
           const uint32_t full_leader = map_to_cta(smem_u32(&bars->full[stage]), 0);
           const uint32_t sa = base + stage * STAGE_BYTES, sb = sa + OP_BYTES;
-          const int k0 = kb * TK;
+          const int k0 = (kb0 + kb) * TK;
           tma_load_2d_pair(sa, &p.a, full_leader, A_MN ? m0 : k0, A_MN ? k0 : m0);
           tma_load_2d_pair(sb, &p.b, full_leader, B_MN ? n0 : k0, B_MN ? k0 : n0);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -351,7 +360,8 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += n_pairs, ++local) {
         const uint32_t d_tmem = tmem_base + (local & 1) * ACC1_COL;
-        const int num_kb = COUNT > 1 && tile >= tiles0 ? all.p[COUNT - 1].num_kb : all.p[0].num_kb;
+        int m0, n0, kb0, num_kb;
+        locate(tile, m0, n0, kb0, num_kb);
         for (int kb = 0; kb < num_kb; ++kb) {
           const uint32_t sfa = tmem_base + SF_COL + sf * SF_COLS, sfb = sfa + SF_B_OFFSET;
           const uint32_t id = kb % SF_GROUP;
@@ -395,13 +405,12 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
     uint32_t sf_phase = 0;
     // lanes 0-3: A, 4-7 and 8-11: the two column blocks of B; blocks of one row: four rows a lane
     auto fetch = [&](int tile, int set, uint32_t& byte, uint32_t (&rows4)[4]) {
-      int m0, n0;
-      const Problem& p = locate(tile, m0, n0);
+      int m0, n0, kb0, num_kb;
+      const Problem& p = locate(tile, m0, n0, kb0, num_kb);
       const Args& g = p.g;
-      const int num_kb = p.num_kb;
-      const int which = lane >> 2, kb = set * SF_GROUP + (lane & 3);
+      const int which = lane >> 2, kb = kb0 + set * SF_GROUP + (lane & 3);
       byte = 0;
-      if (kb < num_kb) {
+      if (kb < kb0 + num_kb) {
         if (which == 0 && !by_row && m0 < g.M) byte = __ldg(g.a_exp + (long long)(m0 >> 7) * g.a_sm + (long long)kb * g.a_sk);
         if ((which == 1 || which == 2) && n0 + (which - 1) * 128 < g.N)
           byte = __ldg(g.b_exp + (long long)((n0 >> 7) + which - 1) * g.b_sn + (long long)kb * g.b_sk);
@@ -410,7 +419,7 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
       for (int i = 0; i < 4; ++i) {
         rows4[i] = 0;
         if (by_row && set * SF_GROUP + i < num_kb && m0 + 4 * lane < g.a_ld)
-          rows4[i] = __ldg(reinterpret_cast<const uint32_t*>(g.a_exp + (long long)(set * SF_GROUP + i) * g.a_ld + m0 + 4 * lane));
+          rows4[i] = __ldg(reinterpret_cast<const uint32_t*>(g.a_exp + (long long)(kb0 + set * SF_GROUP + i) * g.a_ld + m0 + 4 * lane));
       }
       return (num_kb + SF_GROUP - 1) / SF_GROUP;
     };
@@ -458,8 +467,8 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
     const uint32_t free_leader = map_to_cta(smem_u32(&bars->acc_free), 0);
     int local = 0;
     for (int tile = pair; tile < num_tiles; tile += n_pairs, ++local) {
-      int m0, gn0;
-      const Problem& p = locate(tile, m0, gn0);
+      int m0, gn0, kb0, num_kb;
+      const Problem& p = locate(tile, m0, gn0, kb0, num_kb);
       gn0 += group * 128;
       const Args& g = p.g;
       const int M = g.M, N = g.N;
@@ -531,6 +540,37 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
                              : "memory");
                 if (c0 + col < N) reinterpret_cast<uint16_t*>(g.c)[(long long)(m0 + r) * g.ldc + c0 + col] = val;
               }
+          }
+        }
+      } else if constexpr (EPI == EPI_PARTIAL) {      // fp32 rows of this slice, 32 columns at a time
+        const int out_row = kb0 / p.kb_split * p.rows_split + m0;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int chunk = acc == 0 ? 1 - i : i;      // the columns shared with the other accumulator first
+          uint32_t v[64];
+          tmem_ld32(t_row + chunk * 64, v);
+          tmem_ld32(t_row + chunk * 64 + 32, v + 32);
+          tmem_wait_ld(v);
+          if (i == 0 && shared_columns) {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_at(free_leader);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c0 = gn0 + chunk * 64 + h * 32;
+            if (elected) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            epi_sync(group);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t* w = v + h * 32 + j * 4;
+              st_shared16(stage_addr + row * 128 + ((j ^ (row & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            epi_sync(group);
+            if (elected && m0 < M && c0 < N) {
+              tma_store_2d(&p.out, stage_addr, c0, out_row);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
           }
         }
       } else {
@@ -665,7 +705,7 @@ int launch(const Problems<COUNT>& all, cudaStream_t st) {
     configured.fetch_or(bit);
   }
   long long tiles = 0;
-  for (int i = 0; i < COUNT; ++i) tiles += all.p[i].tiles;
+  for (int i = 0; i < COUNT; ++i) tiles += (long long)all.p[i].tiles * all.p[i].splits;
   const int pairs = tiles < sms / 2 ? (int)tiles : sms / 2;
   kern<<<2 * pairs, NUM_THREADS, SMEM_BYTES, st>>>(all);
   return rwkv_launch_status();
@@ -673,7 +713,59 @@ int launch(const Problems<COUNT>& all, cudaStream_t st) {
 
 inline int up(int n, int m) { return (n + m - 1) / m * m; }
 
-// Checks a record and fills in a problem.
+// Slices of the contraction: few tiles and a long contraction leave most SM pairs idle, so the contraction is cut into
+// slices of at least eight blocks whose fp32 sums a second kernel adds in a fixed order.  A block takes 0.3 us, the second
+// kernel and its traffic 4 to 6: slices are used where they save a tile 24 blocks or more, on at most half the pairs
+// (M x N x K, in one piece and in slices: 222 x 64 x 23302 61.7 and 12.7 us, 1024 x 1024 x 32768 78.1 and 35.2,
+// 2304 x 1024 x 8192 25.3 and 22.9; below the rule 2048 x 1024 x 4096 16.0 and 17.2, 512 x 2048 x 2048 10.6 and 13.1).
+int splits_for(int M, int N, int K) {
+  const long long tiles = (long long)(up(M, 2 * TM) / (2 * TM)) * (up(N, TN) / TN);
+  const int kb = up(K, TK) / TK;
+  if (tiles > 37 || kb < 32) return 1;
+  const int s = (int)(74 / tiles) < kb / 8 ? (int)(74 / tiles) : kb / 8;
+  const int per = up((kb + s - 1) / s, SF_GROUP);            // whole sets of scales
+  return kb - per >= 24 ? (kb + per - 1) / per : 1;
+}
+inline int kb_of_slice(int K, int splits) { return up((up(K, TK) / TK + splits - 1) / splits, SF_GROUP); }
+
+// c = (residual +) the sum of the slices' rows
+__global__ void __launch_bounds__(256)
+fp8_sum_slices_kernel(const float* __restrict__ ws, int splits, long long slice, int ldw, int M, int N, const bf16* __restrict__ residual,
+                      long long ldr, bf16* __restrict__ c, long long ldc, int vec) {
+  const int quads = (N + 3) / 4;
+  const long long total = (long long)M * quads;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* p = ws + (long long)m * ldw + n;
+    for (int s = 0; s < splits; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(p + s * slice);
+      f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+    }
+    if (vec) {
+      if (residual) {
+        const uint2 r = *reinterpret_cast<const uint2*>(residual + m * ldr + n);
+        f[0] += bf16_lo(r.x); f[1] += bf16_hi(r.x); f[2] += bf16_lo(r.y); f[3] += bf16_hi(r.y);
+      }
+      *reinterpret_cast<uint2*>(c + m * ldc + n) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < N) c[m * ldc + n + e] = __float2bfloat16_rn(f[e] + (residual ? __bfloat162float(residual[m * ldr + n + e]) : 0.f));
+    }
+  }
+}
+int sum_slices(const Fp8Step& s, int splits, cudaStream_t st) {
+  const int ldw = up(s.N, 4);
+  const long long total = (long long)s.M * ((s.N + 3) / 4), ctas = (total + 255) / 256;
+  const int vec = !(s.N % 4) && !((uintptr_t)s.c & 7) && !(s.ldc % 4) && !((uintptr_t)s.residual & 7) && !(s.ldr % 4);
+  fp8_sum_slices_kernel<<<(int)(ctas < 148 * 16 ? ctas : 148 * 16), 256, 0, st>>>(
+      (const float*)s.workspace, splits, (long long)up(s.M, TM) * ldw, ldw, s.M, s.N, (const bf16*)s.residual, s.ldr, (bf16*)s.c,
+      s.ldc, vec);
+  return rwkv_launch_status();
+}
+
+// Checks a record and fills in a problem; with a workspace the result goes there in slices.
 int describe(const Fp8Step& s, Problem& p) {
   const int M = s.M, N = s.N, K = s.K, a_mn = s.a_mn, b_mn = s.b_mn, epilogue = s.epilogue, q_rows = s.q_rows;
   if (M <= 0 || N <= 0 || K <= 0 || M > 0x7ffffe00 || N > 0x7ffffe00 || K > 0x7ffffe00) return RWKV_ERR_BAD_SHAPE;
@@ -705,7 +797,12 @@ int describe(const Fp8Step& s, Problem& p) {
   g.q_lde = q_rows == 1 ? up(M, 16) : nb_n;
   g.status = (int*)s.status;
   p.out = p.in = p.a;                  // maps that the epilogue does not use are never read
-  if (epilogue <= 1) {
+  p.splits = 1; p.kb_split = kb_n; p.rows_split = up(M, TM);
+  if (epilogue <= 1 && s.workspace) {
+    p.splits = splits_for(M, N, K);
+    p.kb_split = kb_of_slice(K, p.splits);
+    r = encode(&p.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, s.workspace, (long long)p.splits * p.rows_split, N, up(N, 4));
+  } else if (epilogue <= 1) {
     g.direct = ((uintptr_t)s.c & 15) || (s.ldc & 7) || (epilogue == 1 && (((uintptr_t)s.residual & 15) || (s.ldr & 7)));
     if (!g.direct) r = encode(&p.out, b16, 2, s.c, M, N, s.ldc);
     if (!r && epilogue == 1 && !g.direct) r = encode(&p.in, b16, 2, s.residual, M, N, s.ldr);
@@ -724,12 +821,19 @@ int describe(const Fp8Step& s, Problem& p) {
 //   epilogue 0: c = bf16 result (row stride ldc);  1: c = result + residual (bf16, row stride ldr), NT only;
 //            2: (q_val, q_exp) = packed relu(result)^2, NT only;  3: = packed result * 2 sqrt(h), NN only;
 //            the packed result and h are [M,N] with blocks of q_rows rows
+//   workspace (epilogues 0 and 1): rwkv_fp8_workspace(M, N, K) bytes, the contraction runs in slices; null: it does not
 //   status: device int, set non-zero if a device-side wait expired
 int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t st) {
   Problems<1> all;
-  const int r = describe(s, all.p[0]);
+  int r = describe(s, all.p[0]);
   if (r) return r;
   const bool a_mn = s.a_mn, b_mn = s.b_mn;
+  if (s.workspace && s.epilogue <= 1) {
+    if (a_mn && !b_mn) return RWKV_ERR_BAD_SHAPE;
+    r = a_mn ? launch<true, true, EPI_PARTIAL, 0>(all, st)
+             : b_mn ? launch<false, true, EPI_PARTIAL, 0>(all, st) : launch<false, false, EPI_PARTIAL, 0>(all, st);
+    return r ? r : sum_slices(s, all.p[0].splits, st);
+  }
   switch (s.epilogue) {
     case EPI_RELU_SQ:
       if (a_mn || b_mn) return RWKV_ERR_BAD_SHAPE;
@@ -751,5 +855,16 @@ int rwkv_fp8_gemm_two(const Fp8Step& s, const Fp8Step& t, cudaStream_t st) {
   Problems<2> all;
   int r = describe(s, all.p[0]);
   if (!r) r = describe(t, all.p[1]);
-  return r ? r : launch<true, true, EPI_STORE, 0, 2>(all, st);
+  if (r || !s.workspace != !t.workspace) return r ? r : RWKV_ERR_BAD_SHAPE;
+  if (!s.workspace) return launch<true, true, EPI_STORE, 0, 2>(all, st);
+  r = launch<true, true, EPI_PARTIAL, 0, 2>(all, st);
+  if (!r) r = sum_slices(s, all.p[0].splits, st);
+  return r ? r : sum_slices(t, all.p[1].splits, st);
+}
+
+// Bytes of workspace that a product wants (0: none).  Depends on sizes only.
+RWKV_EXPORT long long rwkv_fp8_workspace(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || M > 0x7ffffe00 || N > 0x7ffffe00 || K > 0x7ffffe00) return 0;
+  const int splits = splits_for(M, N, K);
+  return splits > 1 ? (long long)splits * up(M, TM) * up(N, 4) * 4 : 0;
 }

@@ -127,8 +127,12 @@ class _HostRun:
     def nn(self, a, b, out):
         out.copy_(_f32(a) @ _f32(b))
 
-    def tn(self, a, b, out, with_next=False):
+    def tn(self, a, b, out):
         out.copy_(_f32(a).t() @ _f32(b))
+
+    def tn_two(self, a, b, out, c, d, out2):
+        self.tn(a, b, out)
+        self.tn(c, d, out2)
 
     def nt_frozen(self, x, w, out, hidden=None):
         x8 = _matrix(x.device, *x.shape, 1)
@@ -172,7 +176,9 @@ class _DeviceRun:
             # its predecessor is the step that packed `a`, which does not write the weights
             self.steps.append(native.decode(a, b, out, residual, chained=bool(self.steps)))
         else:
-            self.steps.append(native.mm_nt(a, b, out, residual))
+            ws = native.workspace(a.R, b.R, a.C, self.device)
+            self.steps.append(native.mm_nt(a, b, out, residual, ws))
+            self.keep.append(ws)
         self.keep.append(residual)
 
     def nt_frozen(self, x, w, out, hidden=None):
@@ -197,14 +203,28 @@ class _DeviceRun:
 
     def nn(self, a, b, out):
         if a.R:
-            self.steps.append(native.mm_nn(a, b, out))
+            ws = native.workspace(a.R, b.C, a.C, self.device)
+            self.steps.append(native.mm_nn(a, b, out, ws))
+            self.keep.append(ws)
 
-    def tn(self, a, b, out, with_next=False):
-        """``with_next``: the next step is another of these and may run in the same launch."""
+    def tn(self, a, b, out):
         if a.R:
-            self.steps.append(native.mm_tn(a, b, out, with_next))
+            ws = native.workspace(a.C, b.C, a.R, self.device)
+            self.steps.append(native.mm_tn(a, b, out, ws=ws))
+            self.keep.append(ws)
         else:
             out.zero_()
+
+    def tn_two(self, a, b, out, c, d, out2):
+        """``out = a^T b`` and ``out2 = c^T d`` in one launch, where both contractions run in one piece or both in slices."""
+        sizes = (a.C, b.C, a.R), (c.C, d.C, c.R)
+        ws = [native.workspace(*s, self.device) for s in sizes]
+        if not a.R or not c.R or (ws[0] is None) != (ws[1] is None):
+            self.tn(a, b, out)
+            self.tn(c, d, out2)
+            return
+        self.steps += [native.mm_tn(a, b, out, True, ws[0]), native.mm_tn(c, d, out2, ws=ws[1])]
+        self.keep += ws
 
     def nt_relu_sq(self, a, b, q):
         if a.R:
@@ -424,9 +444,13 @@ class _ChannelMix(torch.autograd.Function):
                 run.nn(p8, k8, _rows_of(dx))
             if need_k:
                 dwk = torch.empty(p8.C, x8.C, dtype=ctx.types[1], device=dev)
-                run.tn(p8, x8, dwk, with_next=need_v)
             if need_v:
                 dwv = torch.empty(d8.C, h8.C, dtype=ctx.types[2], device=dev)
+            if need_k and need_v:
+                run.tn_two(p8, x8, dwk, d8, h8, dwv)
+            elif need_k:
+                run.tn(p8, x8, dwk)
+            elif need_v:
                 run.tn(d8, h8, dwv)
             run.go()
         return dx, dwk, dwv, (dy if need_r else None)

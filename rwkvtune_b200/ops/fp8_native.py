@@ -18,7 +18,7 @@ from . import _ext, gemm_native
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _PACK, _UNPACK, _GEMM, _DECODE = 0, 1, 2, 3
 _STORE, _RESIDUAL, _RELU_SQ, _RELU_SQ_GRAD = 0, 1, 2, 3
-_record = struct.Struct("=12i3q12Q").pack      # Fp8Step, field by field
+_record = struct.Struct("=12i3q13Q").pack      # Fp8Step, field by field
 _launch = None                                 # rwkv_fp8_run, bound at the first call
 _status_address = {}
 
@@ -33,16 +33,16 @@ def _status(device: torch.device) -> int:
 def pack(x: torch.Tensor, q) -> bytes:
     """``x [R, C]`` with unit inner stride -> ``q``."""
     return _record(_PACK, q.R, q.C, 0, 0, q.rows, _DTYPES[x.dtype], 0, 0, 0, 0, 0, x.stride(0) if q.R > 1 else q.C, 0, 0,
-                   x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, q.address, q.exponent_address, 0)
+                   x.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, q.address, q.exponent_address, 0, 0)
 
 
 def unpack(p, out: torch.Tensor) -> bytes:
     return _record(_UNPACK, p.R, p.C, 0, p.rows, 0, _DTYPES[out.dtype], 0, 0, 0, 0, 0, 0, p.C, 0, 0, p.address,
-                   p.exponent_address, 0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0)
+                   p.exponent_address, 0, 0, out.data_ptr(), 0, 0, 0, 0, 0, 0, 0)
 
 
 def _product(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, out=None, residual=None, h=None, q=None,
-             with_next: int = 0) -> bytes:
+             with_next: int = 0, workspace=None) -> bytes:
     ph = he = pq = qe = qr = pr = ldr = 0
     if h is not None:
         ph, he = h.address, h.exponent_address
@@ -52,23 +52,36 @@ def _product(a, b, M: int, N: int, K: int, a_mn: int, b_mn: int, epilogue: int, 
         pr, ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
     return _record(_GEMM, M, N, K, a.rows, qr, 0, a_mn, b_mn, epilogue, 0, with_next, 0, N, ldr, 0, a.address, a.exponent_address,
                    b.address, b.exponent_address, 0 if out is None else out.data_ptr(), pr, ph, he, pq, qe,
-                   _status(a.data.device))
+                   0 if workspace is None else workspace.data_ptr(), _status(a.data.device))
 
 
-def mm_nt(a, b, out, residual=None) -> bytes:
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(M: int, N: int, K: int) -> int:
+    fn = _ext.lib().rwkv_fp8_workspace
+    fn.restype = ctypes.c_longlong
+    return fn(M, N, K)
+
+
+def workspace(M: int, N: int, K: int, device):
+    """Room for the slices of a product of few tiles and a long contraction; ``None`` if it runs in one piece."""
+    n = _workspace_bytes(M, N, K)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def mm_nt(a, b, out, residual=None, ws=None) -> bytes:
     """``out [M, N] = a [M, K] @ b [N, K]^T (+ residual)``"""
-    return _product(a, b, a.R, b.R, a.C, 0, 0, _STORE if residual is None else _RESIDUAL, out, residual)
+    return _product(a, b, a.R, b.R, a.C, 0, 0, _STORE if residual is None else _RESIDUAL, out, residual, workspace=ws)
 
 
-def mm_nn(a, b, out) -> bytes:
+def mm_nn(a, b, out, ws=None) -> bytes:
     """``out [M, N] = a [M, K] @ b [K, N]``"""
-    return _product(a, b, a.R, b.C, a.C, 0, 1, _STORE, out)
+    return _product(a, b, a.R, b.C, a.C, 0, 1, _STORE, out, workspace=ws)
 
 
-def mm_tn(a, b, out, with_next: bool = False) -> bytes:
+def mm_tn(a, b, out, with_next: bool = False, ws=None) -> bytes:
     """``out [M, N] = a [K, M]^T @ b [K, N]``, both in tiles; ``with_next``: in one launch with the next record, another of
-    these"""
-    return _product(a, b, a.C, b.C, a.R, 1, 1, _STORE, out, with_next=int(with_next))
+    these (both with a workspace or neither)"""
+    return _product(a, b, a.C, b.C, a.R, 1, 1, _STORE, out, with_next=int(with_next), workspace=ws)
 
 
 def mm_nt_relu_sq(a, b, q) -> bytes:
@@ -111,7 +124,7 @@ def decode(x, b, out=None, residual=None, q=None, chained: bool = False) -> byte
         if residual is not None:
             epilogue, pr, ldr = _RESIDUAL, residual.data_ptr(), residual.stride(0) if M > 1 else N
     return _record(_DECODE, M, N, K, 1, 1, 0, 0, 0, epilogue, chained, 0, ldx, N, ldr, px, pa, ae, b.address,
-                   b.exponent_address, po, pr, 0, 0, pq, qe, _status(b.data.device))
+                   b.exponent_address, po, pr, 0, 0, pq, qe, 0, _status(b.data.device))
 
 
 def run(device: torch.device, steps) -> None:

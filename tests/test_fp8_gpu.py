@@ -235,21 +235,40 @@ def test_long_contraction_and_many_tiles():
 
 
 @pytest.mark.parametrize("first,second", [((300, 520, 384), (130, 90, 1000)), ((2048, 1024, 129), (1024, 2048, 129)),
-                                          ((1, 1, 1), (4100, 2600, 700))])
+                                          ((1, 1, 1), (4100, 2600, 700)), ((200, 300, 6000), (130, 523, 2500)), ((200, 300, 6000), (130, 523, 5000)),
+                                          ((300, 300, 4000), (4100, 2600, 700))])
 def test_two_products_in_one_launch(first, second):
-    outs, wants = [], []
-    run = None
+    args, wants = [], []
     for i, (M, N, K) in enumerate((first, second)):
         a, b = ops.pack_fp8(sample(K, M, seed=i).cuda()), ops.pack_fp8(sample(K, N, seed=5 + i).cuda())
-        outs.append(torch.full((M, N), math.nan, dtype=BF, device="cuda"))
-        run = run or fp8._run_on(a.data)
-        run.tn(a, b, outs[-1], with_next=i == 0)
-        run.keep += [a, b]
+        args += [a, b, torch.full((M, N), math.nan, dtype=BF, device="cuda")]
         A, B = values64(a), values64(b)
         wants.append((A.t() @ B, A.abs().t() @ B.abs(), K))
+    run = fp8._run_on(args[2])
+    run.tn_two(*args)
     run.go()
-    for out, want in zip(outs, wants):
+    for out, want in zip(args[2::3], wants):
         near(out, *want)
+
+
+@pytest.mark.parametrize("M,N,K", [(130, 200, 5000), (257, 523, 8200), (300, 64, 33000), (1000, 1024, 8192), (129, 40, 5050)])
+def test_few_tiles_and_a_long_contraction(M, N, K):
+    """Products whose contraction runs in slices, in all three layouts, with a residual and with rows that are not aligned."""
+    from rwkvtune_b200.ops import fp8_native as native
+
+    assert native._workspace_bytes(M, N, K) > 0
+    res = sample(M, N, seed=7).cuda()
+    for rows in (1, 128):
+        a, b = ops.pack_fp8(sample(M, K).cuda(), rows=rows), ops.pack_fp8(weights(N, K).cuda())
+        A, B = values64(a), values64(b)
+        near(product("nt", a, b, M, N), A @ B.t(), A.abs() @ B.abs().t(), K)
+        near(product("nt", a, b, M, N, res), res.double() + A @ B.t(), A.abs() @ B.abs().t() + res.double().abs(), K)
+        b = ops.pack_fp8(weights(K, N).cuda())
+        B = values64(b)
+        near(product("nn", a, b, M, N), A @ B, A.abs() @ B.abs(), K)
+    a, b = ops.pack_fp8(sample(K, M).cuda()), ops.pack_fp8(sample(K, N, seed=5).cuda())
+    A, B = values64(a), values64(b)
+    near(product("tn", a, b, M, N), A.t() @ B, A.abs().t() @ B.abs(), K)
 
 
 def test_non_finite_blocks_reach_exactly_their_products():
