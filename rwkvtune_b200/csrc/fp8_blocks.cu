@@ -189,7 +189,7 @@ constexpr int TILE_THREADS = 512;
 
 // A CTA walks over tiles and has the next one in flight while it works on the present one.
 template <typename T, int V>
-__global__ void __launch_bounds__(TILE_THREADS, 2)
+__global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 4 ? 1 : 2)
 fp8_pack_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
                       int R, int C, int ldv, uint32_t tiles, uint32_t blocks) {
   rwkv_chain_trigger();
@@ -290,7 +290,7 @@ int pack_v(const T* x, long long ld, uint8_t* values, uint8_t* exps, int R, int 
                                                                             up(R, 16), blocks);
     } else {
       const uint32_t tiles = (uint32_t)((n + FP8_BLOCK - 1) / FP8_BLOCK) * blocks;
-      fp8_pack_tiles_kernel<T, V><<<grid_for(tiles, 2), TILE_THREADS, 0, st>>>(
+      fp8_pack_tiles_kernel<T, V><<<grid_for(tiles, sizeof(T) == 4 ? 1 : 2), TILE_THREADS, 0, st>>>(
           src, ld, dst, exps + (long long)(r0 / FP8_BLOCK) * blocks, n, C, ldv, tiles, blocks);
     }
   }

@@ -301,8 +301,12 @@ gemm_fp8_kernel(const __grid_constant__ Problems<COUNT> all) {
       num_kb = min(p.kb_split, p.num_kb - kb0);
       tile %= p.tiles;
     }
-    m0 = (tile / p.tiles_n) * (2 * TM) + (int)rank * TM;
-    n0 = (tile % p.tiles_n) * TN;
+    // eight rows of tiles at a time, column by column: what runs at once shares its operands in L2 (2902 -> 2870 us for a
+    // feed-forward half of 32768 x 2048 under the power cap)
+    const int band = tile / (8 * p.tiles_n), rest = tile - band * (8 * p.tiles_n);
+    const int height = min(8, p.tiles / p.tiles_n - band * 8);
+    m0 = (band * 8 + rest % height) * (2 * TM) + (int)rank * TM;
+    n0 = rest / height * TN;
     return p;
   };
 
