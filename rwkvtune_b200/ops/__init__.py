@@ -32,6 +32,7 @@ _KERNELS: Dict[str, bool] = {
     "linear_logprob_entropy": True,
     "gemm": True,
     "gather": True,
+    "fp8": True,
 }
 
 

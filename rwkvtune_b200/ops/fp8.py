@@ -27,6 +27,7 @@ from typing import Optional, Union
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import _KERNELS
 from . import fp8_native as native
 from . import reference
 
@@ -240,7 +241,7 @@ class _DeviceRun:
 
 
 def _run_on(t: torch.Tensor):
-    return (_DeviceRun if t.is_cuda else _HostRun)(t.device)
+    return (_DeviceRun if t.is_cuda and _KERNELS["fp8"] else _HostRun)(t.device)
 
 
 def _f32(p: Fp8Blocks) -> torch.Tensor:

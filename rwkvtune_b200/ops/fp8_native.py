@@ -24,8 +24,12 @@ _status_address = {}
 
 
 def _status(device: torch.device) -> int:
+    """Address of the device's status word; null (no record is kept) if the first call of all is being captured into a
+    graph, whose memory the word must not live in."""
     at = _status_address.get(device.index)
     if at is None:
+        if device.index not in gemm_native._STATUS and torch.cuda.is_current_stream_capturing():
+            return 0
         at = _status_address[device.index] = gemm_native._status(device).data_ptr()
     return at
 

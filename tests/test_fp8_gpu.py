@@ -371,6 +371,114 @@ def test_captured_and_replayed():
             assert torch.equal(out, ops.fp8_channel_mix_ffn(x, k8, v8, res))
 
 
+def test_powers_of_two_pass_through():
+    """Scales are powers of two: moving one from an operand to the other changes no bit, however far."""
+    x, w = sample(200, 384).cuda(), weights(264, 384).cuda()
+    for frozen in (False, True):
+        hold = ops.pack_fp8 if frozen else (lambda t: t)
+        want = ops.fp8_linear(x, hold(w))
+        for e in (-90, -40, 40, 90):
+            assert torch.equal(ops.fp8_linear(x * 2.0 ** e, hold(w * 2.0 ** -e)), want)
+        assert torch.equal(ops.fp8_linear(x[:5] * 2.0 ** 80, hold(w * 2.0 ** -80)), ops.fp8_linear(x[:5], hold(w)))
+
+
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_strided_residuals_and_weights(M):
+    base, x = sample(M, 700, seed=3).cuda(), sample(M, 256).cuda()
+    wk, wv = weights(512, 256).cuda(), weights(256, 512, 2).cuda()
+    args = ((wk, wv), (ops.pack_fp8(wk), ops.pack_fp8(wv)))
+    for res in (base[:, 1:257], base[:, 8:264], base[:, ::2][:, :256], base[:1, :256].expand(M, 256), base.view(-1)[5:5 + M * 256].view(M, 256)):
+        for a in args:
+            assert torch.equal(ops.fp8_channel_mix_ffn(x, *a, res), ops.fp8_channel_mix_ffn(x, *a, res.contiguous().clone()))
+    assert torch.equal(ops.fp8_linear(x, wk.t().contiguous().t()), ops.fp8_linear(x, wk))
+    assert torch.equal(ops.fp8_linear(x.t().contiguous().t(), wk), ops.fp8_linear(x, wk))
+
+
+def test_offsets_beyond_32_bits():
+    R, C = 1_100_000, 2048                                    # 2.25 G values
+    x = torch.zeros(R, C, dtype=BF, device="cuda")
+    tail = sample(300, C).cuda()
+    x[-300:], x[:300] = tail, tail
+    w8 = ops.pack_fp8(weights(72, C).cuda())
+    for rows in (1, 128):
+        p = ops.pack_fp8(x, rows=rows)
+        y = ops.unpack_fp8(p)
+        off = R % 128 if rows == 128 else 0                   # the last tile is short: compare whole tiles
+        want = ops.unpack_fp8(ops.pack_fp8(x[R - 300 - off - (R - 300 - off) % rows:], rows=rows))
+        assert torch.equal(y[-300:], want[-300:]) and torch.equal(y[:256], ops.unpack_fp8(ops.pack_fp8(tail, rows=rows))[:256])
+        del y, want
+        out = product("nt", p, w8, R, 72)
+        W = values64(w8)
+        tail_values = ops.unpack_fp8(ops.pack_fp8(x[R - 300 - off - (R - 300 - off) % rows:], rows=rows), torch.float32).double()[-300:]
+        near(out[-300:], tail_values @ W.t(), tail_values.abs() @ W.abs().t(), C)
+        assert not out[300 + 128:1000].any()
+        del out, p
+
+
+def test_two_threads_at_once():
+    import threading
+
+    x, w = sample(150, 256).cuda(), weights(200, 256).cuda()
+    w8 = ops.pack_fp8(w)
+    want, errors = (ops.fp8_linear(x, w), ops.fp8_linear(x[:9], w8)), []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got = ops.fp8_linear(x, w), ops.fp8_linear(x[:9], w8)
+                    torch.cuda.current_stream().synchronize()
+                    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        except Exception as exc:       # noqa: BLE001 - reported by the main thread
+            errors.append(exc)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+
+
+def test_plain_statement_on_the_gpu():
+    """The family can be switched off like the others: the same operators in plain PyTorch."""
+    x, w = sample(140, 256).cuda(), weights(96, 256).cuda()
+    y, p = ops.fp8_linear(x, w), ops.pack_fp8(x)
+    ops.set_kernel_enabled("fp8", False)
+    try:
+        plain, q = ops.fp8_linear(x, w), ops.pack_fp8(x)
+    finally:
+        ops.set_kernel_enabled("fp8", True)
+    assert torch.equal(p.exponents, q.exponents) and torch.equal(ops.unpack_fp8(p), ops.unpack_fp8(q))
+    X, W = values64(p), values64(ops.pack_fp8(w))
+    near(plain, X @ W.t(), X.abs() @ W.abs().t(), 256)
+    near(y, X @ W.t(), X.abs() @ W.abs().t(), 256)
+
+
+def test_backward_captured_and_replayed():
+    """A training pass as one graph: the replay follows the inputs, and leaves its own results alone."""
+    x, w = torch.zeros(150, 256, dtype=BF, device="cuda").requires_grad_(), weights(200, 256).cuda().requires_grad_()
+    dy = torch.zeros(150, 200, dtype=BF, device="cuda")
+
+    def run():
+        y = ops.fp8_linear(x, w)
+        return (y.detach(), *torch.autograd.grad(y, [x, w], dy))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    for seed in (1, 2):
+        with torch.no_grad():
+            x.copy_(sample(150, 256, seed=seed)), dy.copy_(sample(150, 200, seed=seed + 5))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [o.clone() for o in outs]
+        assert all(torch.equal(a, b) for a, b in zip(kept, run()))
+
+
 def test_broadcast_gradients():
     x, w = sample(140, 128).cuda().requires_grad_(), weights(96, 128).cuda().requires_grad_()
     ops.fp8_linear(x, w).sum().backward()
