@@ -8,6 +8,8 @@
 //   rows = 128: a CTA of 512 threads walks over tiles with the next one's loads in flight; warp maxima meet in shared
 //               memory (one CTA a tile: 43.2 us, walking: 33.3 us, 6.06 TB/s).
 //
+// Launched through rwkv_launch: inside a chain of decode launches they are part of it.
+//
 // Arithmetic in the rest of the library flushes numbers below 2^-126 to zero, and so do these kernels.
 #include <cuda_fp16.h>
 
@@ -156,7 +158,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(ROW_THREADS)
 fp8_pack_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
                      uint32_t units, int C, int ldv, int lde, uint32_t blocks) {
-  rwkv_chain_trigger();       // a chained decode product may fetch its weights meanwhile
+  rwkv_chain_begin();         // a chained decode product may fetch its weights meanwhile
   const int part = threadIdx.x & 7;
   const uint32_t step = gridDim.x * (ROW_THREADS / 8);
   Raw16<T> next;
@@ -192,7 +194,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 4 ? 1 : 2)
 fp8_pack_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
                       int R, int C, int ldv, uint32_t tiles, uint32_t blocks) {
-  rwkv_chain_trigger();
+  rwkv_chain_begin();
   __shared__ uint32_t warp_max[2][TILE_THREADS / 32];
   Raw16<T> next[2];
   auto fetch = [&](uint32_t tile) {
@@ -236,6 +238,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(ROW_THREADS)
 fp8_unpack_kernel(const uint8_t* __restrict__ values, const uint8_t* __restrict__ exps, T* __restrict__ y, long long ldy,
                   uint32_t units, int C, int ldv, int lde, int rows, uint32_t blocks) {
+  rwkv_chain_begin();
   const int part = threadIdx.x & 7;
   for (uint32_t u = blockIdx.x * (ROW_THREADS / 8) + (threadIdx.x >> 3); u < units; u += gridDim.x * (ROW_THREADS / 8)) {
     const uint32_t row = u / blocks, kb = u - row * blocks;
@@ -286,12 +289,12 @@ int pack_v(const T* x, long long ld, uint8_t* values, uint8_t* exps, int R, int 
     uint8_t* dst = values + (long long)r0 * ldv;
     if (rows == 1) {
       const long long ctas = ((long long)n * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
-      fp8_pack_rows_kernel<T, V><<<grid_for(ctas, 16), ROW_THREADS, 0, st>>>(src, ld, dst, exps + r0, (uint32_t)n * blocks, C, ldv,
-                                                                            up(R, 16), blocks);
+      rwkv_launch(fp8_pack_rows_kernel<T, V>, dim3(grid_for(ctas, 16)), dim3(ROW_THREADS), 0, st, src, ld, dst, exps + r0,
+                  (uint32_t)n * blocks, C, ldv, up(R, 16), (uint32_t)blocks);
     } else {
       const uint32_t tiles = (uint32_t)((n + FP8_BLOCK - 1) / FP8_BLOCK) * blocks;
-      fp8_pack_tiles_kernel<T, V><<<grid_for(tiles, sizeof(T) == 4 ? 1 : 2), TILE_THREADS, 0, st>>>(
-          src, ld, dst, exps + (long long)(r0 / FP8_BLOCK) * blocks, n, C, ldv, tiles, blocks);
+      rwkv_launch(fp8_pack_tiles_kernel<T, V>, dim3(grid_for(tiles, sizeof(T) == 4 ? 1 : 2)), dim3(TILE_THREADS), 0, st, src, ld,
+                  dst, exps + (long long)(r0 / FP8_BLOCK) * blocks, n, C, ldv, tiles, (uint32_t)blocks);
     }
   }
   return rwkv_launch_status();
@@ -315,9 +318,9 @@ int unpack_v(const uint8_t* values, const uint8_t* exps, T* y, long long ldy, in
   for (int r0 = 0; r0 < R; r0 += most) {
     const int n = R - r0 < most ? R - r0 : most;
     const long long ctas = ((long long)n * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
-    fp8_unpack_kernel<T, V><<<grid_for(ctas, 32), ROW_THREADS, 0, st>>>(
-        values + (long long)r0 * ldv, exps + (rows == 1 ? r0 : (long long)(r0 / FP8_BLOCK) * blocks), y + r0 * ldy, ldy,
-        (uint32_t)n * blocks, C, ldv, lde, rows, blocks);
+    rwkv_launch(fp8_unpack_kernel<T, V>, dim3(grid_for(ctas, 32)), dim3(ROW_THREADS), 0, st, values + (long long)r0 * ldv,
+                exps + (rows == 1 ? (long long)r0 : (long long)(r0 / FP8_BLOCK) * blocks), y + r0 * ldy, ldy, (uint32_t)n * blocks, C,
+                ldv, lde, rows, (uint32_t)blocks);
   }
   return rwkv_launch_status();
 }

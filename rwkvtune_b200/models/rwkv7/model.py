@@ -231,7 +231,8 @@ class RWKV7TimeMix(nn.Module):
             if first:
                 v_first = v
             nxt = getattr(self, "_decode_next", None)          # the channel-mix half of this block
-            out = _project_add(self.output, z, x, _weights_of(getattr(nxt, "key", None)))
+            held = getattr(nxt, "_packed", None)               # its 8-bit weights, if it decodes with those
+            out = _project_add(self.output, z, x, [held[1][0].data] if held is not None else _weights_of(getattr(nxt, "key", None)))
             return out, v_first, (last if want_state else None), (new_state if want_state else None)
         if self.layer_id == 0:
             w, k, v, a_, b_ = ops.timemix_prep(k, v, None, w_lin, a_lin, None, self.w0, self.a0, None,

@@ -190,7 +190,7 @@ class _DeviceRun:
         if form == 2:
             x = native.decode_input(x)
             self.keep.append(x)
-            self.steps.append(native.decode(x, w, out, q=hidden))
+            self.steps.append(native.decode(x, w, out, q=hidden, chained=native.chaining()))
             return
         x8 = _matrix(x.device, x.shape[0], x.shape[1], 1)
         self.keep.append(x8)

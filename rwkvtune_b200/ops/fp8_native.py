@@ -105,6 +105,11 @@ def decode_form(M: int, N: int, K: int, packed: bool = False) -> int:
     return _ext.lib().rwkv_fp8_decode_form(M, N, K, int(packed)) if M <= 128 else 0
 
 
+def chaining() -> bool:
+    """True inside a chain of decode launches, during which no kernel writes weights (``_ext.launch_chaining``)."""
+    return _ext._CHAINING
+
+
 def decode_input(x: torch.Tensor) -> torch.Tensor:
     """``x [M, K]`` with rows that start on 16 bytes."""
     if x.stride(1) == 1 and x.data_ptr() % 16 == 0 and (x.shape[0] == 1 or (x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1])):
