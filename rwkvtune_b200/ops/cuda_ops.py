@@ -191,6 +191,8 @@ def _f32(t: torch.Tensor) -> torch.Tensor:
     key = (t.data_ptr(), t.numel(), t.dtype)
     stamp = (_PARAM_EPOCH, t._version)
     hit = _F32_CACHE.get(key)
+    if hit is not None and hit[2]() is not t:     # another parameter, since freed, lay at this address
+        hit = None
     if hit is not None and hit[0] == stamp:
         return hit[1]
     if hit is not None:
