@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include "fp8_format.cuh"
+#include "fp8_steps.cuh"
 
 namespace {
 
@@ -189,20 +190,48 @@ fp8_pack_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict
 
 constexpr int TILE_THREADS = 512;
 
-// A CTA walks over tiles and has the next one in flight while it works on the present one.
-template <typename T, int V>
+// Up to three matrices whose tiles follow one another: the operands of one pass in one launch.
+struct TileJob {
+  const void* x;
+  long long ldx;
+  uint8_t *values, *exps;
+  int R, C, ldv;
+  uint32_t blocks, end;           // column blocks; number of tiles up to and with this matrix
+};
+constexpr int MAX_JOBS = 3;
+struct TileJobs {
+  TileJob job[MAX_JOBS];
+  int count;
+};
+
+// A CTA walks over tiles and has the next one in flight while it works on the present one.  MANY: more than one matrix
+// (looking a tile's matrix up costs a single one 34.0 -> 36.8 us at 32768 x 2048).
+template <typename T, int V, bool MANY>
 __global__ void __launch_bounds__(TILE_THREADS, sizeof(T) == 4 ? 1 : 2)
-fp8_pack_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
-                      int R, int C, int ldv, uint32_t tiles, uint32_t blocks) {
+fp8_pack_tiles_kernel(const __grid_constant__ TileJobs all) {
   rwkv_chain_begin();
   __shared__ uint32_t warp_max[2][TILE_THREADS / 32];
+  const uint32_t tiles = MANY ? all.job[all.count - 1].end : all.job[0].end;
+  const int part = threadIdx.x & 7;
+  // the matrix of a tile, the tile's number in it, and this thread's first row and the tile's first column
+  const auto locate = [&](uint32_t tile, uint32_t& own, int& row, int& col) -> const TileJob& {
+    int j = 0;
+    while (MANY && j + 1 < all.count && tile >= all.job[j].end) ++j;
+    const TileJob& m = MANY ? all.job[j] : all.job[0];
+    own = tile - (j ? all.job[j - 1].end : 0);
+    row = (int)(own / m.blocks) * FP8_BLOCK + (threadIdx.x >> 3);
+    col = (int)(own % m.blocks) * FP8_BLOCK;
+    return m;
+  };
   Raw16<T> next[2];
-  auto fetch = [&](uint32_t tile) {
-    const int row0 = (int)(tile / blocks) * FP8_BLOCK + (threadIdx.x >> 3), col = (int)(tile % blocks) * FP8_BLOCK;
+  const auto fetch = [&](uint32_t tile) {
+    uint32_t own;
+    int row0, col;
+    const TileJob& m = locate(tile, own, row0, col);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = row0 + i * (TILE_THREADS / 8);
-      load16<T, V>(x + (long long)min(row, R - 1) * ldx + col, threadIdx.x & 7, row < R ? C - col : 0, next[i]);
+      load16<T, V>((const T*)m.x + min(row, m.R - 1) * m.ldx + col, part, row < m.R ? m.C - col : 0, next[i]);
     }
   };
   uint32_t tile = blockIdx.x;
@@ -214,23 +243,25 @@ fp8_pack_tiles_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restric
     const uint32_t now = tile;
     tile += gridDim.x;
     if (tile < tiles) fetch(tile);
-    uint32_t m = max(abs_bits16(f[0]), abs_bits16(f[1]));
+    uint32_t top = max(abs_bits16(f[0]), abs_bits16(f[1]));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) warp_max[turn][threadIdx.x >> 5] = m;
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) warp_max[turn][threadIdx.x >> 5] = top;
     __syncthreads();
-    m = warp_max[turn][threadIdx.x & (TILE_THREADS / 32 - 1)];
+    top = warp_max[turn][threadIdx.x & (TILE_THREADS / 32 - 1)];
 #pragma unroll
-    for (int o = TILE_THREADS / 64; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const uint32_t e = fp8_block_exponent(m);
-    const int row0 = (int)(now / blocks) * FP8_BLOCK + (threadIdx.x >> 3), col = (int)(now % blocks) * FP8_BLOCK;
+    for (int o = TILE_THREADS / 64; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t e = fp8_block_exponent(top);
+    uint32_t own;
+    int row0, col;
+    const TileJob& m = locate(now, own, row0, col);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int row = row0 + i * (TILE_THREADS / 8);
-      if (row < R)
-        store_packed<V / sizeof(T)>(values + (long long)row * ldv + col, threadIdx.x & 7, ldv - col, quantise16(f[i], e));
+      if (row < m.R)
+        store_packed<V / sizeof(T)>(m.values + (long long)row * m.ldv + col, part, m.ldv - col, quantise16(f[i], e));
     }
-    if (threadIdx.x == 0) exps[now] = (uint8_t)e;
+    if (threadIdx.x == 0) m.exps[own] = (uint8_t)e;
   }
 }
 
@@ -280,34 +311,55 @@ int rows_at_once(int R, int per_row) {
 }
 
 template <typename T, int V>
-int pack_v(const T* x, long long ld, uint8_t* values, uint8_t* exps, int R, int C, int rows, cudaStream_t st) {
-  const int blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK, ldv = up(C, 16);
-  const int most = rows_at_once(R, blocks);
-  for (int r0 = 0; r0 < R; r0 += most) {
-    const int n = R - r0 < most ? R - r0 : most;
-    const T* src = x + r0 * ld;
-    uint8_t* dst = values + (long long)r0 * ldv;
-    if (rows == 1) {
-      const long long ctas = ((long long)n * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
-      rwkv_launch(fp8_pack_rows_kernel<T, V>, dim3(grid_for(ctas, 16)), dim3(ROW_THREADS), 0, st, src, ld, dst, exps + r0,
-                  (uint32_t)n * blocks, C, ldv, up(R, 16), (uint32_t)blocks);
-    } else {
-      const uint32_t tiles = (uint32_t)((n + FP8_BLOCK - 1) / FP8_BLOCK) * blocks;
-      rwkv_launch(fp8_pack_tiles_kernel<T, V>, dim3(grid_for(tiles, sizeof(T) == 4 ? 1 : 2)), dim3(TILE_THREADS), 0, st, src, ld,
-                  dst, exps + (long long)(r0 / FP8_BLOCK) * blocks, n, C, ldv, tiles, (uint32_t)blocks);
-    }
+int pack_rows_v(const Fp8Step& s, cudaStream_t st) {
+  const int R = s.M, C = s.N, blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK, ldv = up(C, 16), most = rows_at_once(R, blocks);
+  for (long long r0 = 0; r0 < R; r0 += most) {
+    const int n = R - r0 < most ? (int)(R - r0) : most;
+    const long long ctas = ((long long)n * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
+    rwkv_launch(fp8_pack_rows_kernel<T, V>, dim3(grid_for(ctas, 16)), dim3(ROW_THREADS), 0, st, (const T*)s.x + r0 * s.ldx, s.ldx,
+                (uint8_t*)s.q_val + r0 * ldv, (uint8_t*)s.q_exp + r0, (uint32_t)n * blocks, C, ldv, up(R, 16), (uint32_t)blocks);
   }
   return rwkv_launch_status();
 }
+template <typename T, int V>
+int pack_tiles_v(const Fp8Step* s, int count, cudaStream_t st) {
+  TileJobs all = {};
+  uint32_t tiles = 0;
+  const auto launch = [&] {
+    if (!all.count) return;
+    rwkv_launch(all.count > 1 ? fp8_pack_tiles_kernel<T, V, true> : fp8_pack_tiles_kernel<T, V, false>,
+                dim3(grid_for(tiles, sizeof(T) == 4 ? 1 : 2)), dim3(TILE_THREADS), 0, st, all);
+    all.count = 0;
+    tiles = 0;
+  };
+  for (int i = 0; i < count; ++i) {
+    const int R = s[i].M, C = s[i].N, blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK, ldv = up(C, 16), most = rows_at_once(R, blocks);
+    for (long long r0 = 0; r0 < R; r0 += most) {
+      const int n = R - r0 < most ? (int)(R - r0) : most;
+      const uint32_t own = (uint32_t)((n + FP8_BLOCK - 1) / FP8_BLOCK) * blocks;
+      if (all.count == MAX_JOBS || tiles + own > 0x40000000u) launch();
+      tiles += own;
+      all.job[all.count++] = {(const T*)s[i].x + r0 * s[i].ldx, s[i].ldx, (uint8_t*)s[i].q_val + r0 * ldv,
+                              (uint8_t*)s[i].q_exp + r0 / FP8_BLOCK * blocks, n, C, ldv, (uint32_t)blocks, tiles};
+    }
+  }
+  launch();
+  return rwkv_launch_status();
+}
 template <typename T>
-int pack_t(const void* x, long long ld, uint8_t* values, uint8_t* exps, int R, int C, int rows, cudaStream_t st) {
-  const T* p = (const T*)x;
-  switch (access_bytes(x, ld * (long long)sizeof(T))) {
-    case 32: return pack_v<T, 32>(p, ld, values, exps, R, C, rows, st);
-    case 16: return pack_v<T, 16>(p, ld, values, exps, R, C, rows, st);
-    case 8: return pack_v<T, 8>(p, ld, values, exps, R, C, rows, st);
-    case 4: return pack_v<T, 4>(p, ld, values, exps, R, C, rows, st);
-    default: return pack_v<T, sizeof(T)>(p, ld, values, exps, R, C, rows, st);
+int pack_t(const Fp8Step* s, int count, cudaStream_t st) {
+  int v = 32;
+  for (int i = 0; i < count; ++i) {
+    const int w = access_bytes(s[i].x, s[i].ldx * (long long)sizeof(T));
+    if (w < v) v = w;
+  }
+  const bool by_row = s[0].q_rows == 1;
+  switch (v) {
+    case 32: return by_row ? pack_rows_v<T, 32>(*s, st) : pack_tiles_v<T, 32>(s, count, st);
+    case 16: return by_row ? pack_rows_v<T, 16>(*s, st) : pack_tiles_v<T, 16>(s, count, st);
+    case 8: return by_row ? pack_rows_v<T, 8>(*s, st) : pack_tiles_v<T, 8>(s, count, st);
+    case 4: return by_row ? pack_rows_v<T, 4>(*s, st) : pack_tiles_v<T, 4>(s, count, st);
+    default: return by_row ? pack_rows_v<T, sizeof(T)>(*s, st) : pack_tiles_v<T, sizeof(T)>(s, count, st);
   }
 }
 template <typename T, int V>
@@ -315,11 +367,11 @@ int unpack_v(const uint8_t* values, const uint8_t* exps, T* y, long long ldy, in
   const int ldv = up(C, 16), blocks = (C + FP8_BLOCK - 1) / FP8_BLOCK;
   const int lde = rows == 1 ? up(R, 16) : blocks;
   const int most = rows_at_once(R, blocks);
-  for (int r0 = 0; r0 < R; r0 += most) {
-    const int n = R - r0 < most ? R - r0 : most;
+  for (long long r0 = 0; r0 < R; r0 += most) {
+    const int n = R - r0 < most ? (int)(R - r0) : most;
     const long long ctas = ((long long)n * blocks + ROW_THREADS / 8 - 1) / (ROW_THREADS / 8);
-    rwkv_launch(fp8_unpack_kernel<T, V>, dim3(grid_for(ctas, 32)), dim3(ROW_THREADS), 0, st, values + (long long)r0 * ldv,
-                exps + (rows == 1 ? (long long)r0 : (long long)(r0 / FP8_BLOCK) * blocks), y + r0 * ldy, ldy, (uint32_t)n * blocks, C,
+    rwkv_launch(fp8_unpack_kernel<T, V>, dim3(grid_for(ctas, 32)), dim3(ROW_THREADS), 0, st, values + r0 * ldv,
+                exps + (rows == 1 ? r0 : r0 / FP8_BLOCK * blocks), y + r0 * ldy, ldy, (uint32_t)n * blocks, C,
                 ldv, lde, rows, (uint32_t)blocks);
   }
   return rwkv_launch_status();
@@ -342,24 +394,22 @@ bool args_ok(const void* values, long long ld, int dtype, int R, int C, int rows
 
 }  // namespace
 
-// x [R, C] (row stride ldx, dtype 0 bf16, 1 fp16, 2 fp32) -> values [R, C rounded up to 16], exponents as in fp8_format.cuh
-RWKV_EXPORT int rwkv_fp8_pack(const void* x, int dtype, long long ldx, void* values, void* exps, int R, int C, int rows,
-                              void* stream) {
-  if (!args_ok(values, ldx, dtype, R, C, rows)) return RWKV_ERR_BAD_SHAPE;
-  cudaStream_t st = (cudaStream_t)stream;
-  uint8_t *v = (uint8_t*)values, *e = (uint8_t*)exps;
-  if (dtype == 0) return pack_t<bf16>(x, ldx, v, e, R, C, rows, st);
-  if (dtype == 1) return pack_t<__half>(x, ldx, v, e, R, C, rows, st);
-  return pack_t<float>(x, ldx, v, e, R, C, rows, st);
+// Pack: x [M, N] (row stride ldx, dtype 0 bf16, 1 fp16, 2 fp32) -> q_val [M, N rounded up to 16], q_exp as in fp8_format.cuh,
+// blocks of q_rows rows.  More than one record: tiles of one type each, one launch for up to three.
+int rwkv_fp8_pack(const Fp8Step* s, int count, cudaStream_t st) {
+  for (int i = 0; i < count; ++i) {
+    if (!args_ok(s[i].q_val, s[i].ldx, s[i].dtype, s[i].M, s[i].N, s[i].q_rows)) return RWKV_ERR_BAD_SHAPE;
+    if (count > 1 && (s[i].q_rows != FP8_BLOCK || s[i].dtype != s[0].dtype)) return RWKV_ERR_BAD_SHAPE;
+  }
+  if (s[0].dtype == 0) return pack_t<bf16>(s, count, st);
+  return s[0].dtype == 1 ? pack_t<__half>(s, count, st) : pack_t<float>(s, count, st);
 }
 
-// the values a packed matrix stands for, y [R, C] (row stride ldy)
-RWKV_EXPORT int rwkv_fp8_unpack(const void* values, const void* exps, void* y, int dtype, long long ldy, int R, int C, int rows,
-                                void* stream) {
-  if (!args_ok(values, ldy, dtype, R, C, rows)) return RWKV_ERR_BAD_SHAPE;
-  cudaStream_t st = (cudaStream_t)stream;
-  const uint8_t *v = (const uint8_t*)values, *e = (const uint8_t*)exps;
-  if (dtype == 0) return unpack_t<bf16>(v, e, y, ldy, R, C, rows, st);
-  if (dtype == 1) return unpack_t<__half>(v, e, y, ldy, R, C, rows, st);
-  return unpack_t<float>(v, e, y, ldy, R, C, rows, st);
+// Unpack: the values that (a_val, a_exp) [M, N] stands for -> c (row stride ldc)
+int rwkv_fp8_unpack(const Fp8Step& s, cudaStream_t st) {
+  if (!args_ok(s.a_val, s.ldc, s.dtype, s.M, s.N, s.a_rows)) return RWKV_ERR_BAD_SHAPE;
+  const uint8_t *v = (const uint8_t*)s.a_val, *e = (const uint8_t*)s.a_exp;
+  if (s.dtype == 0) return unpack_t<bf16>(v, e, s.c, s.ldc, s.M, s.N, s.a_rows, st);
+  if (s.dtype == 1) return unpack_t<__half>(v, e, s.c, s.ldc, s.M, s.N, s.a_rows, st);
+  return unpack_t<float>(v, e, s.c, s.ldc, s.M, s.N, s.a_rows, st);
 }

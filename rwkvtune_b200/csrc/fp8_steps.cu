@@ -3,11 +3,6 @@
 // therefore describes the launches in one array of plain records.
 #include "fp8_steps.cuh"
 
-RWKV_EXPORT int rwkv_fp8_pack(const void* x, int dtype, long long ldx, void* values, void* exps, int R, int C, int rows,
-                              void* stream);
-RWKV_EXPORT int rwkv_fp8_unpack(const void* values, const void* exps, void* y, int dtype, long long ldy, int R, int C, int rows,
-                                void* stream);
-
 // Runs `count` steps in order on `stream`; returns the status of the first that was refused or failed to launch.
 RWKV_EXPORT int rwkv_fp8_run(const Fp8Step* steps, int count, void* stream) {
   if (count < 0 || (count > 0 && !steps)) return RWKV_ERR_BAD_SHAPE;
@@ -15,8 +10,16 @@ RWKV_EXPORT int rwkv_fp8_run(const Fp8Step* steps, int count, void* stream) {
     const Fp8Step& s = steps[i];
     int r = RWKV_ERR_BAD_SHAPE;
     switch (s.kind) {
-      case FP8_STEP_PACK: r = rwkv_fp8_pack(s.x, s.dtype, s.ldx, s.q_val, s.q_exp, s.M, s.N, s.q_rows, stream); break;
-      case FP8_STEP_UNPACK: r = rwkv_fp8_unpack(s.a_val, s.a_exp, s.c, s.dtype, s.ldc, s.M, s.N, s.a_rows, stream); break;
+      case FP8_STEP_PACK: {                   // tiles of one type that follow one another go out together
+        int n = 1;
+        while (s.q_rows == 128 && i + n < count && steps[i + n].kind == FP8_STEP_PACK && steps[i + n].q_rows == 128 &&
+               steps[i + n].dtype == s.dtype)
+          ++n;
+        r = rwkv_fp8_pack(steps + i, n, (cudaStream_t)stream);
+        i += n - 1;
+        break;
+      }
+      case FP8_STEP_UNPACK: r = rwkv_fp8_unpack(s, (cudaStream_t)stream); break;
       case FP8_STEP_GEMM:
         if (!s.with_next) {
           r = rwkv_fp8_gemm(s, (cudaStream_t)stream);

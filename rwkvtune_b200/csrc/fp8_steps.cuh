@@ -23,6 +23,8 @@ struct Fp8Step {
   void* status;
 };
 
+int rwkv_fp8_pack(const Fp8Step* s, int count, cudaStream_t stream);
+int rwkv_fp8_unpack(const Fp8Step& s, cudaStream_t stream);
 int rwkv_fp8_gemm(const Fp8Step& s, cudaStream_t stream);
 int rwkv_fp8_gemm_two(const Fp8Step& s, const Fp8Step& t, cudaStream_t stream);
 int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t stream);
