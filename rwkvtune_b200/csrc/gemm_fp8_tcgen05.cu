@@ -22,14 +22,13 @@
 // the overlap costs one 64-column read per tile instead of a whole drained accumulator.  Two groups of four warps drain a
 // tile, 128 columns each.
 //
-// What bounds it (e4m3 at twice the measured bf16 GEMM rate: 3.32 PFLOP/s burst, 2.78 sustained): the tensor pipe is active
-// for 92 % of the cycles in dW 8192 x 2048 x 16384, 88 % in 16384 x 2048 x 8192, 79 and 75 % in the two packed epilogues at
-// a contraction of 2048, where the 650 cycles between two tiles' products weigh most (accumulator complete, shared columns
-// read, pair told).  A step of 128 columns takes 570 cycles against 512 of the pipe: its operands cross shared memory at the
-// full 128 bytes a cycle, half written by TMA and half read.  32768 x 2048 x 2048 in 109 us (2.5 PFLOP/s), x 8192 in 367 us
-// (3.0), relu^2 packed 32768 x 8192 x 2048 in 370-405 us, its derivative 415-440.  In a long run the 1000 W cap holds the SMs
-// near 1.28 GHz and everything takes 1.15 times as long.  Four or three ring stages instead of five: NN x 8192 433 and 524
-// us against 411.
+// What bounds it.  A step of 128 contraction elements is 512 cycles of the tensor pipe.  Measured over whole kernels it takes
+// 519 cycles in dW 8192 x 2048 x 32768 (TN), 534 in 32768 x 2048 x 8192 (NN), and 606 to 628 at a contraction of 2048, where
+// the 650 cycles between two tiles' products weigh most (accumulator complete, shared columns read, both CTAs told).  With
+// that many products a cycle the power cap sets the clock: 1.32 to 1.45 GHz on random data against 1.75 to 1.8 on zeros.
+// 32768 x 2048 x 2048 in 94 to 109 us, x 8192 in 365 us (3.0 PFLOP/s), relu^2 packed 32768 x 8192 x 2048 in 383 to 405 us, its
+// derivative 411 to 440, dW 8192 x 2048 x 32768 in 396; in a run of seconds (1.28 GHz) 1.15 times that.  Four or three ring
+// stages instead of five: NN x 8192 433 and 524 us against 411.
 //
 // Every mbarrier wait is bounded as in gemm_tcgen05_2cta.cu: on expiry a code goes to `status`, all roles leave, the CTAs
 // meet, tensor memory is released and the kernel returns.

@@ -14,6 +14,7 @@ training with the state carried between chunks
 from __future__ import annotations
 
 import math
+import weakref
 from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -301,21 +302,33 @@ class RWKV7ChannelMix(nn.Module):
     def _weights_stamp(self):
         return self.key.weight._version, self.value.weight._version, ops.param_epoch()
 
+    def _weights_kept(self, held) -> bool:
+        """True while the weights are the parameters, and at the versions, that were packed."""
+        return held[0] == self._weights_stamp() and held[2]() is self.key.weight and held[3]() is self.value.weight
+
     def pack(self) -> None:
-        """Hold key and value in 8 bits beside the weights; forward passes without autograd use those from now on."""
+        """Hold key and value in 8 bits beside the weights; forward passes without autograd use those from now on.  Called
+        again it writes to the same memory where it can, so that a captured step follows."""
         if not self._plain():
             raise ValueError("8-bit feed-forward weights need plain projections (merge the adapter; no ZeRO-3 panels)")
-        packed = ops.pack_fp8(self.key.weight), ops.pack_fp8(self.value.weight)
-        object.__setattr__(self, "_packed", (self._weights_stamp(), packed))
+        held, weights = getattr(self, "_packed", None), (self.key.weight, self.value.weight)
+        again = held is not None and all(tuple(p.shape) == tuple(w.shape) and (p.dtype, p.device) == (w.dtype, w.device)
+                                         for p, w in zip(held[1], weights))
+        packed = tuple(ops.pack_fp8(w, out=p) for w, p in zip(weights, held[1] if again else (None, None)))
+        object.__setattr__(self, "_packed", (self._weights_stamp(), packed, *(weakref.ref(w) for w in weights)))
 
     def unpack(self) -> None:
         object.__setattr__(self, "_packed", None)
+
+    def __getstate__(self):
+        """Copies and pickles carry the weights, not their packed form (pack the copy)."""
+        return {k: v for k, v in self.__dict__.items() if k != "_packed"}
 
     def forward(self, x, ln_w, ln_b, x_prev=None, want_state: bool = False):
         (xk,), last, x = ops.ln_shift_mix_unbound(x, ln_w, ln_b, self.x_k, x_prev)
         held = getattr(self, "_packed", None)
         if held is not None and not torch.is_grad_enabled():
-            if held[0] != self._weights_stamp():
+            if not self._weights_kept(held):
                 raise RuntimeError("the feed-forward weights have changed since pack_ffn(): call it again, or unpack_ffn()")
             return ops.fp8_channel_mix_ffn(xk, *held[1], x), (last if want_state else None)
         if getattr(self.config, "ffn_precision", "bf16") == "fp8" and not _decoding(xk):
@@ -523,8 +536,8 @@ class RWKV7Model(GenerationMixin, nn.Module):
     def pack_ffn(self) -> "RWKV7Model":
         """Hold every block's feed-forward weights in 8 bits as well (half their bf16 size again): passes without autograd -
         decoding, prefill, evaluation - then run those products in 8 bits.  A token's result does not depend on the batch
-        it is in.  Call it again after changing the weights; a stale copy is refused.  A captured decode graph keeps the
-        form that the weights had when it was captured."""
+        it is in.  Call it again after changing the weights (captured decode graphs then follow); a stale copy is refused
+        outside of replays."""
         for block in self.blocks:
             block.ffn.pack()
         return self

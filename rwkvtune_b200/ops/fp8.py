@@ -248,9 +248,10 @@ def _f32(p: Fp8Blocks) -> torch.Tensor:
     return reference.fp8_unpack(p.values, p.exponents, p.rows)
 
 
-def pack_fp8(x: torch.Tensor, rows: int = BLOCK) -> Fp8Blocks:
+def pack_fp8(x: torch.Tensor, rows: int = BLOCK, out: Optional[Fp8Blocks] = None) -> Fp8Blocks:
     """Hold ``x [..., C]`` in 8 bits (leading dimensions are flattened to rows).  ``rows=1``: one scale per token and 128
-    channels; ``rows=128``: one per tile of 128 x 128.  Not differentiable."""
+    channels; ``rows=128``: one per tile of 128 x 128.  ``out``: an earlier result for the same shape, type, device and
+    ``rows``, written again in place (a captured graph that reads it sees the new values).  Not differentiable."""
     if not isinstance(x, torch.Tensor) or x.dtype not in _FLOATS:
         raise TypeError(f"pack_fp8 takes a bfloat16, float16 or float32 tensor, got {getattr(x, 'dtype', type(x).__name__)}")
     if rows not in (1, BLOCK):
@@ -258,7 +259,13 @@ def pack_fp8(x: torch.Tensor, rows: int = BLOCK) -> Fp8Blocks:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"pack_fp8: the last dimension must not be empty, got shape {tuple(x.shape)}")
     x2 = _rows_of(x.detach())
-    p = _matrix(x.device, x2.shape[0], x2.shape[1], rows, x.shape, x.dtype)
+    if out is None:
+        p = _matrix(x.device, x2.shape[0], x2.shape[1], rows, x.shape, x.dtype)
+    else:
+        p = out
+        if not isinstance(p, Fp8Blocks) or (tuple(p.shape), p.dtype, p.rows, p.device) != (tuple(x.shape), x.dtype, rows, x.device):
+            raise ValueError(f"pack_fp8: out does not hold a {tuple(x.shape)} tensor of {x.dtype} on {x.device} with rows={rows}: {out!r}")
+        torch.autograd.graph.increment_version(p.data)      # a backward pass that kept the old values is refused
     run = _run_on(x)
     run.pack(x2, p)
     run.go()

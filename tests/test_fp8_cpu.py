@@ -93,6 +93,27 @@ def test_shapes_leading_dimensions_and_empty():
     assert ops.unpack_fp8(ops.pack_fp8(torch.ones(7))).shape == (7,)
 
 
+def test_packing_again_in_place():
+    x, y = sample(6, 40, BF).view(2, 3, 40), sample(6, 40, BF, 1).view(2, 3, 40)
+    for rows in (1, 128):
+        p = ops.pack_fp8(x, rows=rows)
+        q = ops.pack_fp8(y, rows=rows, out=p)
+        assert q is p and torch.equal(ops.unpack_fp8(p), ops.unpack_fp8(ops.pack_fp8(y, rows=rows)))
+        for bad in (y[:1], y.float(), y.transpose(0, 1)):
+            with pytest.raises(ValueError):
+                ops.pack_fp8(bad, rows=rows, out=p)
+        with pytest.raises(ValueError):
+            ops.pack_fp8(y, rows=129 - rows, out=p)
+    with pytest.raises(ValueError):
+        ops.pack_fp8(y, out=p.data)
+    w = ops.pack_fp8(weights(16, 40))
+    a = sample(3, 40, torch.float32).requires_grad_()
+    out = ops.fp8_linear(a, w).sum()
+    ops.pack_fp8(weights(16, 40, 5), out=w)
+    with pytest.raises(RuntimeError):              # the forward pass saw other weights
+        out.backward()
+
+
 def weights(N, K, seed=1):
     g = torch.Generator().manual_seed(seed)
     return (torch.rand(N, K, generator=g) - 0.5) * 2 / math.sqrt(K)

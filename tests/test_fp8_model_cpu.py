@@ -142,6 +142,24 @@ def test_stale_packed_weights_are_refused():
         with pytest.raises(RuntimeError, match="pack_ffn"):
             m(ids)
     m.train().loss(*batch()).backward()            # training uses the weights themselves
+    m.eval().pack_ffn()
+    kept = m.blocks[0].ffn._packed[1][0].address
+    m.pack_ffn()
+    assert m.blocks[0].ffn._packed[1][0].address == kept
+    m.blocks[0].ffn.key.weight = torch.nn.Parameter(m.blocks[0].ffn.key.weight.detach().clone())
+    with torch.no_grad(), pytest.raises(RuntimeError, match="pack_ffn"):
+        m(ids)
+
+
+def test_copies_and_pickles_of_a_packed_model():
+    import pickle
+
+    m, ids = make().eval(), batch()[0]
+    with torch.no_grad():
+        plain, packed = m(ids), m.pack_ffn()(ids)
+        for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+            assert torch.equal(other(ids), plain) and torch.equal(other.pack_ffn()(ids), packed)
+        assert torch.equal(m(ids), packed)
 
 
 def test_packing_wrapped_projections_is_refused():

@@ -118,6 +118,22 @@ def test_packed_decode_steps():
     assert gemm_native.check_status() == 0
 
 
+def test_a_captured_step_follows_weights_that_are_packed_again():
+    from rwkvtune_b200.inference import GRPOBatchGenerator
+
+    m = make().eval().pack_ffn()
+    gen = GRPOBatchGenerator(m, None, torch.device("cuda", 0), eos_token_id=0, use_cuda_graph=True)
+    args = dict(input_ids=[[5, 6, 7, 8]] * 2, max_new_tokens=10, num_generations=1, temperature=1.0, top_p=1.0, seed=3)
+    first = gen.generate(**args)["completion_ids"].cpu()
+    with torch.no_grad():
+        for b in m.blocks:
+            b.ffn.value.weight.mul_(-3.0)
+    m.pack_ffn()
+    again = gen.generate(**args)["completion_ids"].cpu()
+    eager = GRPOBatchGenerator(m, None, torch.device("cuda", 0), eos_token_id=0, use_cuda_graph=False).generate(**args)
+    assert torch.equal(again, eager["completion_ids"].cpu()) and not torch.equal(first, again)
+
+
 def test_packed_and_plain_logits_are_near():
     m, (ids, _) = make().eval(), batch()
     with torch.no_grad():
