@@ -243,6 +243,45 @@ def bench_decode_core(C, out, hbm, paths=64, layers=8):
         cuda_ops.INPLACE_STATE = False
 
 
+def bench_fp8(B, T, C, out, hbm, tf):
+    """Packing, the products of packed operands and the decode products; rates against the copy and the bf16 GEMM peak."""
+    from rwkvtune_b200.ops import fp8
+
+    M, H = B * T, 4 * C
+    rnd = lambda *shape: torch.randn(*shape, device="cuda").to(BF)  # noqa: E731
+    x, res = rnd(M, C), rnd(M, C)
+    for rows in (1, 128):
+        p = ops.pack_fp8(x, rows=rows)
+        for tag, fn in (("pack", lambda: ops.pack_fp8(x, rows=rows, out=p)), ("unpack", lambda: ops.unpack_fp8(p))):
+            ms = timeit(fn)
+            out[f"fp8_{tag}_rows{rows}_us"] = ms * 1e3
+            out[f"fp8_{tag}_rows{rows}_frac_hbm"] = M * C * 3 / ms / 1e6 / hbm
+    x8, k8, v8 = ops.pack_fp8(x), ops.pack_fp8(rnd(H, C)), ops.pack_fp8(rnd(C, H))
+    h8, p8 = fp8._room(x.device, (M, H, 128), (M, H, 128))
+    y, dk = torch.empty_like(x), torch.empty(H, C, dtype=BF, device="cuda")
+
+    def step(name, *args):
+        def fn():
+            run = fp8._run_on(x)
+            getattr(run, name)(*args)
+            run.go()
+        return fn
+
+    for tag, fn in (("key_relu_sq", step("nt_relu_sq", x8, k8, h8)), ("value_residual", step("nt", h8, v8, y, res)),
+                    ("dvalue_relu_sq_grad", step("nn_relu_sq_grad", x8, v8, h8, p8)), ("dkey", step("nn", p8, k8, y)),
+                    ("dw_key", step("tn", p8, x8, dk))):
+        ms = timeit(fn)
+        out[f"fp8_{tag}_us"] = ms * 1e3
+        out[f"fp8_{tag}_tflops_over_bf16_peak"] = 2 * M * C * H / ms / 1e9 / tf
+    for n in (1, 64):
+        xs, head = rnd(n, C), ops.pack_fp8(rnd(65536, C))
+        with torch.no_grad():
+            ms = _graph_time(lambda: ops.fp8_linear(xs, head))
+            out[f"fp8_head_{n}rows_us"] = ms * 1e3
+            out[f"fp8_head_{n}rows_frac_hbm"] = 65536 * C / ms / 1e6 / hbm
+            out[f"fp8_ffn_{n}rows_us"] = _graph_time(lambda: ops.fp8_channel_mix_ffn(xs, k8, v8, xs)) * 1e3
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--only", default="")
@@ -266,6 +305,8 @@ def main():
         bench_decode_gemm(a.C, out, hbm)
     if not only or "decode_core" in only:
         bench_decode_core(a.C, out, hbm)
+    if not only or "fp8" in only:
+        bench_fp8(a.B, a.T, a.C, out, hbm, tf)
     for k, v in out.items():
         print(f"{k}: {v:.4g}" if isinstance(v, float) else f"{k}: {v}")
     if a.json:
