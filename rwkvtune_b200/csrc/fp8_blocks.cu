@@ -13,6 +13,8 @@
 // Arithmetic in the rest of the library flushes numbers below 2^-126 to zero, and so do these kernels.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "fp8_format.cuh"
 #include "fp8_steps.cuh"
 
@@ -327,8 +329,10 @@ int pack_tiles_v(const Fp8Step* s, int count, cudaStream_t st) {
   uint32_t tiles = 0;
   const auto launch = [&] {
     if (!all.count) return;
-    rwkv_launch(all.count > 1 ? fp8_pack_tiles_kernel<T, V, true> : fp8_pack_tiles_kernel<T, V, false>,
-                dim3(grid_for(tiles, sizeof(T) == 4 ? 1 : 2)), dim3(TILE_THREADS), 0, st, all);
+    auto kern = fp8_pack_tiles_kernel<T, V, false>;
+    if constexpr (std::is_same<T, bf16>::value)           // only the products' operands come several at a time
+      if (all.count > 1) kern = fp8_pack_tiles_kernel<T, V, true>;
+    rwkv_launch(kern, dim3(grid_for(tiles, sizeof(T) == 4 ? 1 : 2)), dim3(TILE_THREADS), 0, st, all);
     all.count = 0;
     tiles = 0;
   };
@@ -337,7 +341,7 @@ int pack_tiles_v(const Fp8Step* s, int count, cudaStream_t st) {
     for (long long r0 = 0; r0 < R; r0 += most) {
       const int n = R - r0 < most ? (int)(R - r0) : most;
       const uint32_t own = (uint32_t)((n + FP8_BLOCK - 1) / FP8_BLOCK) * blocks;
-      if (all.count == MAX_JOBS || tiles + own > 0x40000000u) launch();
+      if (all.count == (std::is_same<T, bf16>::value ? MAX_JOBS : 1) || tiles + own > 0x40000000u) launch();
       tiles += own;
       all.job[all.count++] = {(const T*)s[i].x + r0 * s[i].ldx, s[i].ldx, (uint8_t*)s[i].q_val + r0 * ldv,
                               (uint8_t*)s[i].q_exp + r0 / FP8_BLOCK * blocks, n, C, ldv, (uint32_t)blocks, tiles};

@@ -571,14 +571,14 @@ RWKV_EXPORT int rwkv_fp8_decode_form(int M, int N, int K, int packed) {
 }
 
 // x: bf16 rows (16-byte aligned, K a multiple of 8) or, if null, packed tokens in (a_val, a_exp) with blocks of one row;
-// epilogue 0, 1, 2 as in gemm_fp8_tcgen05.cu with q_rows = 1.  chained: may start before its predecessor in the stream has
+// epilogue 0, 1 (packed tokens only), 2 as in gemm_fp8_tcgen05.cu with q_rows = 1.  chained: may start before its predecessor in the stream has
 // finished; the weights must not be written by it.
 int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t st) {
   const int M = s.M, N = s.N, K = s.K;
   if (M < 1 || M > 128 || N < 1 || K < 1 || N > 0x7ffffe00 || K > 0x7ffffe00 || s.epilogue < 0 || s.epilogue > 2)
     return RWKV_ERR_BAD_SHAPE;
   const bool packed = !s.x;
-  if (packed ? !s.a_val || !s.a_exp || s.a_rows != 1 : (K % 8 || s.ldx < K)) return RWKV_ERR_BAD_SHAPE;
+  if (packed ? !s.a_val || !s.a_exp || s.a_rows != 1 : (K % 8 || s.ldx < K || s.epilogue == 1)) return RWKV_ERR_BAD_SHAPE;
   if (!packed && (((uintptr_t)s.x & 15) || s.ldx % 8)) return RWKV_ERR_BAD_ALIGNMENT;
   if (s.epilogue == 2 ? !s.q_val || !s.q_exp || s.q_rows != 1 : !s.c || s.ldc < N || (s.epilogue == 1 && (!s.residual || s.ldr < N)))
     return RWKV_ERR_BAD_SHAPE;
@@ -608,6 +608,5 @@ int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t st) {
     if (s.epilogue == 2) return launch<true, EPI_RELU_SQ>(mw, mx, g, lay.smem, ch, st);
     return s.epilogue == 1 ? launch<true, EPI_RESIDUAL>(mw, mx, g, lay.smem, ch, st) : launch<true, EPI_STORE>(mw, mx, g, lay.smem, ch, st);
   }
-  if (s.epilogue == 2) return launch<false, EPI_RELU_SQ>(mw, mx, g, lay.smem, ch, st);
-  return s.epilogue == 1 ? launch<false, EPI_RESIDUAL>(mw, mx, g, lay.smem, ch, st) : launch<false, EPI_STORE>(mw, mx, g, lay.smem, ch, st);
+  return s.epilogue == 2 ? launch<false, EPI_RELU_SQ>(mw, mx, g, lay.smem, ch, st) : launch<false, EPI_STORE>(mw, mx, g, lay.smem, ch, st);
 }

@@ -76,7 +76,7 @@ struct Barriers {
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 2 * OUT_BYTES + SF_STAGES * SF_BYTES + 512 + 1024;
 
 struct Args {
-  int M, N, K;
+  int M, N;
   const uint8_t* a_exp;
   const uint8_t* b_exp;
   int a_rows;                    // 1 or 128
@@ -797,7 +797,7 @@ int describe(const Fp8Step& s, Problem& p) {
   p.tiles = (int)tiles; p.tiles_n = up(N, TN) / TN; p.num_kb = kb_n;
   Args& g = p.g;
   g = {};
-  g.M = M; g.N = N; g.K = K;
+  g.M = M; g.N = N;
   g.a_exp = (const uint8_t*)s.a_exp; g.b_exp = (const uint8_t*)s.b_exp;
   g.a_rows = s.a_rows;
   g.a_ld = up(M, 16);

@@ -118,7 +118,8 @@ def decode_input(x: torch.Tensor) -> torch.Tensor:
 
 
 def decode(x, b, out=None, residual=None, q=None, chained: bool = False) -> bytes:
-    """``out = x @ b^T (+ residual)`` or ``q = packed relu(x @ b^T)^2`` for at most 128 rows; ``x`` is packed or bf16."""
+    """``out = x @ b^T (+ residual)`` or ``q = packed relu(x @ b^T)^2`` for at most 128 rows; ``x`` is packed, or bf16 if there
+    is no residual."""
     N, K = b.R, b.C
     if isinstance(x, torch.Tensor):
         M, px, pa, ae = x.shape[0], x.data_ptr(), 0, 0

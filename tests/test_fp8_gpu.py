@@ -189,7 +189,7 @@ def test_few_rows(M, N, K):
     for t in forms:
         out, out_r = (torch.full((M, N), math.nan, dtype=BF, device="cuda") for _ in range(2))
         (q,) = fp8._room(x.device, (M, N, 1))
-        native.run(x.device, [native.decode(t, w8, out), native.decode(t, w8, out_r, res), native.decode(t, w8, q=q)])
+        native.run(x.device, [native.decode(t, w8, out), native.decode(x8, w8, out_r, res), native.decode(t, w8, q=q)])
         near(out, pre, mag, K)
         near(out_r, res.double() + pre, mag + res.double().abs(), K)
         packed_near(q, torch.relu(pre) ** 2, 2 * pre.abs() * mag + 1e-30, K, 1)
