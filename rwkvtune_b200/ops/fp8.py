@@ -311,13 +311,14 @@ class _Linear(torch.autograd.Function):
         if not (need_x and need_w):
             a, b = _room(x.device, None if need_w else (M, K, BLOCK), None if need_x else (N, K, BLOCK))
             x8, w8 = x8 or a, w8 or b
-        y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+        # in its final shape: autograd refuses to write in place to a view made in here
+        y = x.new_empty((*x.shape[:-1], N))
         run = _run_on(x)
         run.pack(x2, x8)
         run.pack(w, w8)
-        run.nt(x8, w8, y)
+        run.nt(x8, w8, _rows_of(y))
         run.go()
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+        return y
 
     @staticmethod
     @once_differentiable

@@ -285,3 +285,18 @@ def test_no_second_derivative():
     (g,) = torch.autograd.grad(ops.fp8_linear(x, w).sum(), [x], create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("frozen", [False, True])
+@pytest.mark.parametrize("shape", [(64,), (4, 64), (2, 3, 64), (0, 3, 64)])
+def test_result_may_be_written_in_place(shape, frozen):
+    # the map is y = P(x) P(W)^T and then 2 y + 1 in place: the gradient is twice that of y itself, exactly (a power of two)
+    x, w = torch.randn(shape, requires_grad=True), torch.randn(40, 64)
+    weight = ops.pack_fp8(w) if frozen else w.requires_grad_()
+    y = ops.fp8_linear(x, weight)
+    (want,) = torch.autograd.grad(y.sum(), [x])
+    z = ops.fp8_linear(x, weight)
+    z.mul_(2).add_(1)
+    assert torch.equal(z, y * 2 + 1)
+    (got,) = torch.autograd.grad(z.sum(), [x])
+    assert torch.equal(got, 2 * want)
