@@ -113,7 +113,7 @@ class _HostRun:
 
     def pack(self, x, q):
         if q.R:
-            values, exponents = reference.fp8_pack(x, q.rows)
+            values, exponents = reference.fp8_pack(x.detach(), q.rows)
             q.values.copy_(values)
             q.exponents.copy_(exponents)
 
@@ -161,10 +161,11 @@ class _DeviceRun:
 
     def pack(self, x, q):
         if q.R:
-            if (q.C > 1 and x.stride(1) != 1) or (q.R > 1 and x.stride(0) < q.C):
+            s0, s1 = x.stride()
+            if (s1 != 1 and q.C > 1) or (s0 < q.C and q.R > 1):
                 x = x.contiguous()
+                self.keep.append(x)
             self.steps.append(native.pack(x, q))
-            self.keep.append(x)
 
     def unpack(self, p, out):
         if p.R:
@@ -184,15 +185,16 @@ class _DeviceRun:
 
     def nt_frozen(self, x, w, out, hidden=None):
         """``out = P(x) w^T`` or ``hidden = P(relu(P(x) w^T)^2)`` with ``x`` packed row by row."""
-        if not x.shape[0]:
+        M = x.shape[0]
+        if not M:
             return
-        form = native.decode_form(x.shape[0], w.R, w.C)
+        form = native.decode_form(M, w.R, w.C)
         if form == 2:
             x = native.decode_input(x)
             self.keep.append(x)
             self.steps.append(native.decode(x, w, out, q=hidden, chained=native.chaining()))
             return
-        x8 = _matrix(x.device, x.shape[0], x.shape[1], 1)
+        x8 = _matrix(self.device, M, w.C, 1)
         self.keep.append(x8)
         self.pack(x, x8)
         if hidden is None:
@@ -258,7 +260,7 @@ def pack_fp8(x: torch.Tensor, rows: int = BLOCK, out: Optional[Fp8Blocks] = None
         raise ValueError(f"pack_fp8: rows is 1 or {BLOCK}, got {rows!r}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"pack_fp8: the last dimension must not be empty, got shape {tuple(x.shape)}")
-    x2 = _rows_of(x.detach())
+    x2 = _rows_of(x)
     if out is None:
         p = _matrix(x.device, x2.shape[0], x2.shape[1], rows, x.shape, x.dtype)
     else:
@@ -279,7 +281,7 @@ def unpack_fp8(p: Fp8Blocks, dtype: Optional[torch.dtype] = None) -> torch.Tenso
     dtype = p.dtype if dtype is None else dtype
     if dtype not in _FLOATS:
         raise TypeError(f"unpack_fp8: unsupported type {dtype}")
-    out = torch.empty(p.shape, dtype=dtype, device=p.device)
+    out = torch.empty(p.shape, dtype=dtype, device=p.data.device)
     run = _run_on(out)
     run.unpack(p, out)
     run.go()
@@ -372,7 +374,7 @@ def _linear_frozen(x, w8):
     return y
 
 
-def _check_activation(name: str, x, like=None) -> None:
+def _check_activation(name: str, x) -> None:
     if not isinstance(x, torch.Tensor) or x.dtype not in _FLOATS:
         raise TypeError(f"{name} takes a floating-point tensor, got {getattr(x, 'dtype', type(x).__name__)}")
     if x.is_cuda and x.dtype != torch.bfloat16:
@@ -383,7 +385,7 @@ def _check_activation(name: str, x, like=None) -> None:
 
 def _check_weight(name: str, w, x, n_in: int) -> bool:
     """Shape, type and device of a weight ``[out, in]``; True when it is packed."""
-    packed = isinstance(w, Fp8Blocks)
+    packed = type(w) is Fp8Blocks
     if packed:
         if w.rows != BLOCK or len(w.shape) != 2:
             raise ValueError(f"{name}: a packed weight is a matrix packed with rows={BLOCK}, got {w!r}")
@@ -391,9 +393,10 @@ def _check_weight(name: str, w, x, n_in: int) -> bool:
         raise TypeError(f"{name}: a weight is a floating-point matrix or a packed one, got {getattr(w, 'dtype', type(w).__name__)}")
     elif w.is_cuda and w.dtype != torch.bfloat16:
         raise TypeError(f"{name}: the 8-bit products take and return bfloat16 on CUDA, got a weight in {w.dtype}")
-    if len(w.shape) != 2 or w.shape[1] != n_in or 0 in w.shape:
-        raise ValueError(f"{name}: a weight [out, {n_in}] was expected, got {tuple(w.shape)}")
-    if w.device != x.device:
+    shape = w.shape
+    if len(shape) != 2 or shape[1] != n_in or not shape[0] or not n_in:
+        raise ValueError(f"{name}: a weight [out, {n_in}] was expected, got {tuple(shape)}")
+    if (w.data if packed else w).device != x.device:
         raise ValueError(f"{name}: input on {x.device}, weight on {w.device}")
     return packed
 
@@ -494,7 +497,7 @@ class _ChannelMixFrozen(torch.autograd.Function):
 def _channel_mix_frozen(x, k8, v8, residual):
     x2 = _rows_of(x)
     h8 = _matrix(x.device, x2.shape[0], k8.R, 1)
-    y = torch.empty(residual.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(residual.shape)
     run = _run_on(x)
     run.nt_frozen(x2, k8, None, h8)
     run.nt(h8, v8, _rows_of(y), _rows_of(residual))
@@ -514,9 +517,9 @@ def fp8_channel_mix_ffn(xk: torch.Tensor, w_key: Union[torch.Tensor, Fp8Blocks],
         raise ValueError(f"{name}: either both weights are packed or neither is")
     if not isinstance(residual, torch.Tensor) or residual.dtype != xk.dtype or residual.device != xk.device:
         raise TypeError(f"{name}: the residual must have the input's type and device")
-    if residual.shape != xk.shape[:-1] + (w_value.shape[0],):
-        raise ValueError(f"{name}: a residual of shape {tuple(xk.shape[:-1]) + (w_value.shape[0],)} was expected, got "
-                         f"{tuple(residual.shape)}")
+    want = (*xk.shape[:-1], w_value.shape[0])
+    if residual.shape != want:
+        raise ValueError(f"{name}: a residual of shape {want} was expected, got {tuple(residual.shape)}")
     if not residual.is_contiguous() and (residual.dim() != 2 or residual.stride(1) != 1 or residual.stride(0) < residual.shape[1]):
         residual = residual.contiguous()
     if not packed:
