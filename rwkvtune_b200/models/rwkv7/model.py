@@ -14,6 +14,7 @@ training with the state carried between chunks
 from __future__ import annotations
 
 import math
+import threading
 import weakref
 from typing import Any, Dict, List, Optional, Sequence, Tuple
 
@@ -58,6 +59,15 @@ def _decode_spec(layer: nn.Module, x: torch.Tensor, act: Optional[str] = None, r
 def _decoding(x: torch.Tensor) -> bool:
     """Few rows, no autograd, on the GPU: the grouped decode GEMM applies."""
     return x.is_cuda and not torch.is_grad_enabled() and x.numel() // x.shape[-1] <= 128
+
+
+_first_run = threading.local()      # .active: this thread is in the first run of a block that backward runs again
+
+
+def _training_pass() -> bool:
+    """True where a gradient is taken: under autograd, or in the first, untracked run of a recomputed block, which has to
+    be the same function as the second."""
+    return torch.is_grad_enabled() or getattr(_first_run, "active", False)
 
 
 def _weights_of(*layers) -> list:
@@ -327,11 +337,11 @@ class RWKV7ChannelMix(nn.Module):
     def forward(self, x, ln_w, ln_b, x_prev=None, want_state: bool = False):
         (xk,), last, x = ops.ln_shift_mix_unbound(x, ln_w, ln_b, self.x_k, x_prev)
         held = getattr(self, "_packed", None)
-        if held is not None and not torch.is_grad_enabled():
+        if held is not None and not _training_pass():
             if not self._weights_kept(held):
                 raise RuntimeError("the feed-forward weights have changed since pack_ffn(): call it again, or unpack_ffn()")
             return ops.fp8_channel_mix_ffn(xk, *held[1], x), (last if want_state else None)
-        if getattr(self.config, "ffn_precision", "bf16") == "fp8" and not _decoding(xk):
+        if getattr(self.config, "ffn_precision", "bf16") == "fp8" and (_training_pass() or not _decoding(xk)):
             if not self._plain():
                 raise RuntimeError("ffn_precision='fp8' needs plain feed-forward projections (no adapter, no ZeRO-3 panels)")
             return ops.fp8_channel_mix_ffn(xk, self.key.weight, self.value.weight, x), (last if want_state else None)
@@ -427,8 +437,13 @@ class _Recompute(torch.autograd.Function):
             ctx.packed = p.offset, p.R, p.C, p.rows, p.shape, p.dtype
             keep[0] = p.data
         ctx.save_for_backward(*keep)
-        with torch.no_grad():
-            outs = fn(block, *tensors)
+        outer = getattr(_first_run, "active", False)
+        _first_run.active = True
+        try:
+            with torch.no_grad():
+                outs = fn(block, *tensors)
+        finally:
+            _first_run.active = outer
         return tuple(outs)
 
     @staticmethod
@@ -453,6 +468,8 @@ def _has_active_dropout(block: nn.Module) -> bool:
 
 def _checkpoint_block(fn, block, *tensors):
     """Recompute-in-backward wrapper for one block (random-number state is only preserved by the library path)."""
+    if not torch.is_grad_enabled():      # nothing to recompute, nothing to keep
+        return fn(block, *tensors)
     bits = getattr(block.config, "grad_cp_bits", 16)
     if _has_active_dropout(block):
         if bits == 8:

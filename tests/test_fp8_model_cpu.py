@@ -208,3 +208,33 @@ def test_pipeline_switch():
 
     pipe = InferencePipeline(model=make(), device="cpu", tokenizer=object(), ffn_8bit=True)
     assert all(b.ffn._packed is not None for b in pipe.model.blocks)
+
+
+@pytest.mark.parametrize("precision", ["bf16", "fp8"])
+def test_training_a_packed_model_with_recomputed_blocks(precision):
+    """The first run of a recomputed block has no autograd either, but it belongs to a training pass: it takes the weights
+    that the second run takes, not their packed copy."""
+    ids, labels = batch()
+    want = grads(make(grad_cp=1, ffn_precision=precision), ids, labels)
+    got = grads(make(grad_cp=1, ffn_precision=precision).pack_ffn(), ids, labels)
+    once = grads(make(ffn_precision=precision).pack_ffn(), ids, labels)
+    for loss, gr in (got, once):
+        assert loss == want[0] and set(gr) == set(want[1]) and all(torch.equal(gr[n], want[1][n]) for n in gr)
+
+
+def test_checkpointed_passes_without_autograd_keep_nothing():
+    m, ids = make(grad_cp=1, grad_cp_bits=8).train(), batch()[0]
+    from rwkvtune_b200.models.rwkv7.model import _block_plain, _checkpoint_block
+
+    real, calls = ops.pack_fp8, []
+    x = torch.randn(1, 9, 64)
+    try:
+        ops.pack_fp8 = lambda *a, **k: calls.append(a) or real(*a, **k)
+        with torch.no_grad():
+            y, _ = _checkpoint_block(_block_plain, m.blocks[0], x, torch.zeros_like(x))
+    finally:
+        ops.pack_fp8 = real
+    with torch.no_grad():
+        assert not calls and torch.equal(y, _block_plain(m.blocks[0], x, torch.zeros_like(x))[0])
+        packed = m.eval().pack_ffn()(ids)                 # the flag of the first run does not outlive it
+        assert not torch.equal(packed, m.unpack_ffn()(ids))

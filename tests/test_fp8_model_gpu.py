@@ -140,3 +140,24 @@ def test_packed_and_plain_logits_are_near():
         plain = m(ids).float()
         packed = m.pack_ffn()(ids).float()
     assert (packed - plain).norm() < ((1 + 2 ** -4) ** 2 - 1) * 2 * plain.norm() and not torch.equal(packed, plain)
+
+
+def ffn_calls(monkeypatch):
+    """The calls of the 8-bit feed-forward half from here on: True for each one that gets packed weights."""
+    from rwkvtune_b200 import ops
+
+    calls, real = [], ops.fp8_channel_mix_ffn
+    monkeypatch.setattr(ops, "fp8_channel_mix_ffn", lambda *a: calls.append(type(a[1]) is ops.Fp8Blocks) or real(*a))
+    return calls
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_short_recomputed_batches_run_one_function(monkeypatch, packed):
+    """At most 128 tokens, where a pass without autograd would decode: both runs of a recomputed block take the same products."""
+    m = make(ffn_precision="fp8", grad_cp=1).train()
+    if packed:
+        m.pack_ffn()
+    calls = ffn_calls(monkeypatch)
+    ids, labels = (t[:, :40] for t in batch())
+    m.loss(ids, labels).backward()
+    assert calls == [False] * 4                # two blocks, each run twice, on the trainable weights
