@@ -341,7 +341,9 @@ class RWKV7ChannelMix(nn.Module):
             if not self._weights_kept(held):
                 raise RuntimeError("the feed-forward weights have changed since pack_ffn(): call it again, or unpack_ffn()")
             return ops.fp8_channel_mix_ffn(xk, *held[1], x), (last if want_state else None)
-        if getattr(self.config, "ffn_precision", "bf16") == "fp8" and (_training_pass() or not _decoding(xk)):
+        # Passes that carry states without autograd - prefill and decoding - keep the weights' own precision: the trainable
+        # form packs them in every call, and its tiles would tie a sequence's result to those beside it.
+        if getattr(self.config, "ffn_precision", "bf16") == "fp8" and (_training_pass() or not want_state):
             if not self._plain():
                 raise RuntimeError("ffn_precision='fp8' needs plain feed-forward projections (no adapter, no ZeRO-3 panels)")
             return ops.fp8_channel_mix_ffn(xk, self.key.weight, self.value.weight, x), (last if want_state else None)

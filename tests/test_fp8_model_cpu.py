@@ -238,3 +238,27 @@ def test_checkpointed_passes_without_autograd_keep_nothing():
         assert not calls and torch.equal(y, _block_plain(m.blocks[0], x, torch.zeros_like(x))[0])
         packed = m.eval().pack_ffn()(ids)                 # the flag of the first run does not outlive it
         assert not torch.equal(packed, m.unpack_ffn()(ids))
+
+
+def test_state_carrying_passes_without_autograd_keep_the_weights_precision():
+    """Prefill and decoding of a model that trains in 8 bits: the products of the 16-bit model, whatever the length; whole
+    sequences without a state run as in training."""
+    from rwkvtune_b200.inference import GRPOBatchGenerator
+
+    m, n, ids = make(ffn_precision="fp8").eval(), make().eval(), batch()[0]
+    with torch.no_grad():
+        states = [None, None]
+        for part in (ids[:, :30], ids[:, 30:31], ids[:, 31:32]):
+            (a, states[0]), (b, states[1]) = m.forward_with_state(part, states[0]), n.forward_with_state(part, states[1])
+            assert torch.equal(a, b)
+        assert not torch.equal(m(ids), n(ids))
+        rows = torch.randn(1, 40, 64)
+        (y,), (z,) = (model.blocks[0].ffn(rows, torch.ones(64), torch.zeros(64))[:1] for model in (m.train(), m.eval()))
+        assert torch.equal(y, z)
+    args = dict(input_ids=[[5, 6, 7]] * 3, max_new_tokens=6, num_generations=50, temperature=1.0, top_p=1.0, seed=3)
+    a, b = (GRPOBatchGenerator(x, None, torch.device("cpu"), eos_token_id=0).generate(**args)["completion_ids"] for x in (m, n))
+    assert torch.equal(a, b)
+    # with a state and autograd (training in chunks) the 8-bit products run
+    x = torch.randn(1, 5, 64, requires_grad=True)
+    outs = [model.blocks[0].ffn(x, torch.ones(64), torch.zeros(64), torch.zeros(1, 64), True)[0] for model in (m, n)]
+    assert not torch.equal(*outs)

@@ -161,3 +161,19 @@ def test_short_recomputed_batches_run_one_function(monkeypatch, packed):
     ids, labels = (t[:, :40] for t in batch())
     m.loss(ids, labels).backward()
     assert calls == [False] * 4                # two blocks, each run twice, on the trainable weights
+
+
+@pytest.mark.parametrize("paths", [64, 160])
+def test_rollouts_of_a_model_that_trains_in_8_bits(monkeypatch, paths):
+    """More sequences than the decode products take, and fewer: neither prefill nor decoding packs a weight, and the tokens
+    are those of the 16-bit model."""
+    from rwkvtune_b200.inference import GRPOBatchGenerator
+
+    m, outs = make(ffn_precision="fp8").eval(), []
+    calls = ffn_calls(monkeypatch)
+    for precision in ("fp8", "bf16"):
+        m.config.ffn_precision = precision
+        gen = GRPOBatchGenerator(m, None, torch.device("cuda", 0), eos_token_id=0, use_cuda_graph=False)
+        outs.append(gen.generate(input_ids=[list(range(1, 150)), [5, 6, 7]], max_new_tokens=4, num_generations=paths // 2, temperature=1.0,
+                                 top_p=1.0, seed=3)["completion_ids"].cpu())
+    assert not calls and torch.equal(*outs)
