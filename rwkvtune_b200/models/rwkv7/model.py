@@ -313,8 +313,9 @@ class RWKV7ChannelMix(nn.Module):
         return self.key.weight._version, self.value.weight._version, ops.param_epoch()
 
     def _weights_kept(self, held) -> bool:
-        """True while the weights are the parameters, and at the versions, that were packed."""
-        return held[0] == self._weights_stamp() and held[2]() is self.key.weight and held[3]() is self.value.weight
+        """True while the projections are still plain and their weights the parameters, at the versions, that were packed."""
+        return (self._plain() and held[0] == self._weights_stamp() and held[2]() is self.key.weight
+                and held[3]() is self.value.weight)
 
     def pack(self) -> None:
         """Hold key and value in 8 bits beside the weights; forward passes without autograd use those from now on.  Called
@@ -339,7 +340,9 @@ class RWKV7ChannelMix(nn.Module):
         held = getattr(self, "_packed", None)
         if held is not None and not _training_pass():
             if not self._weights_kept(held):
-                raise RuntimeError("the feed-forward weights have changed since pack_ffn(): call it again, or unpack_ffn()")
+                raise RuntimeError("the feed-forward weights have changed since pack_ffn(): call it again, or unpack_ffn()"
+                                   if self._plain() else
+                                   "the feed-forward projections were wrapped or sharded after pack_ffn(): unpack_ffn() first")
             return ops.fp8_channel_mix_ffn(xk, *held[1], x), (last if want_state else None)
         # Passes that carry states without autograd - prefill and decoding - keep the weights' own precision: the trainable
         # form packs them in every call, and its tiles would tie a sequence's result to those beside it.

@@ -262,3 +262,20 @@ def test_state_carrying_passes_without_autograd_keep_the_weights_precision():
     x = torch.randn(1, 5, 64, requires_grad=True)
     outs = [model.blocks[0].ffn(x, torch.ones(64), torch.zeros(64), torch.zeros(1, 64), True)[0] for model in (m, n)]
     assert not torch.equal(*outs)
+
+
+def test_adapters_and_shards_that_come_after_packing():
+    """A packed copy knows nothing of an adapter wrapped around the projections later, nor of panels: it is refused."""
+    m, ids = make().eval().pack_ffn(), batch()[0]
+    m = get_peft_model(m, LoraConfig(r=4, lora_alpha=8, target_modules=["ffn.key", "ffn.value"])).eval()
+    assert not m.blocks[0].ffn._plain()
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="unpack_ffn"):
+            m(ids)
+        for b in m.blocks:
+            b.ffn.unpack()
+        m(ids)
+        n = make().eval().pack_ffn()
+        n.blocks[0].ffn.key._sharded = object()
+        with pytest.raises(RuntimeError, match="unpack_ffn"):
+            n(ids)
