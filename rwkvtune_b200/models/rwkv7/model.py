@@ -310,7 +310,10 @@ class RWKV7ChannelMix(nn.Module):
         return all(type(m) is Linear and getattr(m, "_sharded", None) is None for m in (self.key, self.value))
 
     def _weights_stamp(self):
-        return self.key.weight._version, self.value.weight._version, ops.param_epoch()
+        """Changes with every write that can be seen: tensor operations count versions, ``.data = `` and moves change the
+        address, the optimiser kernels raise the epoch."""
+        k, v = self.key.weight, self.value.weight
+        return k._version, v._version, k.data_ptr(), v.data_ptr(), ops.param_epoch()
 
     def _weights_kept(self, held) -> bool:
         """True while the projections are still plain and their weights the parameters, at the versions, that were packed."""
@@ -558,8 +561,9 @@ class RWKV7Model(GenerationMixin, nn.Module):
     def pack_ffn(self) -> "RWKV7Model":
         """Hold every block's feed-forward weights in 8 bits as well (half their bf16 size again): passes without autograd -
         decoding, prefill, evaluation - then run those products in 8 bits.  A token's result does not depend on the batch
-        it is in.  Call it again after changing the weights (captured decode graphs then follow); a stale copy is refused
-        outside of replays."""
+        it is in.  Call it again after changing or moving the weights (captured decode graphs then follow); a stale copy is
+        refused outside of replays.  Writes into ``weight.data`` itself (``weight.data.mul_(2)``) leave no trace that could be
+        checked: write under ``torch.no_grad()``, or pack again."""
         for block in self.blocks:
             block.ffn.pack()
         return self

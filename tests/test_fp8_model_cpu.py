@@ -279,3 +279,17 @@ def test_adapters_and_shards_that_come_after_packing():
         n.blocks[0].ffn.key._sharded = object()
         with pytest.raises(RuntimeError, match="unpack_ffn"):
             n(ids)
+
+
+def test_weights_replaced_or_moved_after_packing():
+    """``weight.data = other`` (what moving and casting a model do as well) counts no version."""
+    for change in (lambda m: setattr(m.blocks[1].ffn.value.weight, "data", m.blocks[1].ffn.value.weight.data * 2),
+                   lambda m: m.to(torch.bfloat16)):
+        m, ids = make().eval().pack_ffn(), batch()[0]
+        with torch.no_grad():
+            m(ids)
+            change(m)
+            with pytest.raises(RuntimeError, match="pack_ffn"):
+                m(ids)
+            m.pack_ffn()
+            m(ids)

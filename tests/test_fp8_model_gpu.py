@@ -177,3 +177,12 @@ def test_rollouts_of_a_model_that_trains_in_8_bits(monkeypatch, paths):
         outs.append(gen.generate(input_ids=[list(range(1, 150)), [5, 6, 7]], max_new_tokens=4, num_generations=paths // 2, temperature=1.0,
                                  top_p=1.0, seed=3)["completion_ids"].cpu())
     assert not calls and torch.equal(*outs)
+
+
+def test_moving_a_packed_model_names_the_packing():
+    m, (ids, _) = make().cpu().eval().pack_ffn(), batch()
+    m.cuda()
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="pack_ffn"):
+            m(ids)
+        m.pack_ffn()(ids)
