@@ -231,7 +231,7 @@ class TrainEngine:
         by host-side launch cost (a few thousand launches per step); a replay issues them in one call.  Parameter
         gradients accumulate into the flat gradient buffer exactly as in eager mode.  Cached fp32 parameter copies
         are invalidated first so that their refresh kernels are part of the recording."""
-        ops.bump_param_epoch()
+        ops.bump_param_epoch(counted=True)
         torch.cuda.synchronize()
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
@@ -316,7 +316,7 @@ class TrainEngine:
                 self.opt.step(lr)
                 self.opt.zero_grad()
                 self.optimizer_steps += 1
-                ops.bump_param_epoch()
+                ops.bump_param_epoch(counted=True)
         return loss
 
     def backward_and_step(self, loss: torch.Tensor, lr: float) -> bool:
@@ -335,7 +335,7 @@ class TrainEngine:
                 self.opt.step(lr)
                 self.opt.zero_grad()
                 self.optimizer_steps += 1
-                ops.bump_param_epoch()
+                ops.bump_param_epoch(counted=True)
         return boundary
 
     def train_step_from_host(self, idx_cpu: torch.Tensor, labels_cpu: torch.Tensor, lr: float) -> float:

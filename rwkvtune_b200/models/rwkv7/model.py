@@ -311,9 +311,9 @@ class RWKV7ChannelMix(nn.Module):
 
     def _weights_stamp(self):
         """Changes with every write that can be seen: tensor operations count versions, ``.data = `` and moves change the
-        address, the optimiser kernels raise the epoch."""
+        address, the optimiser kernels count on the parameters that they own."""
         k, v = self.key.weight, self.value.weight
-        return k._version, v._version, k.data_ptr(), v.data_ptr(), ops.param_epoch()
+        return k._version, v._version, k.data_ptr(), v.data_ptr(), ops.param_writes(k), ops.param_writes(v)
 
     def _weights_kept(self, held) -> bool:
         """True while the projections are still plain and their weights the parameters, at the versions, that were packed."""

@@ -43,10 +43,23 @@ def param_epoch() -> int:
     return cuda_ops_epoch.EPOCH[0]
 
 
-def bump_param_epoch() -> None:
+def param_writes(p) -> tuple:
+    """Changes whenever ``p`` may have been rewritten through raw pointers: by the optimiser that owns it, or by a writer
+    that did not say whose parameters it wrote."""
+    from . import cuda_ops_epoch
+
+    owned = getattr(p, "flat_writes", None)
+    return cuda_ops_epoch.UNCOUNTED[0], owned[0] if owned is not None else -1
+
+
+def bump_param_epoch(counted: bool = False) -> None:
+    """Parameters were rewritten behind autograd's back.  ``counted``: the writer has counted that on its own parameters
+    (``FlatParamSpace.wrote``), so copies of other models' parameters stay valid."""
     from . import cuda_ops_epoch
 
     cuda_ops_epoch.EPOCH[0] += 1
+    if not counted:
+        cuda_ops_epoch.UNCOUNTED[0] += 1
     try:
         from . import cuda_ops
 

@@ -63,13 +63,19 @@ class FlatParamSpace:
         self.grads = alloc(self.padded, self.dtype, self.device)
         self.params.zero_()
         self.grads.zero_()
+        self.writes = [0]       # writes to the buffer, which the parameters' own version counters do not show
         with torch.no_grad():
             for seg, p in zip(self.segments, params):
                 view = self.params[seg.start:seg.start + seg.numel].view(seg.shape)
                 view.copy_(p.data)
                 p.data = view
+                p.flat_writes = self.writes
                 p.grad = self.grads[seg.start:seg.start + seg.numel].view(seg.shape)
         self._params_list = params
+
+    def wrote(self) -> None:
+        """The parameters' values have been rewritten in the flat buffer."""
+        self.writes[0] += 1
 
     def shard_range(self, rank: int) -> Tuple[int, int]:
         return rank * self.shard_numel, (rank + 1) * self.shard_numel

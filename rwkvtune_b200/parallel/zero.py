@@ -160,6 +160,7 @@ class ZeroOptimizer:
 
         ``grad_scale`` multiplies the summed gradient (``1 / accumulate_grad_batches`` when the loss
         was not pre-divided)."""
+        self.space.wrote()
         if self._p2p is not None:
             self._p2p.step(lr, grad_scale)
             return
@@ -190,6 +191,7 @@ class ZeroOptimizer:
         self.step_count = int(step)
         self.space.params[self.lo:self.hi].copy_(self.master)
         self._gather_params()
+        self.space.wrote()
 
 
 def merge_shards(shards: List[Dict[str, object]]):

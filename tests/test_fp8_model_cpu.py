@@ -293,3 +293,30 @@ def test_weights_replaced_or_moved_after_packing():
                 m(ids)
             m.pack_ffn()
             m(ids)
+
+
+def test_another_models_optimiser_leaves_a_packed_copy_valid():
+    """The engine's own model is refused after a step and after loading a state; a packed model beside it is not."""
+    ids, labels = batch()
+    beside = [make().eval().pack_ffn(), make().eval().requires_grad_(False).pack_ffn()]
+    eng = TrainEngine(make(), EngineConfig(lr_init=1e-3, precision="fp32"), DistContext())
+    own = eng.model.pack_ffn()
+    with torch.no_grad():
+        want = [m(ids) for m in beside]
+        own(ids)
+    eng.train_step(ids, labels, 1e-3)
+    with torch.no_grad():
+        assert all(torch.equal(m(ids), w) for m, w in zip(beside, want))
+        with pytest.raises(RuntimeError, match="pack_ffn"):
+            own(ids)
+        own.pack_ffn()(ids)
+        full = [torch.ones(eng.space.numel) for _ in range(3)]
+        eng.opt.load_full_state(*full, step=3)
+        with pytest.raises(RuntimeError, match="pack_ffn"):
+            own(ids)
+        assert torch.equal(beside[0](ids), want[0])
+        copied = copy.deepcopy(own).pack_ffn()                 # a copy belongs to no optimiser
+        kept = copied(ids)
+    eng.train_step(ids, labels, 1e-3)
+    with torch.no_grad():
+        assert torch.equal(copied(ids), kept)
