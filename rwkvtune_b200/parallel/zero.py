@@ -192,6 +192,9 @@ class ZeroOptimizer:
         self.space.params[self.lo:self.hi].copy_(self.master)
         self._gather_params()
         self.space.wrote()
+        from .. import ops
+
+        ops.bump_param_epoch(counted=True)      # cached copies of small parameters
 
 
 def merge_shards(shards: List[Dict[str, object]]):

@@ -178,3 +178,16 @@ def test_checkpoint_publication_replacement_rotation_and_lookup(tmp_path):
     assert ckpt.find_checkpoint(str(weights)) == str(weights)                  # a bare file is taken as it is
     assert ckpt.find_checkpoint(str(tmp_path / "nowhere")) is None and ckpt.find_checkpoint(None) is None
     assert ckpt.read_meta(str(tmp_path / "rwkv7-batch3")) == {}
+
+
+def test_loading_an_optimiser_state_reaches_cached_parameter_copies():
+    """The token-shift coefficients are cached for passes without autograd; a state loaded between two passes is followed."""
+    torch.manual_seed(0)
+    model = RWKV7Model(RWKVConfig(n_layer=2, n_embd=64, vocab_size=128, dim_att_lora=16, dim_gate_lora=16, dim_mv_lora=16))
+    eng = TrainEngine(model, EngineConfig(lr_init=1e-3, precision="fp32"), DistContext())
+    att = eng.model.blocks[1].att
+    with torch.no_grad():
+        assert torch.equal(att.mix_matrix()[0], att.x_r.reshape(-1))
+        master = eng.opt.master[:eng.space.numel].clone() + 1.0
+        eng.opt.load_full_state(master, torch.zeros_like(master), torch.zeros_like(master), step=1)
+        assert torch.equal(att.mix_matrix()[0], att.x_r.reshape(-1))
