@@ -90,7 +90,11 @@ class Fp8Blocks:
 
 
 def _matrix(device, R: int, C: int, rows: int, shape=None, dtype=torch.bfloat16) -> Fp8Blocks:
-    """An uninitialised packed matrix in a buffer of its own."""
+    """An uninitialised packed matrix in a buffer of its own.  An ordinary tensor under ``torch.inference_mode`` as well: a
+    packed weight is written again and kept for backward elsewhere."""
+    if torch.is_inference_mode_enabled():
+        with torch.inference_mode(False):
+            return _matrix(device, R, C, rows, shape, dtype)
     return Fp8Blocks(torch.empty(sum(_sizes(R, C, rows)), dtype=torch.uint8, device=device), 0, R, C, rows, shape, dtype)
 
 

@@ -300,3 +300,22 @@ def test_result_may_be_written_in_place(shape, frozen):
     assert torch.equal(z, y * 2 + 1)
     (got,) = torch.autograd.grad(z.sum(), [x])
     assert torch.equal(got, 2 * want)
+
+
+@pytest.mark.parametrize("again", [False, True])
+def test_packed_under_inference_mode(again):
+    """A weight packed for serving can be packed again and trained against outside of it, and the other way round."""
+    w, v, x = weights(16, 40), weights(16, 40, 5), sample(3, 40, torch.float32)
+    for rows in (1, 128):
+        with torch.inference_mode():
+            p = ops.pack_fp8(w, rows=rows)
+        with torch.inference_mode(again):
+            ops.pack_fp8(v, rows=rows, out=p)
+        assert torch.equal(ops.unpack_fp8(p), ops.unpack_fp8(ops.pack_fp8(v, rows=rows)))
+    a = x.clone().requires_grad_()
+    ops.fp8_linear(a, p).sum().backward()
+    b = x.clone().requires_grad_()
+    ops.fp8_linear(b, ops.pack_fp8(v)).sum().backward()
+    assert torch.equal(a.grad, b.grad)
+    with torch.inference_mode():
+        assert torch.equal(ops.fp8_linear(x, p), ops.fp8_linear(x, ops.pack_fp8(v)))
