@@ -25,6 +25,7 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _KERNELS
@@ -405,6 +406,13 @@ def _check_weight(name: str, w, x, n_in: int) -> bool:
     return packed
 
 
+def _differentiated(a, b=None) -> bool:
+    """True if autograd has to see the call: a gradient will be asked for, or a forward-mode level is open (whose tangents
+    are refused there; a plain call would drop them)."""
+    return ((torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad)))
+            or forward_ad._current_level >= 0)
+
+
 def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]) -> torch.Tensor:
     """``x @ weight^T`` as a product of 8-bit operands; ``weight [out, in]`` is a tensor (packed in the call, receives a
     gradient) or what :func:`pack_fp8` made of one (frozen: only ``x`` receives a gradient)."""
@@ -412,7 +420,7 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Blocks]) -> torch
     packed = _check_weight("fp8_linear", weight, x, x.shape[-1])
     if not packed:
         return _Linear.apply(x, weight)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _differentiated(x):
         return _LinearFrozen.apply(x, weight.data, weight)
     return _linear_frozen(x, weight)
 
@@ -528,6 +536,6 @@ def fp8_channel_mix_ffn(xk: torch.Tensor, w_key: Union[torch.Tensor, Fp8Blocks],
         residual = residual.contiguous()
     if not packed:
         return _ChannelMix.apply(xk, w_key, w_value, residual)
-    if torch.is_grad_enabled() and (xk.requires_grad or residual.requires_grad):
+    if _differentiated(xk, residual):
         return _ChannelMixFrozen.apply(xk, w_key.data, w_value.data, residual, w_key, w_value)
     return _channel_mix_frozen(xk, w_key, w_value, residual)[0]

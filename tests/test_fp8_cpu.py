@@ -319,3 +319,22 @@ def test_packed_under_inference_mode(again):
     assert torch.equal(a.grad, b.grad)
     with torch.inference_mode():
         assert torch.equal(ops.fp8_linear(x, p), ops.fp8_linear(x, ops.pack_fp8(v)))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_forward_mode_derivatives_are_refused(frozen, grad):
+    """No tangent is dropped in silence; tensors without one pass through an open level as they are."""
+    import torch.autograd.forward_ad as fwd
+
+    x, res, wk, wv = sample(4, 64, torch.float32), sample(4, 64, torch.float32, 2), weights(32, 64), weights(64, 32)
+    if frozen:
+        wk, wv = ops.pack_fp8(wk), ops.pack_fp8(wv)
+    want = ops.fp8_linear(x, wk), ops.fp8_channel_mix_ffn(x, wk, wv, res)
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        dual, dual_res = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(res, torch.ones_like(res))
+        for call in (lambda: ops.fp8_linear(dual, wk), lambda: ops.fp8_channel_mix_ffn(dual, wk, wv, res),
+                     lambda: ops.fp8_channel_mix_ffn(x, wk, wv, dual_res)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(ops.fp8_linear(x, wk), want[0]) and torch.equal(ops.fp8_channel_mix_ffn(x, wk, wv, res), want[1])
