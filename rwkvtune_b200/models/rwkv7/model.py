@@ -326,6 +326,9 @@ class RWKV7ChannelMix(nn.Module):
         if not self._plain():
             raise ValueError("8-bit feed-forward weights need plain projections (merge the adapter; no ZeRO-3 panels)")
         held, weights = getattr(self, "_packed", None), (self.key.weight, self.value.weight)
+        for w in weights:
+            if w.is_cuda and w.dtype != torch.bfloat16:
+                raise ValueError(f"8-bit feed-forward weights run beside a bfloat16 model on CUDA, this one is in {w.dtype}")
         again = held is not None and all(tuple(p.shape) == tuple(w.shape) and (p.dtype, p.device) == (w.dtype, w.device)
                                          for p, w in zip(held[1], weights))
         packed = tuple(ops.pack_fp8(w, out=p) for w, p in zip(weights, held[1] if again else (None, None)))

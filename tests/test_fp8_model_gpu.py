@@ -186,3 +186,14 @@ def test_moving_a_packed_model_names_the_packing():
         with pytest.raises(RuntimeError, match="pack_ffn"):
             m(ids)
         m.pack_ffn()(ids)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_packing_other_types_is_refused_at_once(dtype):
+    from rwkvtune_b200.inference.pipeline import InferencePipeline
+
+    m = make().to(dtype)
+    with pytest.raises(ValueError, match="bfloat16"):
+        m.pack_ffn()
+    with pytest.raises(ValueError, match="bfloat16"):
+        InferencePipeline(model=m, device="cuda", tokenizer=object(), ffn_8bit=True)
