@@ -43,14 +43,33 @@ __device__ __forceinline__ void rwkv_chain_begin() {
   rwkv_chain_trigger();
   rwkv_chain_wait();
 }
-inline int& rwkv_chain_flag() {
-  static int flag = 0;
-  return flag;
+//
+// A chain belongs to one host thread and one stream.  Its first launch is an ordinary one: a kernel before it may have
+// announced its dependents early while it still writes something that counts as constant from here on (the packing
+// kernels do, and may write weights), and chained launches only ever wait for their direct predecessor.  The same goes
+// for the launch after a kernel of the chain that may have written weights (rwkv_chain_restart).
+struct RwkvChain {
+  bool on, joined;              // joined: the last launch on `stream` belongs to the chain
+  cudaStream_t stream;
+};
+inline RwkvChain& rwkv_chain() {
+  static thread_local RwkvChain chain = {};
+  return chain;
 }
+// True if the launch that follows on `st` may be chained to its predecessor; it then is the chain's last launch.
+inline bool rwkv_chain_next(cudaStream_t st) {
+  RwkvChain& c = rwkv_chain();
+  if (!c.on) return false;
+  const bool joined = c.joined && c.stream == st;
+  c.joined = true;
+  c.stream = st;
+  return joined;
+}
+inline void rwkv_chain_restart() { rwkv_chain().joined = false; }
 template <typename... KArgs, typename... Args>
 static inline void rwkv_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                                Args... args) {
-  if (!rwkv_chain_flag()) {
+  if (!rwkv_chain_next(st)) {
     kernel<<<grid, block, smem, st>>>(args...);
     return;
   }

@@ -8,7 +8,8 @@
 //   rows = 128: a CTA of 512 threads walks over tiles with the next one's loads in flight; warp maxima meet in shared
 //               memory (one CTA a tile: 43.2 us, walking: 33.3 us, 6.06 TB/s).
 //
-// Launched through rwkv_launch: inside a chain of decode launches they are part of it.
+// Launched through rwkv_launch: inside a chain of decode launches they are part of it.  Tiles may be weights, which products of
+// the chain fetch before they wait: the launch after them is an ordinary one.
 //
 // Arithmetic in the rest of the library flushes numbers below 2^-126 to zero, and so do these kernels.
 #include <cuda_fp16.h>
@@ -348,6 +349,7 @@ int pack_tiles_v(const Fp8Step* s, int count, cudaStream_t st) {
     }
   }
   launch();
+  rwkv_chain_restart();
   return rwkv_launch_status();
 }
 template <typename T>

@@ -491,7 +491,7 @@ RWKV_EXPORT int rwkv_gemm_decode_tcgen05_traced(const void* const* xs, const voi
     attr[n_attr].val.clusterDim.z = split;
     ++n_attr;
   }
-  if (rwkv_chain_flag()) {
+  if (rwkv_chain_next(cfg.stream)) {
     attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
     ++n_attr;
@@ -510,9 +510,10 @@ RWKV_EXPORT int rwkv_gemm_decode_tcgen05(const void* const* xs, const void* cons
                                          prefetch_weights, status, stream, nullptr, nullptr, nullptr, 0);
 }
 
-// Chained launches for the kernels of the decode path (see common.cuh): 1 = on, 0 = off.  Returns the previous value.
+// Chained launches for the kernels of the decode path (see common.cuh), of the calling thread: 1 = on, 0 = off.  Returns the
+// previous value.
 RWKV_EXPORT int rwkv_set_launch_chaining(int on) {
-  const int prev = rwkv_chain_flag();
-  rwkv_chain_flag() = on ? 1 : 0;
+  const int prev = rwkv_chain().on;
+  rwkv_chain() = {on != 0, false, nullptr};
   return prev;
 }

@@ -603,7 +603,8 @@ int rwkv_fp8_decode(const Fp8Step& s, cudaStream_t st) {
   g.q_val = (uint8_t*)s.q_val; g.q_exp = (uint8_t*)s.q_exp;
   g.q_ldv = (N + 15) / 16 * 16; g.q_lde = (M + 15) / 16 * 16;
   g.status = (int*)s.status;
-  const int ch = s.chained;
+  const bool next = rwkv_chain_next(st);
+  const int ch = s.chained && (next || !rwkv_chain().on);      // in a chain: not its first launch
   if (packed) {
     if (s.epilogue == 2) return launch<true, EPI_RELU_SQ>(mw, mx, g, lay.smem, ch, st);
     return s.epilogue == 1 ? launch<true, EPI_RESIDUAL>(mw, mx, g, lay.smem, ch, st) : launch<true, EPI_STORE>(mw, mx, g, lay.smem, ch, st);

@@ -109,6 +109,7 @@ def launch_count() -> int:
 
 import contextlib as _contextlib
 import os as _os
+import threading as _threading
 
 
 # ------------------------------------------------------------------------------- graph capture hygiene
@@ -132,12 +133,17 @@ def capture_safe_gc():
 
 # ------------------------------------------------------------------------------- chained launches
 
-_CHAINING = False
+class _Chain(_threading.local):
+    on = False
+
+
+_CHAIN = _Chain()
 CHAINING_ALLOWED = _os.environ.get("RWKVTUNE_CHAINED_LAUNCH", "1") == "1"
 
 
 def chaining() -> bool:
-    return _CHAINING
+    """True inside :func:`launch_chaining`, in the thread that entered it."""
+    return _CHAIN.on
 
 
 @_contextlib.contextmanager
@@ -145,18 +151,18 @@ def launch_chaining():
     """Inside this context the kernels of the decode path are launched as a programmatic dependent chain: each may be
     scheduled while its predecessor still runs and waits on the device for it before touching activations (see
     ``csrc/common.cuh``).  The decode GEMM additionally streams its first weight tiles before that wait, so the
-    context must not enclose anything that writes model weights.  ``RWKVTUNE_CHAINED_LAUNCH=0`` turns it off."""
-    global _CHAINING
-    if not (CHAINING_ALLOWED and available() and hasattr(lib(), "rwkv_set_launch_chaining")) or _CHAINING:
+    context must not enclose anything that writes model weights (but for ``ops.pack_fp8``, whose launch the next one waits
+    for).  Other threads launch as before.  ``RWKVTUNE_CHAINED_LAUNCH=0`` turns it off."""
+    if not (CHAINING_ALLOWED and available() and hasattr(lib(), "rwkv_set_launch_chaining")) or _CHAIN.on:
         yield
         return
     lib().rwkv_set_launch_chaining(ctypes.c_int(1))
-    _CHAINING = True
+    _CHAIN.on = True
     try:
         yield
     finally:
         lib().rwkv_set_launch_chaining(ctypes.c_int(0))
-        _CHAINING = False
+        _CHAIN.on = False
 
 
 def i32(v: int) -> ctypes.c_int:

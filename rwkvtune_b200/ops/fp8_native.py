@@ -106,8 +106,9 @@ def decode_form(M: int, N: int, K: int, packed: bool = False) -> int:
 
 
 def chaining() -> bool:
-    """True inside a chain of decode launches, during which no kernel writes weights (``_ext.launch_chaining``)."""
-    return _ext._CHAINING
+    """True inside a chain of decode launches, during which no kernel writes weights but the packing ones, which the next
+    launch waits for (``_ext.launch_chaining``)."""
+    return _ext._CHAIN.on
 
 
 def decode_input(x: torch.Tensor) -> torch.Tensor:

@@ -509,3 +509,28 @@ def test_refusals_on_cuda():
         ops.fp8_linear(x.to(BF), ops.pack_fp8(w.cpu()))
     with pytest.raises(TypeError):
         ops.pack_fp8(x.double())
+
+
+@pytest.mark.parametrize("M", [1, 9, 40])
+def test_weights_packed_in_and_before_a_chain_of_decode_launches(M):
+    """Fresh weights every time, without a wait between packing and product: the first launch of a chain, and the one after a
+    packing launch inside it, wait for everything before them."""
+    from rwkvtune_b200.ops import _ext
+
+    x, res = sample(M, 512).cuda(), sample(M, 512, seed=3).cuda()
+    hold = ops.pack_fp8(weights(1024, 512).cuda()), ops.pack_fp8(weights(512, 1024).cuda())
+    fresh = [(weights(1024, 512, s).cuda(), weights(512, 1024, s + 50).cuda()) for s in range(8)]
+    want = [ops.fp8_channel_mix_ffn(x, ops.pack_fp8(k), ops.pack_fp8(v), res) for k, v in fresh]
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        got = []
+        for k, v in fresh:
+            ops.pack_fp8(k, out=hold[0]), ops.pack_fp8(v, out=hold[1])
+            with _ext.launch_chaining():
+                got.append(ops.fp8_channel_mix_ffn(x, *hold, res))
+        with _ext.launch_chaining():
+            for k, v in fresh:
+                ops.pack_fp8(k, out=hold[0]), ops.pack_fp8(v, out=hold[1])
+                got.append(ops.fp8_channel_mix_ffn(x, *hold, res))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want + want))
