@@ -18,7 +18,8 @@ Sums are formed in fp32 and rounded once.  The gradients are those of the produc
 counts as the identity.  Backward keeps ``P(x)``, ``h`` and the packed weights, one byte a value, and nothing in 16 bits.
 
 CUDA tensors run the kernels of ``csrc/fp8_blocks.cu``, ``csrc/gemm_fp8_tcgen05.cu`` and, for at most 128 rows against a
-frozen weight, ``csrc/gemm_fp8_decode.cu`` (bf16 activations; packing also takes fp16 and fp32).  CPU tensors of any of the three types run the same definitions in plain fp32.
+frozen weight, ``csrc/gemm_fp8_decode.cu`` (bf16 activations; packing also takes fp16 and fp32).  CPU tensors of any of the three types run
+the same definitions in plain fp32.  Numbers below 2^-126 count as zero, packed and read back, on both.
 """
 from __future__ import annotations
 

@@ -194,6 +194,11 @@ def fp8_exponents(largest: torch.Tensor) -> torch.Tensor:
     return torch.where(bits >= 0x7F800000, 255, e.clamp(min=0)).to(torch.uint8)
 
 
+def _fp8_flush(x: torch.Tensor) -> torch.Tensor:
+    """Magnitudes below 2^-126 (no normal fp32 numbers) become zero with their sign, as in the kernels' arithmetic."""
+    return torch.where(x.abs() < torch.finfo(torch.float32).tiny, x * 0, x)
+
+
 def _fp8_scale(exponents: torch.Tensor) -> torch.Tensor:
     return torch.ldexp(torch.ones_like(exponents, dtype=torch.float64), exponents.int() - 127)
 
@@ -201,9 +206,9 @@ def _fp8_scale(exponents: torch.Tensor) -> torch.Tensor:
 def fp8_pack(x: torch.Tensor, rows: int):
     """``(values float8_e4m3fn [R, C], exponents uint8 [ceil(R / rows), ceil(C / 128)])`` of a matrix, in blocks of ``rows``
     (1 or 128) by 128: ``x ~ values * 2^(exponents - 127)``, rounded to nearest even.  A block that holds an infinity or a
-    NaN becomes NaN."""
+    NaN becomes NaN; values below 2^-126 count as zero."""
     R, C = x.shape
-    padded = F.pad(x.float(), (0, -C % FP8_BLOCK, 0, -R % rows))
+    padded = F.pad(_fp8_flush(x.float()), (0, -C % FP8_BLOCK, 0, -R % rows))
     blocks = padded.unflatten(1, (-1, FP8_BLOCK)).unflatten(0, (-1, rows))             # [R / rows, rows, C / 128, 128]
     bits = (blocks.contiguous().view(torch.int32) & 0x7FFFFFFF).amax(dim=(1, 3))       # a NaN is larger than infinity here
     e = fp8_exponents(bits.view(torch.float32))
@@ -214,8 +219,8 @@ def fp8_pack(x: torch.Tensor, rows: int):
 
 def fp8_unpack(values: torch.Tensor, exponents: torch.Tensor, rows: int) -> torch.Tensor:
     """The fp32 values that a packed matrix stands for (finite inputs stay finite: a value that the rounding lifted above
-    the largest number is that number)."""
+    the largest number is that number; one below 2^-126 is zero)."""
     R, C = values.shape
     e = exponents.repeat_interleave(rows, 0)[:R].repeat_interleave(FP8_BLOCK, 1)[:, :C]
     top = torch.finfo(torch.float32).max
-    return (values.double() * _fp8_scale(e)).clamp(-top, top).float()
+    return _fp8_flush((values.double() * _fp8_scale(e)).clamp(-top, top)).float()

@@ -338,3 +338,18 @@ def test_forward_mode_derivatives_are_refused(frozen, grad):
             with pytest.raises(NotImplementedError):
                 call()
         assert torch.equal(ops.fp8_linear(x, wk), want[0]) and torch.equal(ops.fp8_channel_mix_ffn(x, wk, wv, res), want[1])
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_numbers_below_the_normal_ones_count_as_zero(dtype, rows):
+    low = 2.0 ** -126
+    x = torch.tensor([[low, -low, low / 2, -low / 2, low / 128, low * 1.5, 0.0]], dtype=dtype)
+    p = ops.pack_fp8(x, rows=rows)
+    assert p.exponents.item() == 0 and p.values.float().tolist() == [[2.0, -2.0, 0.0, 0.0, 0.0, 3.0, 0.0]]
+    assert torch.signbit(p.values.float()).tolist() == [[False, True, False, True, False, False, False]]
+    assert ops.unpack_fp8(p).tolist() == [[low, -low, 0.0, 0.0, 0.0, low * 1.5, 0.0]]
+    # small against the block's largest, above 2^-126 as they are and below it once rounded down
+    y = torch.tensor([[448 * 2.0 ** -126, 2.0 ** -126 * 1.0625, 2.0 ** -127 * 1.9]], dtype=torch.float32)
+    q = ops.pack_fp8(y, rows=rows)
+    assert q.exponents.item() == 1 and ops.unpack_fp8(q).tolist() == [[448 * 2.0 ** -126, 2.0 ** -126, 0.0]]

@@ -534,3 +534,18 @@ def test_weights_packed_in_and_before_a_chain_of_decode_launches(M):
                 got.append(ops.fp8_channel_mix_ffn(x, *hold, res))
     torch.cuda.synchronize()
     assert all(torch.equal(g, w) for g, w in zip(got, want + want))
+
+
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_pack_and_unpack_next_to_the_smallest_normal_numbers(dtype, rows):
+    """Blocks whose values lie around 2^-126: the CPU statement, bit for bit, signs of zeros included."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(140, 400, generator=g) * torch.exp2(torch.randint(-12, 12, (140, 400), generator=g).float())
+    x = (x * 2.0 ** -100 * 2.0 ** -27).to(dtype)
+    x[128:, 128:256] = (torch.randn(12, 128, generator=g) * 2.0 ** -100 * 2.0 ** -30).clamp(-2.0 ** -127, 2.0 ** -127).to(dtype)
+    p = ops.pack_fp8(x.cuda(), rows=rows)
+    same_bits(p, x, rows)
+    for out in (BF, torch.float32):
+        got, want = ops.unpack_fp8(p, out).cpu(), ops.unpack_fp8(p.to("cpu"), out)
+        assert torch.equal(got, want) and torch.equal(torch.signbit(got), torch.signbit(want))
