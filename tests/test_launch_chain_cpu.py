@@ -1,4 +1,4 @@
-"""Chains of dependent launches belong to the thread that opened them (host side, no GPU)."""
+"""Host side of the launches, no GPU: chains of dependent launches belong to the thread that opened them; size caches."""
 import threading
 
 import pytest
@@ -59,3 +59,27 @@ def test_the_library_keeps_a_chain_per_thread():
         assert in_thread(lambda: (switch(0), switch(1), switch(0))) == (0, 0, 1)
     finally:
         assert switch(0) == 1
+
+
+def test_size_caches_are_bounded(monkeypatch):
+    """What is remembered by size does not grow with every new length of a batch; more than 128 rows are not remembered."""
+    class Sizes:
+        def __init__(self):
+            self.rwkv_fp8_workspace = lambda m, n, k: m
+
+        def rwkv_fp8_decode_form(self, m, n, k, packed):
+            return 1
+
+    monkeypatch.setattr(_ext, "lib", lambda fake=Sizes(): fake)
+    caches = [fp8_native._workspace_bytes, fp8_native._decode_form]
+    for c in caches:
+        c.cache_clear()
+    try:
+        for m in range(1, 9000):
+            assert fp8_native._workspace_bytes(m, 64, 64) == m
+            assert fp8_native.decode_form(m, 64, 64) == (1 if m <= 128 else 0)
+        assert all(c.cache_info().maxsize is not None and c.cache_info().currsize <= 4096 for c in caches)
+        assert fp8_native._decode_form.cache_info().currsize == 128
+    finally:
+        for c in caches:
+            c.cache_clear()
