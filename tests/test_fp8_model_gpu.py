@@ -197,3 +197,107 @@ def test_packing_other_types_is_refused_at_once(dtype):
         m.pack_ffn()
     with pytest.raises(ValueError, match="bfloat16"):
         InferencePipeline(model=m, device="cuda", tokenizer=object(), ffn_8bit=True)
+
+
+# ------------------------------------------------------------------------------- which kernels run
+FORWARD = ["pack"] * 3 + ["relu_sq", "residual"]
+BACKWARD = ["pack", "relu_sq_grad", "nn", "tn", "tn"]
+
+
+def launched(monkeypatch):
+    """Names of the 8-bit launches from here on, read from the records that go to the library."""
+    import struct
+
+    from rwkvtune_b200.ops import fp8_native
+
+    names, real = [], fp8_native.run
+
+    def name(record):
+        kind, _, _, _, a_rows, q_rows, _, a_mn, b_mn, epilogue = struct.unpack("=10i", record[:40])
+        if kind == 0:
+            return "pack" if q_rows == 128 else "pack rows"
+        if kind == 1:
+            return "unpack rows" if a_rows == 1 else "unpack"
+        product = ["tn" if a_mn else "nn" if b_mn else "nt", "residual", "relu_sq", "relu_sq_grad"][epilogue]
+        return product if kind == 2 else "decode " + product
+
+    monkeypatch.setattr(fp8_native, "run", lambda device, steps: names.extend(map(name, steps)) or real(device, steps))
+    return names
+
+
+def test_training_pass_launches_exactly_the_8_bit_products(monkeypatch):
+    m, names = make(), launched(monkeypatch)
+    l16, g16 = run(m)
+    assert names == []
+    l8, g8 = run(m, ffn_precision="fp8")
+    assert sorted(names) == sorted(2 * (FORWARD + BACKWARD)) and names[:10] == 2 * FORWARD
+    assert l8 != l16
+    for i in (0, 1):
+        for half in ("key", "value"):
+            n = f"blocks.{i}.ffn.{half}.weight"
+            assert not torch.equal(g8[n], g16[n])
+    del names[:]
+    run(m, ffn_precision="fp8", grad_cp=1, grad_cp_bits=8)      # each block's forward pass twice, its input packed in between
+    assert sorted(names) == sorted(2 * (["pack rows"] + FORWARD + ["unpack rows"] + FORWARD + BACKWARD))
+    del names[:]
+    run(m, grad_cp=1, grad_cp_bits=8)
+    assert sorted(names) == sorted(2 * ["pack rows", "unpack rows"])
+
+
+def test_gradients_of_a_block_inside_the_model(monkeypatch):
+    """What the feed-forward weights of a training step receive, against 64-bit products of the operands that the block saw."""
+    from rwkvtune_b200 import ops
+    from test_fp8_gpu import near, packed_product, values64
+
+    m, seen, real = make(ffn_precision="fp8").train(), [], ops.fp8_channel_mix_ffn
+
+    def recorded(xk, wk, wv, res):
+        y = real(xk, wk, wv, res)
+        entry = {"x": xk.detach().clone(), "res": res.detach().clone(), "y": y.detach().clone()}
+        y.register_hook(lambda g: entry.__setitem__("dy", g.clone()))
+        seen.append(entry)
+        return y
+
+    monkeypatch.setattr(ops, "fp8_channel_mix_ffn", recorded)
+    m.loss(*batch()).backward()
+    assert len(seen) == 2
+    for block, s in zip(m.blocks, seen):
+        wk, wv = block.ffn.key.weight, block.ffn.value.weight
+        x, res, y, dy = (s[k].reshape(-1, s[k].shape[-1]) for k in ("x", "res", "y", "dy"))
+        x8, k8, v8, d8 = (ops.pack_fp8(t.detach()) for t in (x, wk, wv, dy))
+        M, H = x.shape[0], wk.shape[0]
+        h8 = packed_product("nt_relu_sq", x8, k8, M, H, 128)
+        p8 = packed_product("nn_relu_sq_grad", d8, v8, M, H, 128, h8)
+        X, V, D, Hd, P = (values64(t) for t in (x8, v8, d8, h8, p8))
+        near(y, res.double() + Hd @ V.t(), Hd.abs() @ V.abs().t() + res.double().abs(), H)
+        near(wk.grad, P.t() @ X, P.abs().t() @ X.abs(), M)
+        near(wv.grad, D.t() @ Hd, D.abs().t() @ Hd.abs(), M)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_engine_steps_launch_the_8_bit_products(monkeypatch, graph):
+    """Per step, eager or recorded into a graph: the launches of two recomputed blocks; and losses that are not bf16's."""
+    names, losses = launched(monkeypatch), {}
+    for precision in ("bf16", "fp8"):
+        eng = TrainEngine(make(), EngineConfig(lr_init=1e-3, precision="bf16", grad_cp=1, ffn_precision=precision, cuda_graph=graph),
+                          DistContext(device=torch.device("cuda", 0)))
+        ids, labels = batch()
+        losses[precision] = [float(eng.train_step(ids, labels, 1e-3)) for _ in range(4)]
+        # a graph is recorded in the third step and replayed in the third and the fourth
+        passes = (0 if precision == "bf16" else eng.GRAPH_WARMUP_STEPS + 1 if graph else 4)
+        assert sorted(names) == sorted(passes * 2 * (2 * FORWARD + BACKWARD))
+        del names[:]
+    assert all(a != b for a, b in zip(losses["bf16"], losses["fp8"]))
+
+
+def test_packed_decode_steps_launch_the_decode_products(monkeypatch):
+    from rwkvtune_b200.inference import GRPOBatchGenerator
+
+    m = make().eval().pack_ffn()
+    names = launched(monkeypatch)
+    gen = GRPOBatchGenerator(m, None, torch.device("cuda", 0), eos_token_id=0, use_cuda_graph=False)
+    gen.eos_ids = []
+    gen.generate(input_ids=[list(range(1, 150))], max_new_tokens=3, num_generations=12, temperature=1.0, top_p=1.0, seed=3)
+    # 149 prompt tokens of one sequence, then two or three steps of twelve rows
+    assert names[:6] == 2 * ["pack rows", "relu_sq", "residual"]
+    assert len(names) > 6 and names[6:] == len(names[6:]) // 2 * ["decode relu_sq", "decode residual"]
