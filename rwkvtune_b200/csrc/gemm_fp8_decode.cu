@@ -5,7 +5,7 @@
 // accumulator's lanes are full whatever M is; a column block of 128 weights is one CTA's and its contraction is cut over a
 // cluster of S CTAs.  Token m of the sum belongs to CTA m % S: the others write their partial rows into its shared memory,
 // and after one cluster barrier it adds them in a fixed order.  S depends on N and K alone, so a row's result does not
-// depend on how many others there are.
+// depend on how many others there are (of these 128; larger batches run the pair kernel, with other sums).
 //
 // The tokens come either in bf16 - then each CTA packs its part of the contraction itself, row by row, into the
 // shared-memory tiles the tensor core reads, which saves a launch and a round trip - or already packed, fetched by TMA in

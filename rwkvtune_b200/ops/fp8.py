@@ -5,7 +5,10 @@ A matrix is held as e4m3 values with a power-of-two scale for each block (:class
 * tiles of 128 x 128 (``rows=128``): the scale is the same along both directions, so one packed copy is the operand of a
   product over the columns and of one over the rows.  Trainable weights use it for all three of their products.
 * 128 columns of one row (``rows=1``): what a token is stored as depends on that token alone.  Products with a frozen,
-  packed weight use it, so a sequence's result does not depend on what else is in the batch.
+  packed weight use it.  A token's result is then the same bit for bit in batches that run in the same way: those of at most
+  128 rows, and larger ones whose contraction is cut into the same number of slices (it depends on the number of rows).
+  Elsewhere the fp32 sums are taken in another order, which may round a result to its neighbour, and in the feed-forward
+  half a hidden value to the next 8-bit one.
 
 With ``P`` for packing, ``x [M, K]``, ``W [N, K]``::
 

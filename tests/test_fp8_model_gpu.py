@@ -301,3 +301,28 @@ def test_packed_decode_steps_launch_the_decode_products(monkeypatch):
     # 149 prompt tokens of one sequence, then two or three steps of twelve rows
     assert names[:6] == 2 * ["pack rows", "relu_sq", "residual"]
     assert len(names) > 6 and names[6:] == len(names[6:]) // 2 * ["decode relu_sq", "decode residual"]
+
+
+# ------------------------------------------------------------------------------- a token and its batch
+def test_what_a_tokens_result_depends_on():
+    """The 8-bit form of a token is its own; its sums are those of a dispatch form: at most 128 rows, more of them, and among
+    those each number of slices of the contraction.  Within a form a row's bits stay, between forms they agree to the last
+    places of an fp32 sum."""
+    from rwkvtune_b200 import ops
+    from rwkvtune_b200.ops import fp8_native
+    from test_fp8_gpu import near, sample, values64, weights
+
+    N, K = 1024, 8192
+    w8, x = ops.pack_fp8(weights(N, K).cuda()), sample(1300, K).cuda()
+    rows = (20, 128, 256, 300, 600, 1300)
+    slices = {m: fp8_native._workspace_bytes(m, N, K) // (-(-m // 128) * 128 * N * 4) for m in rows[2:]}
+    assert slices[256] == slices[300] and len(set(slices.values())) > 1
+    full = ops.pack_fp8(x, rows=1)
+    W, X = values64(w8), values64(full)
+    out = {}
+    for m in rows:
+        p = ops.pack_fp8(x[:m], rows=1)
+        assert torch.equal(p.values.view(torch.uint8), full.values[:m].view(torch.uint8)) and torch.equal(p.exponents, full.exponents[:m])
+        out[m] = ops.fp8_linear(x[:m], w8)
+        near(out[m], X[:m] @ W.t(), X[:m].abs() @ W.abs().t(), K)
+    assert torch.equal(out[20], out[128][:20]) and torch.equal(out[256], out[300][:256])
