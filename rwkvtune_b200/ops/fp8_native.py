@@ -98,15 +98,11 @@ def mm_nn_relu_sq_grad(a, b, h, q) -> bytes:
     return _product(a, b, a.R, b.C, a.C, 0, 1, _RELU_SQ_GRAD, h=h, q=q)
 
 
+@functools.lru_cache(maxsize=4096)
 def decode_form(M: int, N: int, K: int, packed: bool = False) -> int:
     """How ``x [M, K]`` times a packed ``[N, K]`` weight is run while decoding: 0 not, 1 on packed tokens, 2 on bf16 tokens
     that the kernel packs itself (see ``csrc/gemm_fp8_decode.cu``)."""
-    return _decode_form(M, N, K, packed) if M <= 128 else 0
-
-
-@functools.lru_cache(maxsize=4096)
-def _decode_form(M: int, N: int, K: int, packed: bool) -> int:
-    return _ext.lib().rwkv_fp8_decode_form(M, N, K, int(packed))
+    return _ext.lib().rwkv_fp8_decode_form(M, N, K, int(packed)) if M <= 128 else 0
 
 
 def chaining() -> bool:

@@ -62,7 +62,7 @@ def test_the_library_keeps_a_chain_per_thread():
 
 
 def test_size_caches_are_bounded(monkeypatch):
-    """What is remembered by size does not grow with every new length of a batch; more than 128 rows are not remembered."""
+    """What is remembered by size does not grow with every new length of a batch."""
     class Sizes:
         def __init__(self):
             self.rwkv_fp8_workspace = lambda m, n, k: m
@@ -71,7 +71,7 @@ def test_size_caches_are_bounded(monkeypatch):
             return 1
 
     monkeypatch.setattr(_ext, "lib", lambda fake=Sizes(): fake)
-    caches = [fp8_native._workspace_bytes, fp8_native._decode_form]
+    caches = [fp8_native._workspace_bytes, fp8_native.decode_form]
     for c in caches:
         c.cache_clear()
     try:
@@ -79,7 +79,6 @@ def test_size_caches_are_bounded(monkeypatch):
             assert fp8_native._workspace_bytes(m, 64, 64) == m
             assert fp8_native.decode_form(m, 64, 64) == (1 if m <= 128 else 0)
         assert all(c.cache_info().maxsize is not None and c.cache_info().currsize <= 4096 for c in caches)
-        assert fp8_native._decode_form.cache_info().currsize == 128
     finally:
         for c in caches:
             c.cache_clear()
