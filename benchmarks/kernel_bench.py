@@ -273,13 +273,77 @@ def bench_fp8(B, T, C, out, hbm, tf):
         ms = timeit(fn)
         out[f"fp8_{tag}_us"] = ms * 1e3
         out[f"fp8_{tag}_tflops_over_bf16_peak"] = 2 * M * C * H / ms / 1e9 / tf
-    for n in (1, 64):
-        xs, head = rnd(n, C), ops.pack_fp8(rnd(65536, C))
+    del x8, h8, p8, y, dk
+    # decoding: a step's weights come from HBM (each replay cycles through more of them than L2 holds); "in_l2" repeats one pair
+    layers = int(256e6 // (2 * H * C)) + 2
+    pairs = [(ops.pack_fp8(rnd(H, C)), ops.pack_fp8(rnd(C, H))) for _ in range(layers)]
+    squares = [ops.pack_fp8(rnd(C, C)) for _ in range(int(256e6 // (C * C)) + 2)]
+    heads = [ops.pack_fp8(rnd(65536, C)) for _ in range(2)]
+    with torch.no_grad():
+        for n in (1, 16, 64):
+            xs = rnd(n, C)
+            for tag, ws, nbytes in (("square", squares, C * C), ("head", heads, 65536 * C)):
+                ms = _graph_time(lambda: [ops.fp8_linear(xs, w) for w in ws]) / len(ws)
+                out[f"fp8_{tag}_{n}rows_us"] = ms * 1e3
+                out[f"fp8_{tag}_{n}rows_frac_hbm"] = nbytes / ms / 1e6 / hbm
+            for tag, held in (("", pairs), ("_in_l2", pairs[:1] * layers)):
+                ms = _graph_time(lambda: [ops.fp8_channel_mix_ffn(xs, k, v, xs) for k, v in held]) / layers
+                out[f"fp8_ffn_{n}rows{tag}_us"] = ms * 1e3
+                out[f"fp8_ffn_{n}rows{tag}_frac_hbm"] = 2 * H * C / ms / 1e6 / hbm
+
+
+def bench_fp8_ffn(C, out):
+    """The feed-forward half of a block as the model runs it (LayerNorm and token shift included), in bf16 and in 8 bits:
+    decode steps as a chain over more layers than L2 holds, prompts, and training passes of several sizes."""
+    import contextlib
+
+    from rwkvtune_b200.models import RWKVConfig
+    from rwkvtune_b200.models.rwkv7.model import RWKV7ChannelMix
+    from rwkvtune_b200.ops import _ext
+
+    cfg = RWKVConfig(n_layer=24, n_embd=C, vocab_size=65536, dim_ffn=4 * C)
+    layers = int(256e6 // (8 * C * C)) + 2
+    with torch.device("cuda"):
+        mods = [RWKV7ChannelMix(cfg, 1).to(BF) for _ in range(layers)]
+        ln_w, ln_b = (torch.nn.Parameter(t.to(BF)) for t in (torch.ones(C), torch.zeros(C)))
+    for m in mods:
+        torch.nn.init.uniform_(m.value.weight, -0.01, 0.01)
+
+    def walk(x, prev, chained):
+        with _ext.launch_chaining() if chained else contextlib.nullcontext():
+            for m in mods:
+                x = m(x, ln_w, ln_b, prev, prev is not None)[0]
+        return x
+
+    for tag in ("bf16", "8bit"):
+        if tag == "8bit":
+            for m in mods:
+                m.pack()
         with torch.no_grad():
-            ms = _graph_time(lambda: ops.fp8_linear(xs, head))
-            out[f"fp8_head_{n}rows_us"] = ms * 1e3
-            out[f"fp8_head_{n}rows_frac_hbm"] = 65536 * C / ms / 1e6 / hbm
-            out[f"fp8_ffn_{n}rows_us"] = _graph_time(lambda: ops.fp8_channel_mix_ffn(xs, k8, v8, xs)) * 1e3
+            for n in (1, 8, 16, 64, 128):
+                x, prev = torch.randn(n, 1, C, device="cuda").to(BF), torch.randn(n, C, device="cuda").to(BF)
+                out[f"ffn_decode_{n}rows_{tag}_us"] = _graph_time(lambda: walk(x, prev, True)) / layers * 1e3
+            for n in (512, 2048, 8192):
+                x, prev = torch.randn(1, n, C, device="cuda").to(BF), torch.randn(1, C, device="cuda").to(BF)
+                out[f"ffn_prompt_{n}tokens_{tag}_us"] = _graph_time(lambda: walk(x, prev, False)) / layers * 1e3
+    m = mods[0]
+    for n in (512, 1024, 2048, 4096, 8192, 32768):
+        x = torch.randn(1, n, C, device="cuda").to(BF).requires_grad_()
+        dy = torch.randn(1, n, C, device="cuda").to(BF)
+        for tag, cfg.ffn_precision in (("bf16", "bf16"), ("8bit", "fp8")):
+            def step():
+                torch.autograd.grad(m(x, ln_w, ln_b)[0], [x, *m.parameters()], dy)
+            ms = timeit(step, iters=30)          # eager: the host is part of a short training pass
+            out[f"ffn_train_{n}tokens_{tag}_us"] = ms * 1e3
+            side = torch.cuda.Stream()
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with _ext.capture_safe_gc(), torch.cuda.graph(g):
+                step()
+            out[f"ffn_train_{n}tokens_{tag}_captured_us"] = timeit(g.replay) * 1e3
+            del g
 
 
 def main():
@@ -307,6 +371,8 @@ def main():
         bench_decode_core(a.C, out, hbm)
     if not only or "fp8" in only:
         bench_fp8(a.B, a.T, a.C, out, hbm, tf)
+    if not only or "fp8_ffn" in only:
+        bench_fp8_ffn(a.C, out)
     for k, v in out.items():
         print(f"{k}: {v:.4g}" if isinstance(v, float) else f"{k}: {v}")
     if a.json:

@@ -1,7 +1,7 @@
 """GRPO rollout throughput: prompts x generations decoded in lock-step (by default the 1.5B model, 8 prompts of 512
 tokens x 8 generations x 512 new tokens).
 
-    python benchmarks/rollout_bench.py [--model 1.5b] [--prompts 8] [--prompt-len 512] [--generations 8] [--new-tokens 512]
+    python benchmarks/rollout_bench.py [--model 1.5b] [--prompts 8] [--prompt-len 512] [--generations 8] [--new-tokens 512] [--ffn-8bit]
 
 Random-init weights, uniform-random prompt tokens, temperature 1.0, top-p 0.95.  EOS is disabled so every path
 decodes exactly ``new-tokens`` tokens; reports generated tokens per second (device-synchronised wall time).
@@ -36,6 +36,7 @@ def main():
                                                         "(all layers + head + sampler) to this markdown file")
     ap.add_argument("--repetition-penalty", type=float, default=1.0)
     ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--ffn-8bit", action="store_true", help="decode on packed feed-forward weights (RWKV7Model.pack_ffn)")
     a = ap.parse_args()
     dev = torch.device("cuda", 0)
     torch.manual_seed(0)
@@ -43,6 +44,11 @@ def main():
     with torch.device(dev):
         model = RWKV7Model(cfg)
     model = model.to(torch.bfloat16).eval()
+    if a.ffn_8bit:
+        with torch.no_grad():      # the value projections start at zero: give them values like the others'
+            for b in model.blocks:
+                b.ffn.value.weight.uniform_(-0.01, 0.01)
+        model.pack_ffn()
     gen = GRPOBatchGenerator(model, None, dev, eos_token_id=None, use_cuda_graph=not a.no_graph)
     gen.eos_ids = []
     g = torch.Generator().manual_seed(1)
@@ -58,7 +64,8 @@ def main():
     tokens = int(out["lengths"].sum())
     print(json.dumps({"metric": "rollout_tokens_per_sec", "value": tokens / dt, "seconds": dt, "generated_tokens": tokens,
                       "paths": a.prompts * a.generations, "prefill_s": gen.last_stats["prefill_s"],
-                      "decode_s": gen.last_stats["decode_s"], "cuda_graph": not a.no_graph, "model": a.model}))
+                      "decode_s": gen.last_stats["decode_s"], "cuda_graph": not a.no_graph, "model": a.model,
+                      "ffn_8bit": a.ffn_8bit}))
     if a.profile_step:
         profile_decode_step(gen, a.prompts * a.generations, a.profile_step)
 

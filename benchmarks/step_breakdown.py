@@ -1,6 +1,7 @@
 """Where one training step spends its device time, kernel family by kernel family.
 
-    python benchmarks/step_breakdown.py [--layers 4] [--model 1.5b] [--B 8 --T 4096] [--md out.md] [--json out.json]
+    python benchmarks/step_breakdown.py [--layers 4] [--model 1.5b] [--B 8 --T 4096] [--ffn-precision fp8] [--grad-cp 1 --grad-cp-bits 8]
+        [--md out.md] [--json out.json]
 
 Builds a model of the named width with ``--layers`` blocks (a few blocks are enough: every block
 launches the same kernels), runs warm-up steps, then records ``--steps`` optimiser steps with
@@ -30,6 +31,8 @@ sys.path.insert(0, ROOT)
 FAMILIES = [
     ("gemm (tcgen05)", r"gemm_tcgen05|splitk_reduce"),
     ("gemm (decode)", r"gemm_decode"),
+    ("gemm (8-bit)", r"gemm_fp8|fp8_sum_slices|fp8_decode"),
+    ("8-bit packing", r"fp8_pack|fp8_unpack"),
     ("gemm (library)", r"nvjet|cutlass|cublas|gemm|xmma|sm100_|sm90_"),
     ("wkv7 prep", r"wkv7_tc_prep"),
     ("wkv7 scan fwd", r"wkv7_tc_scan"),
@@ -67,6 +70,9 @@ def main():
     ap.add_argument("--T", type=int, default=4096)
     ap.add_argument("--steps", type=int, default=2)
     ap.add_argument("--warmup", type=int, default=3)
+    ap.add_argument("--grad-cp", type=int, default=0)
+    ap.add_argument("--ffn-precision", default="bf16", choices=["bf16", "fp8"])
+    ap.add_argument("--grad-cp-bits", type=int, default=16, choices=[8, 16])
     ap.add_argument("--md", default="")
     ap.add_argument("--json", default="")
     a = ap.parse_args()
@@ -85,7 +91,8 @@ def main():
     torch.manual_seed(1)
     with torch.device(dev):
         model = RWKV7Model(cfg)
-    eng = TrainEngine(model, EngineConfig(lr_init=3e-4, weight_decay=0.01, grad_clip=1.0, precision="bf16", grad_cp=0),
+    eng = TrainEngine(model, EngineConfig(lr_init=3e-4, weight_decay=0.01, grad_clip=1.0, precision="bf16", grad_cp=a.grad_cp,
+                                           ffn_precision=a.ffn_precision, grad_cp_bits=a.grad_cp_bits),
                       DistContext(device=dev))
     ids = torch.randint(0, 65536, (a.B, a.T), device=dev)
     lab = torch.randint(0, 65536, (a.B, a.T), device=dev)
@@ -121,7 +128,8 @@ def main():
         fam[f][0] += ms
         fam[f][1] += n // a.steps
     total = sum(v[0] for v in fam.values())
-    lines = [f"model width {a.model}, {a.layers} of {full_layers} blocks, B={a.B}, T={a.T}; "
+    lines = [f"model width {a.model}, {a.layers} of {full_layers} blocks, B={a.B}, T={a.T}, feed-forward {a.ffn_precision}, "
+             f"grad_cp {a.grad_cp} ({a.grad_cp_bits} bits); "
              f"step {step_ms:.2f} ms by CUDA events (no profiler), kernel time under the profiler {total:.2f} ms",
              "", "| family | ms per step | launches | share |", "|---|---|---|---|"]
     for f, (ms, n) in sorted(fam.items(), key=lambda kv: -kv[1][0]):
