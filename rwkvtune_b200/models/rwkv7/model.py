@@ -180,12 +180,18 @@ class RWKV7TimeMix(nn.Module):
 
     def mix_matrix(self) -> torch.Tensor:
         C = self.x_r.shape[-1]
-        if not torch.is_grad_enabled():   # inference: one cached [6, C] parameter-like tensor, rebuilt when weights change
+        if not torch.is_grad_enabled():   # inference: one cached [6, C] parameter-like tensor, refreshed when weights change
             key = tuple(p._version for p in (self.x_r, self.x_w, self.x_k, self.x_v, self.x_a, self.x_g)) + (ops.param_epoch(),)
             cached = getattr(self, "_mix_cache", None)
             if cached is None or cached[0] != key or cached[1].device != self.x_r.device:
-                m = torch.cat([self.x_r, self.x_w, self.x_k, self.x_v, self.x_a, self.x_g], dim=0).reshape(6, C)
-                cached = (key, torch.nn.Parameter(m.detach().clone(), requires_grad=False))
+                m = torch.cat([self.x_r, self.x_w, self.x_k, self.x_v, self.x_a, self.x_g], dim=0).reshape(6, C).detach()
+                kept = None if cached is None else cached[1]
+                with torch.inference_mode(False), torch.no_grad():      # an ordinary tensor, with a version count
+                    if kept is not None and (kept.device, kept.dtype, kept.shape) == (m.device, m.dtype, m.shape):
+                        kept.copy_(m)             # in place: a captured decode step reads this memory
+                    else:
+                        kept = torch.nn.Parameter(m.clone(), requires_grad=False)
+                cached = (key, kept)
                 object.__setattr__(self, "_mix_cache", cached)
             return cached[1]
         return torch.cat([self.x_r, self.x_w, self.x_k, self.x_v, self.x_a, self.x_g], dim=0).reshape(6, C)

@@ -191,3 +191,22 @@ def test_loading_an_optimiser_state_reaches_cached_parameter_copies():
         master = eng.opt.master[:eng.space.numel].clone() + 1.0
         eng.opt.load_full_state(master, torch.zeros_like(master), torch.zeros_like(master), step=1)
         assert torch.equal(att.mix_matrix()[0], att.x_r.reshape(-1))
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_cached_mixing_coefficients_stay_where_they_are(inference):
+    """A captured decode step reads them: a change of the parameters refreshes the memory instead of replacing it."""
+    torch.manual_seed(0)
+    model = RWKV7Model(RWKVConfig(n_layer=2, n_embd=64, vocab_size=128, dim_att_lora=16, dim_gate_lora=16, dim_mv_lora=16))
+    att = model.blocks[1].att
+    with torch.inference_mode(inference), torch.no_grad():
+        kept = att.mix_matrix()
+    at, version = kept.data_ptr(), kept._version
+    for _ in range(3):
+        with torch.no_grad():
+            att.x_r.add_(1.0)
+        with torch.inference_mode(inference), torch.no_grad():
+            again = att.mix_matrix()
+        assert again._version > version                    # copies in other types follow the count
+        version = again._version
+        assert again is kept and again.data_ptr() == at and torch.equal(again[0], att.x_r.reshape(-1))
