@@ -36,6 +36,7 @@ class _DecodeGraph:
         from ..ops import cuda_ops
 
         self.gen, self.n = weakref.proxy(gen), n      # no cycle generator <-> graph: both die by reference count
+        self.packed = gen._packed_buffers()
         dev = gen.device
         self.tok = torch.zeros(n, 1, dtype=torch.long, device=dev)
         self.state = gen._zero_state(n)
@@ -105,7 +106,14 @@ class GRPOBatchGenerator:
         self.use_cuda_graph = (self.device.type == "cuda" and not sharded) if use_cuda_graph is None else use_cuda_graph
         self._graphs: Dict[int, _DecodeGraph] = {}
 
+    def _packed_buffers(self) -> tuple:
+        buffers = getattr(self.model, "packed_ffn_buffers", None)
+        return buffers() if buffers is not None else ()
+
     def _graph_for(self, n: int) -> "_DecodeGraph":
+        held, now = self._graphs.get(n), self._packed_buffers()
+        if held is not None and (len(held.packed) != len(now) or any(a is not b for a, b in zip(held.packed, now))):
+            del self._graphs[n]        # the feed-forward weights were packed, unpacked or packed elsewhere since
         if n not in self._graphs:
             if len(self._graphs) >= 6:
                 self._graphs.pop(next(iter(self._graphs)))

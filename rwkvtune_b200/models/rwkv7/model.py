@@ -577,6 +577,12 @@ class RWKV7Model(GenerationMixin, nn.Module):
             block.ffn.pack()
         return self
 
+    def packed_ffn_buffers(self) -> tuple:
+        """The memory that passes without autograd read their 8-bit feed-forward weights from; empty if they use none.  A
+        captured step is good for the buffers that it was captured with, and keeps them alive."""
+        held = [getattr(block.ffn, "_packed", None) for block in self.blocks]
+        return tuple(p.data for h in held if h is not None for p in h[1])
+
     def unpack_ffn(self) -> "RWKV7Model":
         for block in self.blocks:
             block.ffn.unpack()

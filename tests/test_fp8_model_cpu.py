@@ -320,3 +320,29 @@ def test_another_models_optimiser_leaves_a_packed_copy_valid():
     eng.train_step(ids, labels, 1e-3)
     with torch.no_grad():
         assert torch.equal(copied(ids), kept)
+
+
+def test_captured_steps_belong_to_the_packed_buffers(monkeypatch):
+    """A generator's captured step is taken again only while the model reads the same packed memory, and keeps that memory."""
+    from rwkvtune_b200.inference import grpo_batch_generator as module
+
+    class Step:
+        def __init__(self, gen, n):
+            self.packed = gen._packed_buffers()
+
+    monkeypatch.setattr(module, "_DecodeGraph", Step)
+    m = make().eval()
+    gen = module.GRPOBatchGenerator(m, None, torch.device("cpu"), eos_token_id=0)
+    plain = gen._graph_for(4)
+    assert gen._graph_for(4) is plain and plain.packed == ()
+    packed = m.pack_ffn() and gen._graph_for(4)
+    assert packed is not plain and len(packed.packed) == 4
+    m.pack_ffn()                                       # written again in place
+    assert gen._graph_for(4) is packed
+    m.blocks[1].ffn.unpack()
+    partly = gen._graph_for(4)
+    assert partly is not packed and len(partly.packed) == 2 and packed.packed[2].numel() > 0
+    m.unpack_ffn()
+    assert gen._graph_for(4).packed == ()
+    m.pack_ffn()                                       # other memory than the first time
+    assert gen._graph_for(4) is not packed

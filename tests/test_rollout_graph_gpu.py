@@ -51,3 +51,18 @@ def test_captured_steps_follow_the_optimiser():
     assert not torch.equal(seen[0], seen[1])
     torch.cuda.synchronize()
     assert gemm_native.check_status() == 0
+
+
+def test_captured_steps_follow_packing_and_unpacking():
+    m = make().eval()
+    captured, eager = generators(m)
+    seen = []
+    for change in (lambda: None, m.pack_ffn, m.pack_ffn, m.unpack_ffn, m.pack_ffn):
+        change()
+        torch.cuda.empty_cache()
+        a, b = tokens(captured), tokens(eager)
+        assert torch.equal(a, b)
+        seen.append(a)
+    assert torch.equal(seen[0], seen[3]) and torch.equal(seen[1], seen[2]) and torch.equal(seen[1], seen[4])
+    torch.cuda.synchronize()
+    assert gemm_native.check_status() == 0
