@@ -10,8 +10,8 @@
 // The tokens come either in bf16 - then each CTA packs its part of the contraction itself, row by row, into the
 // shared-memory tiles the tensor core reads, which saves a launch and a round trip - or already packed, fetched by TMA in
 // the same ring as the weights.  Packing in the kernel repeats the work in every CTA: it is used up to 16 rows (feed-forward
-// half of 2048 channels, packed in the kernel and by a launch before it: 32 rows 14.7 and 13.4 us, 64 rows 20.0 and 15.8;
-// one row 12.0 and 14.2).
+// half of 2048 channels, weights in L2, packed in the kernel and by a launch before it: 32 rows 14.7 and 13.4 us, 64 rows 20.0
+// and 15.8; one row 12.0 and 14.2).
 //
 // Epilogues: store bf16, add a bf16 residual, or relu(y)^2 packed again: a CTA owns exactly one block of 128 columns of
 // every token, so a block's scale is a maximum over one warp.
@@ -21,9 +21,10 @@
 // barrier for that: in front of it, it held back the weight stream too (feed-forward half of one row, chained, weights from
 // HBM: 12.9 us, behind it 11.9; 8 rows 13.1 and 12.4).
 //
-// Back to back in a graph: 2048 -> 2048 for one row 6.0 us (4 MB: latency, 4700 cycles of it between the first instruction
-// and the accumulator), 4096 -> 16384 11.6 us (5.8 TB/s), the head 2048 -> 65536 24.4 us for one row (5.5 TB/s) and 27.9 for
-// 64 (4.8 TB/s); a feed-forward half of 2048 channels 12.0 us for one row, 15.8 for 64.
+// Back to back in a graph that cycles through more weights than L2 holds, as the blocks of a decode step do: 2048 -> 2048 for
+// one row 7.4 us (4 MB: latency, 4700 cycles of it between the first instruction and the accumulator), the head 2048 -> 65536
+// 25.9 us for one row (5.2 TB/s) and 30.5 with the packing launch for 64 (4.4 TB/s); a feed-forward half of 2048 channels 14.1
+// us for one row (2.4 TB/s), 19.5 for 64.  The same half on one pair of weights, which then lies in L2: 12.4 and 16.1 us.
 //
 // Shared memory is at least 112 KB per CTA, so an SM holds at most two of these, and with 256 columns of tensor memory each
 // they never wait for one another's allocation (CTAs of different clusters that did could wait in a circle).

@@ -569,10 +569,11 @@ class RWKV7Model(GenerationMixin, nn.Module):
     # ------------------------------------------------------------------ 8-bit feed-forward weights for inference
     def pack_ffn(self) -> "RWKV7Model":
         """Hold every block's feed-forward weights in 8 bits as well (half their bf16 size again): passes without autograd -
-        decoding, prefill, evaluation - then run those products in 8 bits.  A token is stored in 8 bits on
-        its own; what else is in the batch matters only as the order of sums does (see ``ops.fp8``).  Call it again after changing or moving the weights (captured decode graphs then follow); a stale copy is
-        refused outside of replays.  Writes into ``weight.data`` itself (``weight.data.mul_(2)``) leave no trace that could be
-        checked: write under ``torch.no_grad()``, or pack again."""
+        decoding, prefill, evaluation - then run those products in 8 bits.  A token is stored in 8 bits on its own; what else
+        is in the batch matters only as the order of sums does (see ``ops.fp8``).  Call it again after changing or moving
+        the weights (captured decode graphs then follow); a stale copy is refused outside of replays.  Writes into
+        ``weight.data`` itself (``weight.data.mul_(2)``) leave no trace that could be checked: write under
+        ``torch.no_grad()``, or pack again."""
         for block in self.blocks:
             block.ffn.pack()
         return self
