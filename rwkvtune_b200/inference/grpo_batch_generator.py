@@ -111,9 +111,10 @@ class GRPOBatchGenerator:
         return buffers() if buffers is not None else ()
 
     def _graph_for(self, n: int) -> "_DecodeGraph":
-        held, now = self._graphs.get(n), self._packed_buffers()
-        if held is not None and (len(held.packed) != len(now) or any(a is not b for a, b in zip(held.packed, now))):
-            del self._graphs[n]        # the feed-forward weights were packed, unpacked or packed elsewhere since
+        now = self._packed_buffers()
+        for size, g in list(self._graphs.items()):      # the feed-forward weights were packed, unpacked or packed elsewhere since
+            if len(g.packed) != len(now) or any(a is not b for a, b in zip(g.packed, now)):
+                del self._graphs[size]
         if n not in self._graphs:
             if len(self._graphs) >= 6:
                 self._graphs.pop(next(iter(self._graphs)))

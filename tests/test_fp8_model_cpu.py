@@ -333,10 +333,11 @@ def test_captured_steps_belong_to_the_packed_buffers(monkeypatch):
     monkeypatch.setattr(module, "_DecodeGraph", Step)
     m = make().eval()
     gen = module.GRPOBatchGenerator(m, None, torch.device("cpu"), eos_token_id=0)
+    gen._graph_for(2)
     plain = gen._graph_for(4)
     assert gen._graph_for(4) is plain and plain.packed == ()
     packed = m.pack_ffn() and gen._graph_for(4)
-    assert packed is not plain and len(packed.packed) == 4
+    assert packed is not plain and len(packed.packed) == 4 and list(gen._graphs) == [4]
     m.pack_ffn()                                       # written again in place
     assert gen._graph_for(4) is packed
     m.blocks[1].ffn.unpack()
