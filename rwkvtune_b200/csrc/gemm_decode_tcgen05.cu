@@ -517,3 +517,8 @@ RWKV_EXPORT int rwkv_set_launch_chaining(int on) {
   rwkv_chain() = {on != 0, false, nullptr};
   return prev;
 }
+// The calling thread's next launch is an ordinary one: something that chained kernels read before they wait has been rewritten.
+RWKV_EXPORT int rwkv_restart_launch_chain() {
+  rwkv_chain_restart();
+  return RWKV_OK;
+}

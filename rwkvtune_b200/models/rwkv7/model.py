@@ -191,6 +191,7 @@ class RWKV7TimeMix(nn.Module):
                         kept.copy_(m)             # in place: a captured decode step reads this memory
                     else:
                         kept = torch.nn.Parameter(m.clone(), requires_grad=False)
+                ops.restart_chain()
                 cached = (key, kept)
                 object.__setattr__(self, "_mix_cache", cached)
             return cached[1]

@@ -68,6 +68,13 @@ def bump_param_epoch(counted: bool = False) -> None:
         pass
 
 
+def restart_chain() -> None:
+    """See ``_ext.restart_chain``."""
+    from . import _ext
+
+    _ext.restart_chain()
+
+
 def set_kernel_enabled(name: str, enabled: bool) -> None:
     if name not in _KERNELS:
         raise KeyError(f"unknown kernel family {name!r}; known: {sorted(_KERNELS)}")

@@ -151,8 +151,8 @@ def launch_chaining():
     """Inside this context the kernels of the decode path are launched as a programmatic dependent chain: each may be
     scheduled while its predecessor still runs and waits on the device for it before touching activations (see
     ``csrc/common.cuh``).  The decode GEMM additionally streams its first weight tiles before that wait, so the
-    context must not enclose anything that writes model weights (but for ``ops.pack_fp8``, whose launch the next one waits
-    for).  Other threads launch as before.  ``RWKVTUNE_CHAINED_LAUNCH=0`` turns it off."""
+    context must not enclose anything that writes model weights, but for what restarts the chain: ``ops.pack_fp8`` and the
+    cached copies of small parameters (:func:`restart_chain`).  Other threads launch as before.  ``RWKVTUNE_CHAINED_LAUNCH=0`` turns it off."""
     if not (CHAINING_ALLOWED and available() and hasattr(lib(), "rwkv_set_launch_chaining")) or _CHAIN.on:
         yield
         return
@@ -163,6 +163,13 @@ def launch_chaining():
     finally:
         lib().rwkv_set_launch_chaining(ctypes.c_int(0))
         _CHAIN.on = False
+
+
+def restart_chain() -> None:
+    """After a rewrite of something that chained kernels read before they wait (cached copies of parameters): the next launch
+    waits for it like any other.  Nothing to do outside of a chain."""
+    if _CHAIN.on:
+        lib().rwkv_restart_launch_chain()
 
 
 def i32(v: int) -> ctypes.c_int:

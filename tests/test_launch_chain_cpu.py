@@ -82,3 +82,39 @@ def test_size_caches_are_bounded(monkeypatch):
     finally:
         for c in caches:
             c.cache_clear()
+
+
+def test_refreshed_copies_of_parameters_restart_the_chain(monkeypatch):
+    """Chained kernels read parameters before they wait; a copy that is made inside the chain has to be waited for."""
+    import torch
+
+    from rwkvtune_b200 import ops
+    from rwkvtune_b200.models import RWKV7Model, RWKVConfig
+    from rwkvtune_b200.ops import cuda_ops
+
+    class Library(Recorder):
+        restarts = 0
+
+        def rwkv_restart_launch_chain(self):
+            self.restarts += 1
+
+    fake = Library()
+    monkeypatch.setattr(_ext, "available", lambda: True)
+    monkeypatch.setattr(_ext, "lib", lambda: fake)
+    monkeypatch.setattr(_ext, "CHAINING_ALLOWED", True)
+    p = torch.nn.Parameter(torch.randn(16).to(torch.bfloat16))
+    att = RWKV7Model(RWKVConfig(n_layer=1, n_embd=64, vocab_size=16, dim_att_lora=16, dim_gate_lora=16, dim_mv_lora=16)).blocks[0].att
+    with torch.no_grad():
+        cuda_ops._f32(p), att.mix_matrix()
+        assert fake.restarts == 0                       # outside of a chain there is nothing to restart
+        with _ext.launch_chaining():
+            for expected, touched in ((0, ()), (1, (p,)), (2, (att.x_r,)), (4, (p, att.x_k)), (4, ())):
+                for t in touched:
+                    t.add_(1)
+                cuda_ops._f32(p), att.mix_matrix()
+                assert fake.restarts == expected
+            ops.bump_param_epoch()
+            cuda_ops._f32(p), att.mix_matrix()
+            assert fake.restarts == 6
+            cuda_ops._f32(torch.nn.Parameter(torch.randn(16).to(torch.bfloat16)))
+            assert fake.restarts == 7
